@@ -492,6 +492,35 @@ int retro_b200_op_gemm_mxfp4_grouped(const uint8_t * banks, uint32_t n_expert, u
 int retro_b200_gemm_q4k_noalloc(const uint8_t * d_w, uint32_t n_out, uint32_t n_in, const float * d_x, uint32_t n_tokens, float * d_y,
                                 void * stream);
 
+/* ---- products with 4-bit weights for few tokens (no counterpart in the reference) ----
+ * For decode steps of a few tokens, where a product is a stream of the weights. Two stored formats, as GGUF rows: Q4_0 (2: f16 scale
+ * per 32 weights, 18 bytes) and MXFP4 (39: E8M0 scale per 32, 17 bytes).
+ *
+ * retro_b200_w4_new lays `rows` ([n_expert][n_out][n_in / 32 blocks], host or device memory, read before the call returns) out on
+ * the current device, in about the same number of bytes; n_expert is 1 for a plain matrix. NULL and a message when the type is another one,
+ * n_in is no multiple of 32 or above 262144, n_expert is above 256, or an MXFP4 scale is above 2^96. The handle is immutable: calls
+ * from several threads and streams may use it at once. Free it when no call that uses it is pending.
+ *
+ * The calls below take DEVICE pointers on the handle's device, whichever device is current, enqueue on `stream` (a cudaStream_t of that device,
+ * or NULL) and do not wait, allocate or synchronise, so they may be captured into a CUDA graph. Element types: f32 (0), f16 (1), bf16 (30); x and y choose their own, a residual has
+ * y's. Row strides are in elements and free (x's may be 0). Vectors (norm, bias) and the router are f32. Any number of tokens: sixteen per
+ * pass over the weights. Sums are f32 of exact products with the activations at 22 bits or more; results do not depend on the other tokens' values and are
+ * the same in every run. A token that holds an infinity or a NaN gets NaN or infinity, the other tokens are not affected.
+ * -3 and a message, with nothing enqueued, for a missing or misaligned pointer, another type, a y row stride below a row, and a y that overlaps an input
+ * (except a residual that is y itself: in place).
+ *
+ * w4_matvec: y[t] = W xn[t] + bias + residual[t], where xn = x, or with d_norm x / sqrt(mean(x^2) + eps) * norm.
+ * w4_glu:    y[t] = silu(Wgate xn[t]) * (Wup xn[t]), silu(a) = a / (1 + exp(-a)); the matrices have one type and shape. */
+typedef struct retro_b200_w4 retro_b200_w4;
+retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_t n_out, uint32_t n_in, uint32_t n_expert);
+void retro_b200_w4_free(retro_b200_w4 * w);
+/* Type, {n_expert, n_out, n_in}, device bytes and device of a handle; NULL skips one. */
+int retro_b200_w4_info(const retro_b200_w4 * w, uint32_t * out_type, uint32_t * out_shape_3, uint64_t * out_bytes, int * out_device);
+int retro_b200_w4_matvec(const retro_b200_w4 * w, const void * d_x, uint32_t x_type, int64_t ld_x, uint32_t n_tokens, const float * d_norm, float eps,
+                         const float * d_bias, const void * d_residual, int64_t ld_residual, void * d_y, uint32_t y_type, int64_t ld_y, void * stream);
+int retro_b200_w4_glu(const retro_b200_w4 * gate, const retro_b200_w4 * up, const void * d_x, uint32_t x_type, int64_t ld_x, uint32_t n_tokens,
+                      const float * d_norm, float eps, void * d_y, uint32_t y_type, int64_t ld_y, void * stream);
+
 /* Expert parallelism for mixture-of-experts models (the reference runs them on one GPU only:
  * src/runtime/retro_experts.cpp:86-140 places expert banks on a single device). One engine per GPU;
  * expert e is served by rank e / (n_expert / world). Rank 0 creates the 128-byte NCCL id, every rank

@@ -33,6 +33,7 @@ from .engine import (
     recode_mxfp4_as_q8_0,
     synth_gguf,
 )
+from .w4 import W4Matrix, w4_glu, w4_matvec
 
 __all__ = [
     "ADAPTER_BASE",
@@ -51,6 +52,7 @@ __all__ = [
     "StepOutput",
     "StepRow",
     "TrainerGeneration",
+    "W4Matrix",
     "ep_plan",
     "grammar_check",
     "load_library",
@@ -61,4 +63,6 @@ __all__ = [
     "quantize_row",
     "recode_mxfp4_as_q8_0",
     "synth_gguf",
+    "w4_glu",
+    "w4_matvec",
 ]

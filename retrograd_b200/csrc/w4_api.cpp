@@ -1,0 +1,172 @@
+// C entry points of the products with 4-bit weights (include/retro_b200.h, "products with 4-bit weights"): argument checks,
+// the weight handle, and the switch to the handle's device. The kernels are in w4.cu.
+
+#include "common.hpp"
+#include "blocks.hpp"
+#include "kernels.cuh"
+#include "w4.cuh"
+#include "w4_checks.hpp"
+
+#include "../../include/retro_b200.h"
+
+#include <memory>
+
+using namespace rb200;
+
+struct retro_b200_w4 {
+    W4View view;
+    int device = 0;
+    uint8_t * units = nullptr;
+    size_t bytes = 0;
+    ~retro_b200_w4() { if (units) cudaFree(units); }
+};
+
+namespace {
+
+// Makes `device` current for the call and puts the caller's back.
+class DeviceScope {
+public:
+    explicit DeviceScope(int device) {
+        RB_CUDA(cudaGetDevice(&before_));
+        if (before_ != device) {
+            RB_CUDA(cudaSetDevice(device));
+            switched_ = true;
+        }
+    }
+    ~DeviceScope() { if (switched_) cudaSetDevice(before_); }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope & operator=(const DeviceScope &) = delete;
+
+private:
+    int before_ = 0;
+    bool switched_ = false;
+};
+
+int refuse(const char * op, const std::string & why) {
+    set_error(std::string(op) + ": " + why);
+    return STATUS_INVALID_ARGUMENT;
+}
+
+int launched(const char * op, cudaError_t status) {
+    if (status == cudaSuccess) status = cudaGetLastError();
+    else cudaGetLastError();
+    if (status == cudaSuccess) return STATUS_OK;
+    set_error(std::string(op) + ": launch failed: " + cudaGetErrorString(status));
+    return STATUS_RUNTIME;
+}
+
+int product(const char * op, const retro_b200_w4 * w, const retro_b200_w4 * up, const void * d_x, uint32_t x_type, int64_t ld_x, uint32_t n_tokens,
+            const float * d_norm, float eps, const float * d_bias, const void * d_residual, int64_t ld_residual, void * d_y, uint32_t y_type, int64_t ld_y,
+            void * stream) {
+    return boundary([&]() -> int {
+        if (!w) return refuse(op, "a weight handle is required");
+        if (w->view.n_expert != 1) return refuse(op, "the handle holds a bank of experts");
+        if (up) {
+            if (up->view.n_expert != 1) return refuse(op, "the handle holds a bank of experts");
+            if (up->view.type != w->view.type || up->view.n_out != w->view.n_out || up->view.n_in != w->view.n_in)
+                return refuse(op, "gate and up must have one type and shape");
+            if (up->device != w->device) return refuse(op, "gate and up are on different devices");
+        }
+        const w4::ProductShape shape{n_tokens, w->view.n_in, w->view.n_out};
+        const w4::Rows x{"x", d_x, x_type, ld_x}, y{"y", d_y, y_type, ld_y}, residual{"residual", d_residual, y_type, ld_residual};
+        const std::string why = w4::check_product(shape, x, y, residual, d_norm, eps, d_bias);
+        if (!why.empty()) return refuse(op, why);
+        if (n_tokens == 0) return STATUS_OK;
+        const DeviceScope scope(w->device);
+        W4Product p;
+        p.w = w->view;
+        p.up = up ? &up->view : nullptr;
+        p.x = d_x;
+        p.x_type = x_type;
+        p.ld_x = ld_x;
+        p.n_tokens = (int)n_tokens;
+        p.norm = d_norm;
+        p.eps = eps;
+        p.bias = d_bias;
+        p.residual = d_residual;
+        p.ld_residual = ld_residual;
+        p.y = d_y;
+        p.y_type = y_type;
+        p.ld_y = ld_y;
+        return launched(op, launch_w4_product(p, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+} // namespace
+
+extern "C" {
+
+retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_t n_out, uint32_t n_in, uint32_t n_expert) {
+    retro_b200_w4 * made = nullptr;
+    boundary([&]() -> int {
+        const char * op = "w4_new";
+        if (ggml_type != GGML_Q4_0 && ggml_type != GGML_MXFP4) return refuse(op, "the weights must be Q4_0 (2) or MXFP4 (39)");
+        if (!rows) return refuse(op, "rows are required");
+        if (n_out == 0 || n_in == 0 || n_in % 32 != 0) return refuse(op, "n_out must be at least 1 and n_in a multiple of 32");
+        if (n_in > kW4MaxColumns) return refuse(op, "n_in is larger than 262144");
+        if (n_expert == 0 || n_expert > kW4MaxExperts) return refuse(op, "n_expert must be 1 to 256");
+        if ((uint64_t)n_expert * (((uint64_t)n_out + 15) / 16) * ((n_in + 63) / 64) > 0x7fffffffull) return refuse(op, "the bank is too large");
+        auto w = std::make_unique<retro_b200_w4>();
+        RB_CUDA(cudaGetDevice(&w->device));
+        w->bytes = w4_bytes(ggml_type, n_out, n_in, n_expert);
+        RB_CUDA(cudaMalloc(&w->units, w->bytes));
+        w->view = w4_view(w->units, ggml_type, n_out, n_in, n_expert);
+        // The stored rows, once, in device memory whatever kind of memory they come from.
+        const size_t n_raw = (size_t)n_expert * n_out * (n_in / 32) * (ggml_type == GGML_Q4_0 ? 18 : 17);
+        struct Raw { uint8_t * p = nullptr; cudaStream_t s = nullptr; ~Raw() { if (p) cudaFree(p); if (s) cudaStreamDestroy(s); } } raw;
+        RB_CUDA(cudaMalloc(&raw.p, n_raw + 256));
+        RB_CUDA(cudaStreamCreateWithFlags(&raw.s, cudaStreamNonBlocking));
+        int * d_max = reinterpret_cast<int *>(raw.p + (n_raw + 15) / 16 * 16);
+        RB_CUDA(cudaDeviceSynchronize());       // device rows that another stream is still writing
+        RB_CUDA(cudaMemcpy(raw.p, rows, n_raw, cudaMemcpyDefault));
+        RB_CUDA(cudaDeviceSynchronize());       // the blocking copy has reached the device before another stream reads it
+        RB_CUDA(cudaMemsetAsync(d_max, 0, sizeof(int), raw.s));
+        launch_w4_retile(raw.p, ggml_type, n_out, n_in, n_expert, w->units, d_max, raw.s);
+        RB_CUDA(cudaGetLastError());
+        int h_max = 0;
+        RB_CUDA(cudaMemcpyAsync(&h_max, d_max, sizeof h_max, cudaMemcpyDeviceToHost, raw.s));
+        RB_CUDA(cudaStreamSynchronize(raw.s));
+        if (h_max > (int)kW4MaxScaleByte) return refuse(op, "an MXFP4 scale byte is above 223 (2^96)");
+        made = w.release();
+        return STATUS_OK;
+    });
+    return made;
+}
+
+void retro_b200_w4_free(retro_b200_w4 * w) {
+    if (!w) return;
+    boundary([&]() -> int {
+        std::unique_ptr<retro_b200_w4> owned(w);
+        const DeviceScope scope(w->device);
+        owned.reset();
+        return STATUS_OK;
+    });
+}
+
+int retro_b200_w4_info(const retro_b200_w4 * w, uint32_t * out_type, uint32_t * out_shape_3, uint64_t * out_bytes, int * out_device) {
+    return boundary([&]() -> int {
+        if (!w) return refuse("w4_info", "a weight handle is required");
+        if (out_type) *out_type = w->view.type;
+        if (out_shape_3) {
+            out_shape_3[0] = w->view.n_expert;
+            out_shape_3[1] = w->view.n_out;
+            out_shape_3[2] = w->view.n_in;
+        }
+        if (out_bytes) *out_bytes = w->bytes;
+        if (out_device) *out_device = w->device;
+        return STATUS_OK;
+    });
+}
+
+int retro_b200_w4_matvec(const retro_b200_w4 * w, const void * d_x, uint32_t x_type, int64_t ld_x, uint32_t n_tokens, const float * d_norm, float eps,
+                         const float * d_bias, const void * d_residual, int64_t ld_residual, void * d_y, uint32_t y_type, int64_t ld_y, void * stream) {
+    return product("w4_matvec", w, nullptr, d_x, x_type, ld_x, n_tokens, d_norm, eps, d_bias, d_residual, ld_residual, d_y, y_type, ld_y, stream);
+}
+
+int retro_b200_w4_glu(const retro_b200_w4 * gate, const retro_b200_w4 * up, const void * d_x, uint32_t x_type, int64_t ld_x, uint32_t n_tokens,
+                      const float * d_norm, float eps, void * d_y, uint32_t y_type, int64_t ld_y, void * stream) {
+    if (!up) return boundary([&]() -> int { return refuse("w4_glu", "a weight handle is required"); });
+    return product("w4_glu", gate, up, d_x, x_type, ld_x, n_tokens, d_norm, eps, nullptr, nullptr, 0, d_y, y_type, ld_y, stream);
+}
+
+} // extern "C"
