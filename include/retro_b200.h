@@ -520,6 +520,19 @@ int retro_b200_w4_matvec(const retro_b200_w4 * w, const void * d_x, uint32_t x_t
                          const float * d_bias, const void * d_residual, int64_t ld_residual, void * d_y, uint32_t y_type, int64_t ld_y, void * stream);
 int retro_b200_w4_glu(const retro_b200_w4 * gate, const retro_b200_w4 * up, const void * d_x, uint32_t x_type, int64_t ld_x, uint32_t n_tokens,
                       const float * d_norm, float eps, void * d_y, uint32_t y_type, int64_t ld_y, void * stream);
+/* A mixture-of-experts layer (the graph's: softmax over all experts, the n_used likeliest, ties to the lowest id; `normalise` divides their
+ * probabilities by their sum), in two kernels per sixteen tokens:
+ *   y[t] = residual[t] + sum over t's experts e of w_e Wdown_e (silu(Wgate_e xn[t]) * (Wup_e xn[t])),  logits = router xn[t]
+ * router is f32 [n_expert][n_in of gate], 1 <= n_used <= min(n_expert, 32); down may be of the other stored format. y may be x itself or the residual. d_ids and d_weights, when
+ * not NULL, receive [n_tokens][n_used] chosen experts, likeliest first, and their w_e. A token whose logits hold a NaN still chooses n_used
+ * experts, with weights NaN. d_workspace (16-byte aligned, at least retro_b200_w4_moe_workspace bytes; -3 otherwise) is
+ * the call's alone until its work is done: calls that may run at the same time, two captured graphs among them, need
+ * one each. Nothing in it has to be initialised or is kept. */
+int retro_b200_w4_moe_workspace(const retro_b200_w4 * gate, uint32_t n_tokens, uint32_t n_used, size_t * out_bytes);
+int retro_b200_w4_moe(const float * d_router, const retro_b200_w4 * gate, const retro_b200_w4 * up, const retro_b200_w4 * down, const void * d_x,
+                      uint32_t x_type, int64_t ld_x, uint32_t n_tokens, uint32_t n_used, int normalise, const float * d_norm, float eps,
+                      const void * d_residual, int64_t ld_residual, void * d_y, uint32_t y_type, int64_t ld_y, int32_t * d_ids, float * d_weights,
+                      void * d_workspace, size_t workspace_bytes, void * stream);
 
 /* Expert parallelism for mixture-of-experts models (the reference runs them on one GPU only:
  * src/runtime/retro_experts.cpp:86-140 places expert banks on a single device). One engine per GPU;

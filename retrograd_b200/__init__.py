@@ -33,7 +33,7 @@ from .engine import (
     recode_mxfp4_as_q8_0,
     synth_gguf,
 )
-from .w4 import W4Matrix, w4_glu, w4_matvec
+from .w4 import W4Matrix, w4_glu, w4_matvec, w4_moe, w4_moe_workspace
 
 __all__ = [
     "ADAPTER_BASE",
@@ -65,4 +65,6 @@ __all__ = [
     "synth_gguf",
     "w4_glu",
     "w4_matvec",
+    "w4_moe",
+    "w4_moe_workspace",
 ]

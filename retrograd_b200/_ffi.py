@@ -272,6 +272,10 @@ SYMBOLS = {
                                        C.c_void_p, C.c_uint32, C.c_int64, C.c_void_p]),
     "retro_b200_w4_glu": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_int64, C.c_uint32, C.c_void_p, C.c_float, C.c_void_p, C.c_uint32,
                                     C.c_int64, C.c_void_p]),
+    "retro_b200_w4_moe_workspace": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, _P(C.c_size_t)]),
+    "retro_b200_w4_moe": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_int64, C.c_uint32, C.c_uint32, C.c_int,
+                                    C.c_void_p, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_uint32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_size_t, C.c_void_p]),
     "retro_b200_engine_last_step_io": (C.c_int, [C.c_void_p, _P(C.c_uint64), _P(C.c_uint64)]),
     "retro_b200_grammar_check": (C.c_int, [C.c_char_p, C.c_char_p, _P(C.c_int)]),
     "retro_b200_checked_build": (C.c_int, []),

@@ -449,14 +449,9 @@ struct Stream {
 #pragma unroll
             for (int d = 0; d < kDepth; ++d) {
                 if (cp.item >= n_items) break;
-                if constexpr (MODES == (1 << PACK)) do_step<MX, PARTS, PACK>(buf[d], l, lane, acc);
-                else if constexpr (MODES == (1 << ONE)) do_step<MX, PARTS, ONE>(buf[d], l, lane, acc);
-                else if constexpr (MODES == (1 << TWO)) do_step<MX, PARTS, TWO>(buf[d], l, lane, acc);
-                else {
-                    if ((MODES & (1 << PACK)) && mode == PACK) do_step<MX, PARTS, PACK>(buf[d], l, lane, acc);
-                    else if (mode == ONE) do_step<MX, PARTS, ONE>(buf[d], l, lane, acc);
-                    else do_step<MX, PARTS, TWO>(buf[d], l, lane, acc);
-                }
+                if constexpr (MODES & (1 << PACK)) if (MODES == (1 << PACK) || mode == PACK) do_step<MX, PARTS, PACK>(buf[d], l, lane, acc);
+                if constexpr (MODES & (1 << ONE)) if (MODES == (1 << ONE) || mode == ONE) do_step<MX, PARTS, ONE>(buf[d], l, lane, acc);
+                if constexpr (MODES & (1 << TWO)) if (MODES == (1 << TWO) || mode == TWO) do_step<MX, PARTS, TWO>(buf[d], l, lane, acc);
                 fetch(d);
                 if (--cp.rem == 0) {
                     end_run(mode, r.n, lane, acc, [&](int row, int col, float v) { src.put(cp.item, cp.seg, row, col, v); });
@@ -605,6 +600,420 @@ __global__ void __launch_bounds__(kThreads, 2) w4_product_kernel(ProductArgs a) 
     }
 }
 
+// ---- a mixture-of-experts layer
+//
+// Two kernels. The first: every cluster normalises and routes all tokens for itself (the router is a few hundred
+// kilobytes that the L2 cache holds; one CTA reads an eighth of it) instead of waiting for one place to do it, then multiplies its share of the chosen
+// experts' (gate tile, up tile) pairs and writes h = w_e silu(a) b for each (token, expert) pair. The second treats the chosen
+// experts' down matrices as one long reduction: a cluster owns a range of y's rows, its CTAs divide the experts' concatenated columns,
+// and the sum over experts is part of the sum over the cluster.
+
+struct MoeMeta {                        // in the workspace, in front of h
+    int32_t n;                          // chosen experts
+    int32_t pad[3];
+    uint16_t expert[kW4MaxExperts];     // ascending
+    uint16_t count[kW4MaxExperts];      // their tokens
+    uint16_t pair[kW4MaxExperts][kRowList];     // token * n_used + rank of the expert among the token's
+};
+
+struct MoeArgs {
+    const uint8_t * gate, * up, * down;
+    size_t gate_expert, up_expert, down_expert;     // bytes of one expert
+    const float * router;
+    Act x;
+    int T, E, k, d, ff;
+    int tiles_ff, steps_d, tiles_d, steps_ff;
+    bool normalise;
+    const float * norm;
+    float eps;
+    const void * residual;
+    int64_t ld_residual;
+    void * y;
+    uint32_t y_type;
+    int64_t ld_y;
+    int32_t * ids;
+    float * weights;
+    MoeMeta * meta;
+    float * h;
+    int64_t ld_h;
+    int clusters, x_bytes, c_bytes, logit_bytes, partial_floats;
+};
+
+struct Picks {
+    uint16_t expert[kRowList * kW4MaxUsed];
+    float weight[kRowList * kW4MaxUsed];
+    float rstd[kRowList];
+    uint16_t unique[kW4MaxExperts];
+    uint8_t count[kW4MaxExperts];                   // of unique[i]
+    uint8_t token[kW4MaxExperts][kRowList];
+    int warp_unique[kWarps];
+    int n, most;                                    // unique experts, largest count
+};
+
+// The CTA's columns' part of every (token, expert) logit.
+__device__ void partial_logits(const MoeArgs & a, int k0, int k1, float * out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int EB = 4, TB = 4;       // experts and tokens a warp takes at once
+    const Act router{a.router, a.d, GGML_F32, (uintptr_t)a.router % 16 == 0};
+    for (int e0 = warp * EB; e0 < a.E; e0 += kWarps * EB) {
+        for (int t0 = 0; t0 < a.T; t0 += TB) {
+            float acc[EB][TB] = {};
+            for (int k = k0 + lane * 4; k < k1; k += 128) {
+                float g[4] = {1.f, 1.f, 1.f, 1.f};
+                if (a.norm) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) g[i] = a.norm[k + i];
+                }
+                float r[EB][4];
+#pragma unroll
+                for (int e = 0; e < EB; ++e) load4(router, min(e0 + e, a.E - 1), k, r[e]);
+#pragma unroll
+                for (int t = 0; t < TB; ++t) {
+                    if (t0 + t >= a.T) break;
+                    float v[4];
+                    load4(a.x, t0 + t, k, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = v[i] * g[i];
+#pragma unroll
+                        for (int e = 0; e < EB; ++e) acc[e][t] += r[e][i] * f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                if (t0 + t >= a.T) break;
+#pragma unroll
+                for (int e = 0; e < EB; ++e) {
+                    float v = acc[e][t];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (lane == 0 && e0 + e < a.E) out[(t0 + t) * a.E + e0 + e] = v;
+                }
+            }
+        }
+    }
+}
+
+// Softmax over the experts and the n_used likeliest of one token, by one warp. Ties go to the lowest index; whatever the
+// logits hold, n_used different experts are chosen (a NaN makes the weights NaN).
+__device__ void pick_experts(const float * logits, int E, int k, bool normalise, uint16_t * expert, float * weight) {
+    const int lane = threadIdx.x & 31;
+    constexpr int PER = kW4MaxExperts / 32;
+    float p[PER];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = lane + 32 * j;
+        p[j] = e < E ? logits[e] : -INFINITY;
+        mx = fmaxf(mx, p[j]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        p[j] = lane + 32 * j < E ? expf(p[j] - mx) : 0.f;
+        sum += p[j];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    uint32_t taken = 0;
+    float chosen = 0.f;
+    for (int pick = 0; pick < k; ++pick) {
+        float best = -2.f, value = 0.f;
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = lane + 32 * j;
+            if (e >= E || (taken >> j & 1)) continue;
+            const float v = p[j] / sum;
+            const float key = v >= 0.f ? v : -1.f;      // NaN behind every number
+            if (key > best) { best = key; value = v; at = e; }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float ob = __shfl_xor_sync(0xffffffffu, best, o), ov = __shfl_xor_sync(0xffffffffu, value, o);
+            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+            if (ob > best || (ob == best && oa < at)) { best = ob; value = ov; at = oa; }
+        }
+        if ((at & 31) == lane) taken |= 1u << (at >> 5);
+        if (lane == 0) { expert[pick] = (uint16_t)at; weight[pick] = value; }
+        chosen += value;
+    }
+    if (normalise) {
+        __syncwarp();
+        for (int i = lane; i < k; i += 32) weight[i] /= chosen;
+    }
+}
+
+// The chosen experts in ascending order with their tokens, from the picks of all tokens.
+__device__ void group_picks(const MoeArgs & a, Picks & p, MoeMeta * meta) {
+    const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
+    uint32_t mask = 0;                  // tokens that chose expert e
+    if (e < a.E) {
+        for (int i = 0; i < a.T * a.k; ++i)
+            if (p.expert[i] == e) mask |= 1u << (i / a.k);
+    }
+    const uint32_t chosen = __ballot_sync(0xffffffffu, mask != 0);
+    if (lane == 0) p.warp_unique[warp] = __popc(chosen);
+    if (e == 0) p.most = 1;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += p.warp_unique[w];
+        all += p.warp_unique[w];
+    }
+    if (mask) {
+        const int u = before + __popc(chosen & ((1u << lane) - 1u));
+        const int n = __popc(mask);
+        p.unique[u] = (uint16_t)e;
+        p.count[u] = (uint8_t)n;
+        atomicMax(&p.most, n);
+        int at = 0;
+        for (uint32_t m = mask; m; m &= m - 1) p.token[u][at++] = (uint8_t)(__ffs(m) - 1);
+        if (meta) {
+            meta->expert[u] = (uint16_t)e;
+            meta->count[u] = (uint16_t)n;
+            for (int i = 0; i < n; ++i) {
+                const int t = p.token[u][i];
+                int j = 0;
+                while (j < a.k - 1 && p.expert[t * a.k + j] != e) ++j;
+                meta->pair[u][i] = (uint16_t)(t * a.k + j);
+            }
+        }
+    }
+    if (e == 0) {
+        p.n = all;
+        if (meta) meta->n = all;
+    }
+    __syncthreads();
+}
+
+template <bool MX, int PARTS> struct GateUpSource {
+    const MoeArgs & a;
+    const Picks & p;
+    Staged x;
+    float * partial;
+    const Scratch & sc;
+    int job0, s0, n_steps, ks, most;
+
+    __device__ __forceinline__ int len(int item, int) const {
+        const int sub = item % ks;
+        return part_begin(n_steps, sub + 1, ks) - part_begin(n_steps, sub, ks);
+    }
+    __device__ __forceinline__ Run run(int item, int) const {
+        const int job = job0 + item / ks, s = part_begin(n_steps, item % ks, ks);
+        const int u = job / a.tiles_ff, tile = job % a.tiles_ff;
+        const size_t at = ((size_t)tile * a.steps_d + s0 + s) * w4_unit_bytes(MX);
+        const int e = p.unique[u];
+        Run r;
+        r.p0 = a.gate + e * a.gate_expert + at;
+        r.p1 = a.up + e * a.up_expert + at;
+        r.x = {x.x + (size_t)s * (2 * PARTS * 64) * x.n, MX ? nullptr : x.c + (size_t)s * 2 * x.n, x.n};
+        r.list = p.token[u];
+        r.n = p.count[u];
+        return r;
+    }
+    __device__ __forceinline__ void put(int item, int, int row, int col, float v) const {
+        const int tok = p.token[(job0 + item / ks) / a.tiles_ff][col];
+        partial[((size_t)item * most + col) * kSlotCol + row] = v * sc.f1[0][tok] * sc.f2[0][tok];
+    }
+};
+
+template <bool MX, int PARTS, int MODES>
+__global__ void __launch_bounds__(kThreads, 2) w4_moe_gate_up_kernel(MoeArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Scratch sc;
+    __shared__ Picks picks;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), C = (int)cluster_size();
+    const int cluster = blockIdx.x / C;
+    const int s0 = part_begin(a.steps_d, rank, C), n_steps = part_begin(a.steps_d, rank + 1, C) - s0;
+    Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes), a.T};
+    float * mine = reinterpret_cast<float *>(smem + a.x_bytes + a.c_bytes);         // this CTA's part of the logits
+    float * logits = mine + a.logit_bytes / 4;
+    float * partial = logits + a.logit_bytes / 4;
+
+    pdl_trigger();
+    pdl_wait();
+    stage<MX, PARTS>(a.x, [](int t) { return (int64_t)t; }, a.T, s0 * 64, n_steps, a.d, a.norm, x, sc, 0);
+    partial_logits(a, s0 * 64, min(a.d, (s0 + n_steps) * 64), mine);
+    cluster_sync();
+    if (threadIdx.x < a.T) {
+        float ss = 0.f;
+        for (int c = 0; c < C; ++c) ss += remote_load(remote_address(smem_address(&sc.ss[threadIdx.x]), c));
+        picks.rstd[threadIdx.x] = a.norm ? rsqrtf(ss / (float)a.d + a.eps) : 1.f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.T * a.E; i += kThreads) {
+        float v = 0.f;
+        for (int c = 0; c < C; ++c) v += remote_load(remote_address(smem_address(mine), c) + i * 4);
+        logits[i] = v * picks.rstd[i / a.E];
+    }
+    __syncthreads();
+    for (int t = warp; t < a.T; t += kWarps) pick_experts(logits + t * a.E, a.E, a.k, a.normalise, picks.expert + t * a.k, picks.weight + t * a.k);
+    __syncthreads();
+    const bool first = blockIdx.x == 0;
+    group_picks(a, picks, first ? a.meta : nullptr);
+    if (first) {
+        for (int i = threadIdx.x; i < a.T * a.k; i += kThreads) {
+            if (a.ids) a.ids[i] = picks.expert[i];
+            if (a.weights) a.weights[i] = picks.weight[i];
+        }
+    }
+
+    const int total = picks.n * a.tiles_ff, most = picks.most;
+    const int j_begin = part_begin(total, cluster, a.clusters), j_end = part_begin(total, cluster + 1, a.clusters);
+    const int slots = a.partial_floats / (most * kSlotCol);
+    const int ks = min(split_columns(j_end - j_begin, a.steps_d / C), slots);
+    const int per_round = slots / ks;
+    for (int j0 = j_begin; j0 < j_end; j0 += per_round) {
+        const int jobs = min(per_round, j_end - j0);
+        GateUpSource<MX, PARTS> src{a, picks, x, partial, sc, j0, s0, n_steps, ks, most};
+        Stream<MX, PARTS, MODES, GateUpSource<MX, PARTS>> stream(src, jobs * ks, 1);
+        stream.prefetch();
+        stream.work();
+        cluster_sync();
+        const uint32_t base = smem_address(partial);
+        for (int i = rank + C * warp; i < jobs * most; i += C * kWarps) {
+            const int job = i / most, col = i % most;
+            const int u = (j0 + job) / a.tiles_ff, tile = (j0 + job) % a.tiles_ff;
+            if (col >= picks.count[u]) continue;
+            float v = 0.f;
+            for (int c = 0; c < C; ++c) {
+                const uint32_t at = remote_address(base, c) + (((size_t)job * ks * most + col) * kSlotCol + lane) * 4;
+                for (int s = 0; s < ks; ++s) v += remote_load(at + (uint32_t)(s * most * kSlotCol * 4));
+            }
+            const int t = picks.token[u][col];
+            v *= picks.rstd[t];
+            const float b = __shfl_down_sync(0xffffffffu, v, 16);
+            int j = 0;
+            while (j < a.k - 1 && picks.expert[t * a.k + j] != picks.unique[u]) ++j;
+            const int pair = t * a.k + j, row = tile * 16 + lane;
+            if (lane < 16 && row < a.ff) a.h[pair * a.ld_h + row] = picks.weight[pair] * (v / (1.f + expf(-v)) * b);
+        }
+        cluster_sync();
+    }
+    cluster_sync();     // nobody leaves while its logits are read
+}
+
+struct Seg {
+    int u, s0, len, x_off, c_off, n;
+};
+struct DownTable {
+    Seg seg[kMaxSegs];
+    int n;
+    int next;           // the step behind the chunk
+};
+
+template <bool MX> struct DownSource {
+    const MoeArgs & a;
+    const DownTable & table;
+    uint8_t * smem;
+    float * partial;
+    const Scratch & sc;
+    const uint8_t * identity;
+    int job0, ks;
+
+    __device__ __forceinline__ int len(int item, int seg) const {
+        const int n = table.seg[seg].len, sub = item % ks;
+        return part_begin(n, sub + 1, ks) - part_begin(n, sub, ks);
+    }
+    __device__ __forceinline__ Run run(int item, int seg) const {
+        const Seg & g = table.seg[seg];
+        const int job = job0 + item / ks, s = part_begin(g.len, item % ks, ks);
+        const uint8_t * e = a.down + a.meta->expert[g.u] * a.down_expert;
+        Run r;
+        r.p0 = e + ((size_t)(2 * job) * a.steps_ff + g.s0 + s) * w4_unit_bytes(MX);
+        r.p1 = e + ((size_t)min(2 * job + 1, a.tiles_d - 1) * a.steps_ff + g.s0 + s) * w4_unit_bytes(MX);
+        r.x = {smem + g.x_off + (size_t)s * (2 * 2 * 64) * g.n, MX ? nullptr : reinterpret_cast<float *>(smem + g.c_off) + (size_t)s * 2 * g.n, g.n};
+        r.list = identity;
+        r.n = g.n;
+        return r;
+    }
+    __device__ __forceinline__ void put(int item, int seg, int row, int col, float v) const {
+        const int tok = a.meta->pair[table.seg[seg].u][col] / a.k;
+        partial[((size_t)item * a.T + tok) * kSlotCol + row] += v * sc.f1[seg][col] * sc.f2[seg][col];
+    }
+};
+
+template <bool MX, int MODES>
+__global__ void __launch_bounds__(kThreads, 2) w4_moe_down_kernel(MoeArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Scratch sc;
+    __shared__ DownTable table;
+    __shared__ uint8_t identity[kRowList];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), C = (int)cluster_size();
+    const int cluster = blockIdx.x / C;
+    float * partial = reinterpret_cast<float *>(smem + a.x_bytes);
+    if (threadIdx.x < kRowList) identity[threadIdx.x] = (uint8_t)threadIdx.x;
+    pdl_trigger();
+    pdl_wait();
+    const int total = a.meta->n * a.steps_ff;       // the chosen experts' columns, one behind the other
+    const int begin = part_begin(total, rank, C), end = part_begin(total, rank + 1, C);
+    const int jobs_all = (a.tiles_d + 1) / 2;
+    const int j_begin = part_begin(jobs_all, cluster, a.clusters), j_end = part_begin(jobs_all, cluster + 1, a.clusters);
+    const int slots = a.partial_floats / (a.T * kSlotCol);
+    const int ks = min(split_columns(j_end - j_begin, max(1, total / C)), slots);
+    const int per_round = slots / ks;
+    const Act h{a.h, a.ld_h, GGML_F32, true};
+    for (int j0 = j_begin; j0 < j_end; j0 += per_round) {
+        const int jobs = min(per_round, j_end - j0);
+        for (int i = threadIdx.x; i < jobs * ks * a.T * kSlotCol; i += kThreads) partial[i] = 0.f;
+        for (int p = begin; p < end;) {
+            if (threadIdx.x == 0) {
+                // as many steps as fit into the shared memory for activations
+                int n = 0, used = 0, at = p;
+                while (at < end && n < kMaxSegs) {
+                    const int u = at / a.steps_ff, off = at % a.steps_ff, tokens = a.meta->count[u];
+                    const int each = staged_x_bytes(1, 2, tokens) + staged_c_bytes(MX, 1, tokens);
+                    const int len = min(min(a.steps_ff - off, end - at), (a.x_bytes - used - 16) / each);
+                    if (len <= 0) break;
+                    const int x_bytes = staged_x_bytes(len, 2, tokens);
+                    table.seg[n] = {u, off, len, used, used + x_bytes, tokens};
+                    used += (x_bytes + staged_c_bytes(MX, len, tokens) + 15) / 16 * 16;
+                    at += len;
+                    ++n;
+                }
+                table.n = n;
+                table.next = at;
+            }
+            __syncthreads();
+            DownSource<MX> src{a, table, smem, partial, sc, identity, j0, ks};
+            Stream<MX, 2, MODES, DownSource<MX>> stream(src, jobs * ks, table.n);
+            stream.prefetch();
+            for (int i = 0; i < table.n; ++i) {
+                const Seg & g = table.seg[i];
+                const uint16_t * pair = a.meta->pair[g.u];
+                stage<MX, 2>(h, [pair](int t) { return (int64_t)pair[t]; }, g.n, g.s0 * 64, g.len, a.ff, nullptr,
+                             Staged{smem + g.x_off, reinterpret_cast<float *>(smem + g.c_off), g.n}, sc, i);
+            }
+            __syncthreads();
+            stream.work();
+            p = table.next;
+            __syncthreads();
+        }
+        cluster_sync();
+        const uint32_t base = smem_address(partial);
+        for (int u = rank + C * warp; u < jobs * a.T; u += C * kWarps) {
+            const int job = u / a.T, t = u % a.T;
+            float v = 0.f;
+            for (int c = 0; c < C; ++c) {
+                const uint32_t at = remote_address(base, c) + (((size_t)job * ks * a.T + t) * kSlotCol + lane) * 4;
+                for (int i = 0; i < ks; ++i) v += remote_load(at + (uint32_t)(i * a.T * kSlotCol * 4));
+            }
+            const int row = (j0 + job) * 32 + lane;
+            if (row < a.d) {
+                if (a.residual) v += load1(Act{a.residual, a.ld_residual, a.y_type, false}, t, row);
+                store1(a.y, a.y_type, t * a.ld_y + row, v);
+            }
+        }
+        cluster_sync();
+    }
+}
+
 // ---- retiling
 //
 // Word j (0..3) of lane (g, t) holds row g + 8 (j & 1), columns 8 t + 4 s + 2 (j >> 1) + e of group h, for the products
@@ -723,6 +1132,43 @@ const void * row_at(const void * p, uint32_t type, int64_t ld, int64_t row) {
     return p ? static_cast<const uint8_t *>(p) + row * ld * (int64_t)type_bytes(type) : nullptr;
 }
 
+template <bool MX, int PARTS, int MODES> cudaError_t launch_gate_up(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
+    static PerDeviceOnce once;
+    if (once.first()) {
+        const cudaError_t e = cudaFuncSetAttribute(w4_moe_gate_up_kernel<MX, PARTS, MODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_cluster(w4_moe_gate_up_kernel<MX, PARTS, MODES>, a.clusters * C, C, smem, stream, a);
+}
+
+template <bool MX, int MODES> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
+    static PerDeviceOnce once;
+    if (once.first()) {
+        const cudaError_t e = cudaFuncSetAttribute(w4_moe_down_kernel<MX, MODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_cluster(w4_moe_down_kernel<MX, MODES>, a.clusters * C, C, smem, stream, a);
+}
+
+// The kernels are built for the modes that calls of up to 4, 8 and 16 tokens reach.
+template <bool MX> cudaError_t launch_gate_up_of(const MoeArgs & a, int parts, int C, size_t smem, cudaStream_t stream) {
+    if (parts == 2) {
+        if (a.T <= 4) return launch_gate_up<MX, 2, 1 << PACK>(a, C, smem, stream);
+        if (a.T <= 8) return launch_gate_up<MX, 2, 1 << PACK | 1 << ONE>(a, C, smem, stream);
+        return launch_gate_up<MX, 2, 1 << PACK | 1 << ONE | 1 << TWO>(a, C, smem, stream);
+    }
+    if (a.T <= 8) return launch_gate_up<MX, 1, 1 << ONE>(a, C, smem, stream);
+    return launch_gate_up<MX, 1, 1 << ONE | 1 << TWO>(a, C, smem, stream);
+}
+
+template <bool MX> cudaError_t launch_down_of(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
+    if (a.T <= 4) return launch_down<MX, 1 << PACK>(a, C, smem, stream);
+    if (a.T <= 8) return launch_down<MX, 1 << PACK | 1 << ONE>(a, C, smem, stream);
+    return launch_down<MX, 1 << PACK | 1 << ONE | 1 << TWO>(a, C, smem, stream);
+}
+
+int64_t moe_ld_h(uint32_t ff) { return ((int64_t)ff + 3) / 4 * 4; }
+
 } // namespace
 
 size_t w4_bytes(uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert) {
@@ -797,6 +1243,85 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         cudaError_t e;
         if (mx) e = glu ? launch_product_of<true, true>(a, parts, C, smem, stream) : launch_product_of<true, false>(a, parts, C, smem, stream);
         else e = glu ? launch_product_of<false, true>(a, parts, C, smem, stream) : launch_product_of<false, false>(a, parts, C, smem, stream);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+size_t w4_moe_workspace_bytes(uint32_t ff, uint32_t n_tokens, uint32_t n_used) {
+    const size_t pairs = (size_t)std::min<uint32_t>(n_tokens, kW4PassTokens) * n_used;
+    return (sizeof(MoeMeta) + 255) / 256 * 256 + pairs * (size_t)moe_ld_h(ff) * 4;
+}
+
+cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
+    const bool mx = p.gate.type == GGML_MXFP4, mx_down = p.down.type == GGML_MXFP4;
+    const int parts = p.x_type == GGML_F32 || p.norm ? 2 : 1;
+    const int sms = device_sms();
+    const int E = (int)p.gate.n_expert, d = (int)p.gate.n_in, ff = (int)p.gate.n_out;
+    const int steps_d = (int)p.gate.steps, steps_ff = (int)p.down.steps;
+    auto up_to = [](int x, int unit) { return (x + unit - 1) / unit * unit; };
+    for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
+        n = std::min(kW4PassTokens, p.n_tokens - t0);
+        int C = 8;
+        while (C > steps_d) C /= 2;
+        auto staged = [&] { const int s = (steps_d + C - 1) / C; return staged_x_bytes(s, parts, n) + staged_c_bytes(mx, s, n); };
+        while (n > 1 && staged() > 120 * 1024) n = (n + 1) / 2;
+        MoeArgs a{};
+        a.gate = p.gate.units;
+        a.up = p.up.units;
+        a.down = p.down.units;
+        a.gate_expert = p.gate.expert_bytes;
+        a.up_expert = p.up.expert_bytes;
+        a.down_expert = p.down.expert_bytes;
+        a.router = p.router;
+        a.x = make_act(row_at(p.x, p.x_type, p.ld_x, t0), p.ld_x, p.x_type);
+        a.T = n;
+        a.E = E;
+        a.k = p.n_used;
+        a.d = d;
+        a.ff = ff;
+        a.tiles_ff = (int)p.gate.tiles;
+        a.steps_d = steps_d;
+        a.tiles_d = (int)p.down.tiles;
+        a.steps_ff = steps_ff;
+        a.normalise = p.normalise;
+        a.norm = p.norm;
+        a.eps = p.eps;
+        a.residual = row_at(p.residual, p.y_type, p.ld_residual, t0);
+        a.ld_residual = p.ld_residual;
+        a.y = const_cast<void *>(row_at(p.y, p.y_type, p.ld_y, t0));
+        a.y_type = p.y_type;
+        a.ld_y = p.ld_y;
+        a.ids = p.ids ? p.ids + (size_t)t0 * p.n_used : nullptr;
+        a.weights = p.weights ? p.weights + (size_t)t0 * p.n_used : nullptr;
+        a.meta = static_cast<MoeMeta *>(p.workspace);
+        a.h = reinterpret_cast<float *>(static_cast<uint8_t *>(p.workspace) + (sizeof(MoeMeta) + 255) / 256 * 256);
+        a.ld_h = moe_ld_h((uint32_t)ff);
+
+        // first kernel: at most `reach` experts are chosen
+        const int reach = std::min(E, n * p.n_used);
+        const int s = (steps_d + C - 1) / C;
+        a.x_bytes = up_to(staged_x_bytes(s, parts, n), 128);
+        a.c_bytes = up_to(staged_c_bytes(mx, s, n), 128);
+        a.logit_bytes = up_to(n * E * 4, 128);
+        a.clusters = std::max(1, (int)std::min<int64_t>(2 * sms / C, (int64_t)reach * a.tiles_ff));
+        const int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes;
+        a.partial_floats = std::max(kWarps * n * kSlotCol, (88 * 1024 - fixed) / 4);
+        cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, C, (size_t)fixed + a.partial_floats * 4, stream)
+                           : launch_gate_up_of<false>(a, parts, C, (size_t)fixed + a.partial_floats * 4, stream);
+        if (e != cudaSuccess) return e;
+
+        // second kernel
+        C = 8;
+        while (C > steps_ff * p.n_used) C /= 2;
+        const int jobs = (a.tiles_d + 1) / 2;
+        const int most = std::max(1, 2 * sms / C), per = (jobs + most - 1) / most;
+        a.clusters = (jobs + per - 1) / per;
+        a.x_bytes = 64 * 1024;
+        a.c_bytes = a.logit_bytes = 0;
+        a.partial_floats = std::max(kWarps * n * kSlotCol, std::min(per * kWarps * n * kSlotCol, (100 * 1024 - a.x_bytes) / 4));
+        e = mx_down ? launch_down_of<true>(a, C, (size_t)a.x_bytes + a.partial_floats * 4, stream)
+                    : launch_down_of<false>(a, C, (size_t)a.x_bytes + a.partial_floats * 4, stream);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

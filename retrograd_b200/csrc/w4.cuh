@@ -79,7 +79,7 @@ struct W4Moe {
     float * weights = nullptr;          // [n_tokens][n_used], optional: their weights
     void * workspace = nullptr;
 };
-size_t w4_moe_workspace_bytes(uint32_t n_expert, uint32_t ff, int n_tokens, int n_used);
+size_t w4_moe_workspace_bytes(uint32_t ff, uint32_t n_tokens, uint32_t n_used);
 cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream);
 
 } // namespace rb200

@@ -169,4 +169,58 @@ int retro_b200_w4_glu(const retro_b200_w4 * gate, const retro_b200_w4 * up, cons
     return product("w4_glu", gate, up, d_x, x_type, ld_x, n_tokens, d_norm, eps, nullptr, nullptr, 0, d_y, y_type, ld_y, stream);
 }
 
+int retro_b200_w4_moe_workspace(const retro_b200_w4 * gate, uint32_t n_tokens, uint32_t n_used, size_t * out_bytes) {
+    return boundary([&]() -> int {
+        if (!gate || !out_bytes) return refuse("w4_moe_workspace", "a weight handle and a place for the result are required");
+        if (n_used == 0 || n_used > kW4MaxUsed) return refuse("w4_moe_workspace", "n_used must be 1 to 32");
+        *out_bytes = w4_moe_workspace_bytes(gate->view.n_out, n_tokens, n_used);
+        return STATUS_OK;
+    });
+}
+
+int retro_b200_w4_moe(const float * d_router, const retro_b200_w4 * gate, const retro_b200_w4 * up, const retro_b200_w4 * down, const void * d_x,
+                      uint32_t x_type, int64_t ld_x, uint32_t n_tokens, uint32_t n_used, int normalise, const float * d_norm, float eps,
+                      const void * d_residual, int64_t ld_residual, void * d_y, uint32_t y_type, int64_t ld_y, int32_t * d_ids, float * d_weights,
+                      void * d_workspace, size_t workspace_bytes, void * stream) {
+    return boundary([&]() -> int {
+        const char * op = "w4_moe";
+        if (!gate || !up || !down) return refuse(op, "a weight handle is required");
+        const W4View & g = gate->view, & u = up->view, & d = down->view;
+        if (u.type != g.type || u.n_out != g.n_out || u.n_in != g.n_in || u.n_expert != g.n_expert)
+            return refuse(op, "gate and up must have one type and shape");
+        if (d.n_expert != g.n_expert || d.n_in != g.n_out || d.n_out != g.n_in) return refuse(op, "down must be the transpose of gate in shape");
+        if (up->device != gate->device || down->device != gate->device) return refuse(op, "the banks are on different devices");
+        if (n_used == 0 || n_used > g.n_expert || n_used > kW4MaxUsed) return refuse(op, "n_used must be 1 to n_expert, at most 32");
+        const w4::MoeShape shape{n_tokens, g.n_expert, n_used, g.n_in, g.n_out};
+        const w4::Rows x{"x", d_x, x_type, ld_x}, y{"y", d_y, y_type, ld_y}, residual{"residual", d_residual, y_type, ld_residual};
+        const w4::MoeBuffers buffers{d_router, d_ids, d_weights, d_workspace, workspace_bytes, w4_moe_workspace_bytes(g.n_out, n_tokens, n_used)};
+        const std::string why = w4::check_moe(shape, x, y, residual, d_norm, eps, buffers);
+        if (!why.empty()) return refuse(op, why);
+        if (n_tokens == 0) return STATUS_OK;
+        const DeviceScope scope(gate->device);
+        W4Moe p;
+        p.gate = g;
+        p.up = u;
+        p.down = d;
+        p.router = d_router;
+        p.x = d_x;
+        p.x_type = x_type;
+        p.ld_x = ld_x;
+        p.n_tokens = (int)n_tokens;
+        p.n_used = (int)n_used;
+        p.normalise = normalise != 0;
+        p.norm = d_norm;
+        p.eps = eps;
+        p.residual = d_residual;
+        p.ld_residual = ld_residual;
+        p.y = d_y;
+        p.y_type = y_type;
+        p.ld_y = ld_y;
+        p.ids = d_ids;
+        p.weights = d_weights;
+        p.workspace = d_workspace;
+        return launched(op, launch_w4_moe(p, static_cast<cudaStream_t>(stream)));
+    });
+}
+
 } // extern "C"

@@ -154,3 +154,51 @@ def w4_glu(gate: W4Matrix, up: W4Matrix, x, *, norm=None, eps: float = 1e-5, out
         _check(gate._lib.retro_b200_w4_glu(gate._h, up._h, px, tx, ldx, tokens, _vector("w4_glu", "norm", norm, gate.n_in, device), eps, py, ty, ldy,
                                            _stream(torch, stream, device)))
     return y
+
+
+def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int, *, normalise: bool = False, norm=None, eps: float = 1e-5,
+           residual=None, out=None, ids=None, weights=None, workspace=None, stream=None):
+    """A mixture-of-experts layer for x [tokens, n_in]: y = residual + sum over the n_used likeliest experts of their probability times
+    down(silu(gate xn) * (up xn)). `ids` (int32) and `weights` (float32), [tokens, n_used], receive the routing. `workspace` is a
+    CUDA byte tensor of at least `w4_moe_workspace(gate, tokens, n_used)` bytes that no other pending call uses; by default one is
+    allocated for the call."""
+    torch = _torch()
+    device = _open("w4_moe", gate, up, down)
+    n_in = gate.n_in
+    px, tx, ldx = _rows("w4_moe", "x", x, n_in, device)
+    tokens = x.shape[0]
+    y = _result(torch, "w4_moe", x, out, tokens, n_in, device)
+    py, ty, ldy = _rows("w4_moe", "out", y, n_in, device, tokens)
+    pr, ldr = None, 0
+    if residual is not None:
+        pr, tr, ldr = _rows("w4_moe", "residual", residual, n_in, device, tokens)
+        if tr != ty:
+            raise InvalidArgument("w4_moe: residual must have the result's element type")
+    if not 1 <= n_used <= min(gate.n_expert, 32):
+        raise InvalidArgument("w4_moe: n_used must be 1 to n_expert, at most 32")
+    for name, t, dtype in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (tokens, n_used) or t.get_device() != device or not t.is_contiguous()):
+            raise InvalidArgument(f"w4_moe: {name} must be contiguous {dtype} [{tokens}, {n_used}] on the weights' device")
+    if not tokens:
+        return y
+    on = _stream(torch, stream, device)
+    if workspace is None:
+        workspace = torch.empty(w4_moe_workspace(gate, tokens, n_used), dtype=torch.uint8, device=x.device)
+        if stream is not None and on != torch.cuda.current_stream(device).cuda_stream:
+            # freed to the allocator when this call returns: it must not be handed out before the given stream is done with it
+            workspace.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(on, device=device))
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise InvalidArgument("w4_moe: the workspace must be contiguous on the weights' device")
+    _check(gate._lib.retro_b200_w4_moe(_vector("w4_moe", "router", router, gate.n_expert * n_in, device), gate._h, up._h, down._h, px, tx, ldx, tokens, n_used,
+                                       normalise, _vector("w4_moe", "norm", norm, n_in, device), eps, pr, ldr, py, ty, ldy,
+                                       None if ids is None else ids.data_ptr(), None if weights is None else weights.data_ptr(),
+                                       workspace.data_ptr(), workspace.numel() * workspace.element_size(), on))
+    return y
+
+
+def w4_moe_workspace(gate: W4Matrix, tokens: int, n_used: int) -> int:
+    """Bytes of workspace a `w4_moe` call of `tokens` tokens needs."""
+    _open("w4_moe_workspace", gate)
+    n = C.c_size_t()
+    _check(gate._lib.retro_b200_w4_moe_workspace(gate._h, tokens, n_used, C.byref(n)))
+    return n.value

@@ -147,3 +147,99 @@ def test_glu_against_float64(rb, kind, n_out, n_in, tokens, act):
     bound = 1.1 * ea * np.abs(b) + np.abs(silu64(a)) * eb + 1.1 * ea * eb + 2.0 ** -20 * np.abs(want) + half_step(torch, act) * np.abs(want) + (2.0 ** -25 if act == "f16" else 1e-37)
     over = np.abs(want) > (65000 if act == "f16" else np.inf)
     assert np.where(over, 0, np.abs(np.where(over, 0, y - want)) - bound).max() <= 0
+
+
+def route64(x, router, k, normalise):
+    """Chosen experts (likeliest first, ties to the lowest), their weights, and the probability gap that decided the choice."""
+    logits = x @ router.T
+    p = np.exp(logits - logits.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    order = np.argsort(-p, axis=1, kind="stable")
+    ranked = np.take_along_axis(p, order, 1)
+    gap = np.full(len(p), np.inf)
+    if p.shape[1] > 1:
+        top = ranked[:, : k + 1]
+        gap = ((top[:, :-1] - top[:, 1:]) / top[:, :-1]).min(1)
+    return order, p, gap
+
+
+def moe64(x, p, ids, gate, up, down, normalise):
+    """The layer's sum over experts for given choices, with a bound on an f32 kernel's error. gate, up, down: lists of decode() pairs."""
+    tokens, k = ids.shape
+    d = down[0][0].shape[0]
+    y, bound = np.zeros((tokens, d)), np.zeros((tokens, d))
+    n_in, ff = x.shape[1], down[0][0].shape[1]
+    for t in range(tokens):
+        w = p[t, ids[t]]
+        if normalise:
+            w = w / w.sum()
+        for j, e in enumerate(ids[t]):
+            a, b = gate[e][0] @ x[t], up[e][0] @ x[t]
+            ea, eb = ((f32_bound(n_in) + 2.0 ** -21) * (m[e][1] @ np.abs(x[t])) for m in (gate, up))
+            h = silu64(a) * b
+            eh = 1.1 * ea * np.abs(b) + np.abs(silu64(a)) * eb + 1.1 * ea * eb + 2.0 ** -20 * np.abs(h)
+            y[t] += w[j] * (down[e][0] @ h)
+            bound[t] += w[j] * (down[e][1] @ (eh + (f32_bound(ff) + 2.0 ** -20) * np.abs(h)))
+    return y, bound
+
+
+def moe_inputs(rng, torch, kind, kind_down, E, d, ff, tokens, act):
+    raws = [[stored_rows(rng, kd, n_out, n_in, scale_spread=1) for _ in range(E)] for kd, n_out, n_in in ((kind, ff, d), (kind, ff, d), (kind_down, d, ff))]
+    x = torch.tensor(rng.normal(0, 1, (tokens, d)), dtype=torch.float32).to(dtype_of(torch, act)).cuda()
+    router = rng.normal(0, 2 / np.sqrt(d), (E, d)).astype(np.float32)
+    return raws, x, router
+
+
+MOE = [
+    # kind, kind of down, experts, used, hidden, ff, tokens, act
+    (MXFP4, MXFP4, 1, 1, 32, 32, 1, "f32"), (Q4_0, Q4_0, 2, 1, 64, 96, 3, "f32"), (MXFP4, MXFP4, 8, 2, 256, 160, 5, "bf16"),
+    (Q4_0, MXFP4, 32, 4, 320, 288, 16, "f32"), (MXFP4, Q4_0, 33, 32, 96, 64, 9, "f32"), (Q4_0, Q4_0, 256, 8, 128, 64, 16, "f16"),
+    (MXFP4, MXFP4, 4, 2, 2880, 2880, 2, "f32"), (Q4_0, Q4_0, 3, 3, 1056, 2048, 21, "f32"), (MXFP4, MXFP4, 6, 2, 64, 4096, 16, "bf16"),
+    (Q4_0, Q4_0, 2, 2, 4096, 64, 16, "f32"),
+]
+
+
+@pytest.mark.parametrize("kind,kind_down,E,k,d,ff,tokens,act", MOE)
+def test_moe_against_float64(rb, kind, kind_down, E, k, d, ff, tokens, act):
+    import torch
+
+    rng = np.random.default_rng(E * 1000 + d + ff + tokens)
+    raws, x, router = moe_inputs(rng, torch, kind, kind_down, E, d, ff, tokens, act)
+    gate, up = (rb.W4Matrix(kind, np.stack(r), ff, d, n_expert=E) for r in raws[:2])
+    down = rb.W4Matrix(kind_down, np.stack(raws[2]), d, ff, n_expert=E)
+    decoded = [[decode(kd, r) for r in bank] for kd, bank in ((kind, raws[0]), (kind, raws[1]), (kind_down, raws[2]))]
+    norm = rng.normal(1, 0.2, d).astype(np.float32)
+    x64 = x.double().cpu().numpy()
+    for use_norm, use_residual, normalise in ((False, False, False), (True, True, True)):
+        ids = torch.full((tokens, k), -1, dtype=torch.int32, device="cuda")
+        weights = torch.full((tokens, k), float("nan"), device="cuda")
+        residual = torch.tensor(rng.normal(0, 1, (tokens, d)), dtype=torch.float32).to(x.dtype).cuda() if use_residual else None
+        y = rb.w4_moe(torch.tensor(router).cuda(), gate, up, down, x, k, normalise=normalise, norm=torch.tensor(norm).cuda() if use_norm else None,
+                      residual=residual, ids=ids, weights=weights)
+        xn = normed(x64, norm.astype(np.float64) if use_norm else None, 1e-5)
+        order, p, gap = route64(xn, router.astype(np.float64), k, normalise)
+        got_ids = ids.cpu().numpy()
+        # logits differ by less than 1e-5 (|x| |r| d 2^-24 and the norm's 2^-21): probabilities closer than that may swap places
+        clear = gap > 4e-5
+        assert np.array_equal(got_ids[clear], order[clear, :k]) and clear.mean() > 0.8
+        assert all(len(set(row)) == k for row in got_ids.tolist()) and got_ids.min() >= 0 and got_ids.max() < E
+        w = np.take_along_axis(p, got_ids.astype(np.int64), 1)
+        w = w / w.sum(1, keepdims=True) if normalise else w
+        assert np.abs(weights.double().cpu().numpy() - w).max() <= 4e-5 * w.max()
+        want, bound = moe64(xn, p, got_ids, *decoded, normalise)
+        total = want + (residual.double().cpu().numpy() if use_residual else 0)
+        # a weight's relative error (the logits' error twice, exponentials, sums): 4e-5, on every expert's part
+        bound = bound + 4e-5 * expert_parts(xn, p, got_ids, *decoded, normalise)
+        bound = bound + 2.0 ** -22 * (np.abs(total) + np.abs(want)) + half_step(torch, act) * np.abs(total)
+        error = np.abs(y.double().cpu().numpy() - total)
+        assert (error <= bound).all(), float((error / bound).max())
+
+
+def expert_parts(x, p, ids, gate, up, down, normalise):
+    """Sum of the magnitudes of the experts' parts of y: what an error of the routing weights is relative to."""
+    out = np.zeros((ids.shape[0], down[0][0].shape[0]))
+    for t in range(ids.shape[0]):
+        w = p[t, ids[t]] / (p[t, ids[t]].sum() if normalise else 1.0)
+        for j, e in enumerate(ids[t]):
+            out[t] += w[j] * np.abs(down[e][0] @ (silu64(gate[e][0] @ x[t]) * (up[e][0] @ x[t])))
+    return out
