@@ -1,6 +1,6 @@
 // Products with 4-bit weights for at most sixteen tokens, bound by the weight stream.
 //
-// Mathematics. A unit of 16 rows x 64 columns is the A operand of four m16n8k16 products; the tokens are the columns
+// Mathematics. 16 rows x 64 columns are the A operands of four m16n8k16 products; the tokens are the columns
 // of B. The weights enter as exact f16 values that cost no arithmetic beyond masks and shifts:
 //   Q4_0   the nibble q in the low bits of an f16 is the subnormal q 2^-24, in the next four bits 16 q 2^-24; the
 //          columns whose nibbles sit there get their activations divided by 16. The offset is the product chain's start
@@ -10,17 +10,20 @@
 // hi + lo f16 (22 bits); activations that are f16 or bf16 themselves need no lo. A 32-column group is exactly two
 // products, so its f32 sum comes out on its own, is multiplied by the group's scale and added in f32.
 //
-// Split. A cluster of up to eight CTAs owns a range of row tiles; each CTA takes a range of the columns for all of them, so
-// it converts only its share of the activations. Its warps take (pair of row tiles, part of the CTA's columns) items, and
-// the partial sums meet in shared memory, are added over the cluster's shared memories in a fixed order (no workspace, no
-// atomics: results are the same in every run), and get bias, residual or the gate's activation there. Every warp keeps
-// kDepth units of two tiles in flight in registers.
+// Split. A cluster of up to eight CTAs owns a range of row blocks (32 rows); each CTA takes a range of the columns for all of them, so
+// it converts only its share of the activations. Its warps take (row block, part of the CTA's columns) runs, and
+// write every (row block, token)'s sums into the shared memory of the CTA that owns it, which adds them in a fixed order after one
+// cluster barrier (no workspace, no atomics: results are the same in every run) and applies bias, residual or the gate's
+// activation. Every warp streams its units through a ring of its own in shared memory by asynchronous copies, kStages - 1 units
+// ahead, so that no registers are held by loads in flight and three CTAs fit on an SM.
 
 #include "kernels.cuh"
 #include "blocks.hpp"
 #include "w4.cuh"
 
 #include <algorithm>
+#include <cmath>
+#include <cstddef>
 #include <cuda_bf16.h>
 
 namespace rb200 {
@@ -29,9 +32,10 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kDepth = 4;           // units in flight per warp and row tile
+constexpr int kStages = 4;          // units in a warp's ring
 constexpr int kSlotCol = 36;        // floats per (partial slot, token): 32 rows, padded so that a warp's stores meet no bank twice
 constexpr int kMaxSegs = 16;
+constexpr int kMaxCluster = 8;
 constexpr int kRowList = kW4PassTokens;
 
 struct Act {
@@ -71,6 +75,11 @@ __device__ __forceinline__ void load4(const Act & a, int64_t row, int k, float (
     }
 }
 
+__device__ __forceinline__ void scale4(float (&v)[4], const float * by) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= by[e];
+}
+
 __device__ __forceinline__ void store1(void * p, uint32_t type, int64_t i, float v) {
     if (type == GGML_F32) static_cast<float *>(p)[i] = v;
     else if (type == GGML_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
@@ -81,14 +90,11 @@ __device__ __forceinline__ void store1(void * p, uint32_t type, int64_t i, float
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-}
 __device__ __forceinline__ uint32_t smem_address(const void * p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// Shared-memory float `index` behind `base` of CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t remote_address(uint32_t base, uint32_t rank) {
+// The address of `at` (this CTA's shared memory) in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote_address(uint32_t at, uint32_t rank) {
     uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
     return a;
 }
 __device__ __forceinline__ float remote_load(uint32_t address) {
@@ -96,21 +102,52 @@ __device__ __forceinline__ float remote_load(uint32_t address) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
     return v;
 }
+__device__ __forceinline__ void remote_store(uint32_t address, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
+}
+// The CTAs of a cluster have started: required before the first access to another's shared memory. Arrive early, wait late.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+    cluster_arrive();
+    cluster_wait();
+}
 
 // ---- weights
 
+// The lane's share of a unit: A words and scales of its two row tiles.
 template <bool MX> struct Unit {
-    uint4 q;
-    uint2 s;        // MXFP4 uses .x only
+    uint4 q[2];
+    uint2 s[2];     // MXFP4 uses .x only
 };
 
-template <bool MX> __device__ __forceinline__ void load_unit(Unit<MX> & u, const uint8_t * p, int lane) {
-    // weights are never written while a handle lives, so the read-only path holds even while earlier kernels still run
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.q.x), "=r"(u.q.y), "=r"(u.q.z), "=r"(u.q.w) : "l"(p + lane * 16));
-    if constexpr (MX) {
-        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(u.s.x) : "l"(p + 512 + (lane >> 2) * 4));
-    } else {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(u.s.x), "=r"(u.s.y) : "l"(p + 512 + (lane >> 2) * 8));
+__host__ __device__ constexpr int ring_bytes(bool mx) { return kWarps * kStages * (int)w4_unit_bytes(mx); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t * src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 shared_u4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 shared_u2(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t shared_u1(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+
+template <bool MX> __device__ __forceinline__ void read_unit(uint32_t words, uint32_t scales, Unit<MX> & u) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        u.q[i] = shared_u4(words + i * 512);
+        if constexpr (MX) u.s[i].x = shared_u1(scales + i * 32);
+        else u.s[i] = shared_u2(scales + i * 64);
     }
 }
 
@@ -147,6 +184,12 @@ template <bool MX, int H> __device__ __forceinline__ void scales(const uint2 & s
     }
 }
 
+// c = a b + (s0, s1, s0, s1), and c += a b.
+__device__ __forceinline__ void mma_start(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float s0, float s1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(s0), "f"(s1));
+}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -155,170 +198,214 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 
 // How many tokens a product chain serves. PACK: up to four, MMA column c is token c's hi part and column c + 4 its lo part.
 enum Mode { PACK = 0, ONE = 1, TWO = 2 };
-__device__ __forceinline__ int mode_of(int n, int parts) { return n > 8 ? TWO : parts == 2 && n <= 4 ? PACK : ONE; }
+__host__ __device__ constexpr int mode_of(int n, int parts) { return n > 8 ? TWO : parts == 2 && n <= 4 ? PACK : ONE; }
 
 // ---- activations in shared memory
 //
-// x   [step][group][part][token][32] f16, c [step][group][token] f32: the start value of the group's products (Q4_0).
+// x   [step][group][part][NT tokens][32] f16, then (Q4_0) c [step][group][NT tokens] f32: the start values of the group's products. NT,
+// the tokens there is room for, is a template argument wherever they are read, so that the offsets inside a step are immediates.
+__host__ __device__ constexpr int step_x_bytes(int parts, int nt) { return 2 * parts * nt * 64; }
+__host__ __device__ constexpr int step_c_bytes(bool mx, int nt) { return mx ? 0 : 2 * nt * 4; }
+__host__ __device__ constexpr int step_bytes(bool mx, int parts, int nt) { return step_x_bytes(parts, nt) + step_c_bytes(mx, nt); }
 struct Staged {
     uint8_t * x;
     float * c;
-    int n;          // tokens held
 };
-__host__ __device__ inline int staged_x_bytes(int steps, int parts, int n) { return steps * 2 * parts * n * 64; }
-__host__ __device__ inline int staged_c_bytes(bool mx, int steps, int n) { return mx ? 0 : steps * 2 * n * 4; }
 
 struct Scratch {
     float f1[kMaxSegs][kRowList], f2[kMaxSegs][kRowList];   // a token's sums times f1 times f2 are in the activations' own scale
-    float ss[kRowList];                                     // sum of squares of the CTA's columns
-    float red[2][kWarps];
+    float ss[kMaxCluster][kRowList];                        // sums of squares of each CTA's columns
+    uint32_t top[kWarps];
+    float squares[kWarps];
+    uint64_t zero;                                          // start values of PACK's lo columns
 };
 
-// Converts columns [k0, k0 + 64 steps) of `n` rows. row_of(i) is the row of token i; columns at and behind n_in are zero.
-template <bool MX, int PARTS, class RowOf>
-__device__ void stage(const Act & act, RowOf row_of, int n, int k0, int steps, int n_in, const float * norm, const Staged & out, Scratch & sc, int seg) {
+// One token's row of activations, or the part of it a CTA needs, and where it goes.
+struct StageRow {
+    int64_t row;
+    int k0, steps;              // columns k0 .. k0 + 64 steps - 1; those at and behind n_in are zero
+    int nt, place;              // room of the token set, the token's place in it
+    int seg;                    // row of Scratch::f1, f2
+    Staged out;
+};
+
+template <bool MX, int PARTS> __device__ __forceinline__ void stage_chunk(const StageRow & r, int i, float (&v)[4], float up) {
+    const int step = i >> 4, group = (i >> 3) & 1, at = (i & 7) * 4;
+    const bool inside = i < r.steps * 16;
+    const float factor = !MX && group ? up * 0.0625f : up;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= factor;
+    if constexpr (!MX) {
+        float sum = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (inside && (threadIdx.x & 7) == 0) r.out.c[(step * 2 + group) * r.nt + r.place] = sum * (group ? -128.f : -8.f) * 5.9604644775390625e-8f;
+    }
+    if (inside) {
+        const __half2 h0 = __floats2half2_rn(v[0], v[1]), h1 = __floats2half2_rn(v[2], v[3]);
+        uint8_t * dst = r.out.x + ((step * 2 + group) * PARTS * r.nt + r.place) * 64 + at * 2;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&h0), *reinterpret_cast<const uint32_t *>(&h1));
+        if constexpr (PARTS == 2) {
+            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+            const __half2 l0 = __floats2half2_rn(v[0] - f0.x, v[1] - f0.y), l1 = __floats2half2_rn(v[2] - f1.x, v[3] - f1.y);
+            *reinterpret_cast<uint2 *>(dst + r.nt * 64) = make_uint2(*reinterpret_cast<const uint32_t *>(&l0), *reinterpret_cast<const uint32_t *>(&l1));
+        }
+    }
+}
+
+// Converts n rows; row_of(i) describes them. Each is one warp's work, or with few rows that of several warps. NORM: rows
+// are multiplied by `norm`, and put_squares(row, sum) gets the row's sum of squares. Every thread takes part; a barrier follows at the caller's.
+template <bool MX, int PARTS, bool NORM, class RowOf, class PutSquares>
+__device__ void stage_rows(const Act & act, int n, int n_in, const float * norm, Scratch & sc, RowOf row_of, PutSquares put_squares) {
+    constexpr int kHeld = 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_token = n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 4 : 8;      // warps that share a token
-    const int stride = kWarps / per_token;
-    const int part = warp % per_token;
-    const int count = steps * 16;                                     // chunks of four columns
-    for (int t0 = 0; t0 < n; t0 += stride) {
-        const int t = t0 + warp / per_token;
-        const bool live = t < n;
-        const int64_t row = live ? row_of(t) : 0;
-        float top = 0.f, squares = 0.f;
-        bool finite = true;
-        for (int i = part * 32 + lane; live && i < count; i += per_token * 32) {
-            const int k = k0 + 4 * i;
-            if (k >= n_in) break;
-            float v[4];
-            load4(act, row, k, v);
+    const int shared = n > 4 ? 1 : n > 2 ? 2 : n > 1 ? 4 : 8;      // warps that share a row
+    const int part = warp % shared;
+    for (int i0 = warp / shared; i0 < n || shared > 1; i0 += kWarps / shared) {
+        const bool live = i0 < n;
+        const StageRow r = row_of(live ? i0 : 0);
+        const int count = live ? min(r.steps * 16, (n_in - r.k0) / 4) : 0;     // chunks of four columns that exist, whole groups
+        const int trips = live ? (r.steps * 16 + shared * 32 - 1) / (shared * 32) : 0;
+        const int first = part * 32 + lane;
+        // the largest magnitude as bits: a NaN is above infinity, infinity above every number
+        uint32_t top = 0;
+        float squares = 0.f;
+        float held[kHeld][4];
+        auto look = [&](int i, float (&v)[4]) {
+            v[0] = v[1] = v[2] = v[3] = 0.f;
+            if (i < count) {
+                load4(act, r.row, r.k0 + 4 * i, v);
+                if constexpr (NORM) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                squares += v[e] * v[e];
-                if (norm) v[e] *= norm[k + e];
-                top = fmaxf(top, fabsf(v[e]));
-                finite = finite && fabsf(v[e]) < INFINITY;
+                    for (int e = 0; e < 4; ++e) squares += v[e] * v[e];
+                    scale4(v, norm + r.k0 + 4 * i);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
             }
-        }
+        };
+        if (trips <= kHeld) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            squares += __shfl_xor_sync(0xffffffffu, squares, o);
+            for (int it = 0; it < kHeld; ++it) if (it < trips) look(first + it * shared * 32, held[it]);
+        } else {
+            for (int it = 0; it < trips; ++it) look(first + it * shared * 32, held[0]);
         }
-        if (!__all_sync(0xffffffffu, finite)) top = INFINITY;
-        if (per_token > 1) {
-            if (lane == 0) { sc.red[0][warp] = top; sc.red[1][warp] = squares; }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if constexpr (NORM) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+        }
+        if (shared > 1) {
+            if (lane == 0) { sc.top[warp] = top; sc.squares[warp] = squares; }
             __syncthreads();
-            const int first = warp - part;
-            top = 0.f;
+            top = 0;
             squares = 0.f;
-            for (int i = 0; i < per_token; ++i) { top = fmaxf(top, sc.red[0][first + i]); squares += sc.red[1][first + i]; }
+            for (int i = 0; i < shared; ++i) { top = max(top, sc.top[warp - part + i]); squares += sc.squares[warp - part + i]; }
         }
-        // 2^shift brings the largest magnitude into [2^13, 2^14); in two factors, so that none leaves f32. A row with an
-        // infinity or a NaN is left as it is: its own sums become NaN, those of the other tokens stay what they are.
-        const int shift = top > 0.f && top < INFINITY ? 13 - ilogbf(top) : 0;
-        const float up1 = scalbnf(1.f, shift / 2), up2 = scalbnf(1.f, shift - shift / 2);
+        // 2^shift brings the largest magnitude into [2^13, 2^14), as far as it is an f32 itself (below 2^-113 the values only
+        // come near). A row with an infinity or a NaN is left as it is: its own sums become NaN, those of the other tokens
+        // stay what they are.
+        const int shift = top > 0 && top < 0x7f800000u ? min(126, 13 - ((int)(top >> 23) - 127)) : 0;
+        const float up = __uint_as_float((uint32_t)(shift + 127) << 23);
         if (live && part == 0 && lane == 0) {
             const int down = (MX ? 6 : 24) - shift;
-            sc.f1[seg][t] = scalbnf(1.f, down / 2);
-            sc.f2[seg][t] = scalbnf(1.f, down - down / 2);
-            sc.ss[t] = squares;
+            sc.f1[r.seg][r.place] = __uint_as_float((uint32_t)(down / 2 + 127) << 23);
+            sc.f2[r.seg][r.place] = __uint_as_float((uint32_t)(down - down / 2 + 127) << 23);
+            if constexpr (NORM) put_squares(i0, squares);
         }
-        // the trip count is the warp's, not the lane's: the group sums below are taken by the whole warp
-        const int trips = live ? (count + per_token * 32 - 1) / (per_token * 32) : 0;
-        for (int it = 0; it < trips; ++it) {
-            const int i = it * per_token * 32 + part * 32 + lane;
-            const int k = k0 + 4 * i;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (i < count && k < n_in) {
-                load4(act, row, k, v);
-                if (norm) {
+        if (trips <= kHeld) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= norm[k + e];
+            for (int it = 0; it < kHeld; ++it) if (it < trips) stage_chunk<MX, PARTS>(r, first + it * shared * 32, held[it], up);
+        } else {
+            for (int it = 0; it < trips; ++it) {
+                const int i = first + it * shared * 32;
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+                if (i < count) {
+                    load4(act, r.row, r.k0 + 4 * i, v);
+                    if constexpr (NORM) scale4(v, norm + r.k0 + 4 * i);
                 }
-            }
-            const int step = i >> 4, group = (i >> 3) & 1, at = (i & 7) * 4;
-            const float lower = !MX && group ? 0.0625f : 1.f;
-            __half hi[4], lo[4];
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float f = v[e] * up1 * up2 * lower;
-                hi[e] = __float2half_rn(f);
-                sum += __half2float(hi[e]);
-                if constexpr (PARTS == 2) {
-                    lo[e] = __float2half_rn(f - __half2float(hi[e]));
-                    sum += __half2float(lo[e]);
-                }
-            }
-            if (i < count) {
-                uint8_t * dst = out.x + ((size_t)((step * 2 + group) * PARTS) * out.n + t) * 64 + at * 2;
-                *reinterpret_cast<uint2 *>(dst) = make_uint2((uint32_t)__half_as_ushort(hi[0]) | (uint32_t)__half_as_ushort(hi[1]) << 16,
-                                                             (uint32_t)__half_as_ushort(hi[2]) | (uint32_t)__half_as_ushort(hi[3]) << 16);
-                if constexpr (PARTS == 2)
-                    *reinterpret_cast<uint2 *>(dst + (size_t)out.n * 64) =
-                        make_uint2((uint32_t)__half_as_ushort(lo[0]) | (uint32_t)__half_as_ushort(lo[1]) << 16,
-                                   (uint32_t)__half_as_ushort(lo[2]) | (uint32_t)__half_as_ushort(lo[3]) << 16);
-            }
-            if constexpr (!MX) {
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (i < count && (lane & 7) == 0) out.c[(step * 2 + group) * out.n + t] = sum * (group ? -128.f : -8.f) * 5.9604644775390625e-8f;
+                stage_chunk<MX, PARTS>(r, i, v, up);
             }
         }
-        if (per_token > 1) __syncthreads();     // sc.red is written again for the next tokens
+        if (shared > 1) break;      // that many warps share a row only when one round holds all rows
     }
+}
+
+// The rows of a call's tokens, normalised by its weights when it has any. A row's squares go to every CTA of the cluster.
+template <bool MX, int PARTS>
+__device__ __forceinline__ void stage_tokens(const Act & act, int n, int nt, int s0, int steps, int n_in, const float * norm, const Staged & out, Scratch & sc,
+                                             int rank, int C) {
+    auto row_of = [&](int t) { return StageRow{(int64_t)t, s0 * 64, steps, nt, t, 0, out}; };
+    if (norm) {
+        cluster_wait();
+        stage_rows<MX, PARTS, true>(act, n, n_in, norm, sc, row_of, [&](int t, float squares) {
+            for (int c = 0; c < C; ++c) remote_store(remote_address(smem_address(&sc.ss[rank][t]), c), squares);
+        });
+    } else {
+        stage_rows<MX, PARTS, false>(act, n, n_in, nullptr, sc, row_of, [](int, float) {});
+        cluster_wait();
+    }
+}
+
+// 1 / sqrt(mean of squares + eps) of token t, once the cluster has met after stage_tokens.
+__device__ __forceinline__ float rms_factor(const Scratch & sc, int t, int C, int n_in, float eps) {
+    float ss = 0.f;
+    for (int c = 0; c < C; ++c) ss += sc.ss[c][t];
+    return rsqrtf(ss / (float)n_in + eps);
 }
 
 // ---- the product chain
 
-// A run: consecutive 64-column steps of two row tiles against one set of tokens.
-struct Run {
-    const uint8_t * p0, * p1;   // the tiles' first units
-    int len;                    // steps
-    Staged x;                   // activations, from the run's first step on
-    const uint8_t * list;       // token (place in x) of each MMA column
+// A warp works through runs: the units of a row block against one set of tokens. Consecutive runs with the same tokens and
+// columns are a group. What a group needs of the activations:
+struct Group {
+    Staged x;                   // from the group's first step on
+    const uint8_t * list;       // token (place in x) of each MMA column; unused where the places are the columns
     int n;                      // how many
+    int seg;                    // row of Scratch::f1, f2
 };
 
-// Where a lane finds its B fragments and start values of one run.
+// Where a lane finds its B fragments and start values, and the factors of its columns' sums.
 struct Lane {
-    const uint8_t * b[2];
-    const float * c[2][2];
-    int b_step, b_part, b_group, c_step, c_group;
+    uint32_t b[2], c[2][2];             // shared-memory addresses at the group's first step
+    uint32_t c_step;
+    float f1[2][2], f2[2][2];
 };
 
-template <bool MX, int PARTS>
-__device__ __forceinline__ void begin_run(const Run & r, int mode, int lane, Lane & l) {
+template <bool MX, int PARTS, int MODE, int NT, bool LIST>
+__device__ __forceinline__ void begin_group(const Group & r, int lane, const Scratch & sc, Lane & l) {
+    constexpr int NC = MODE == TWO ? 2 : 1;
     const int g = lane >> 2, t4 = lane & 3;
-    l.b_part = r.x.n * 64;
-    l.b_group = PARTS * l.b_part;
-    l.b_step = 2 * l.b_group;
-    l.c_step = 2 * r.x.n;
-    l.c_group = r.x.n;
-    if (mode == PACK) {
-        const int tok = r.list[min(g & 3, r.n - 1)];
-        l.b[0] = r.x.x + (size_t)tok * 64 + t4 * 16 + (g >= 4 ? l.b_part : 0);
-    } else {
-        l.b[0] = r.x.x + (size_t)r.list[min(g, r.n - 1)] * 64 + t4 * 16;
-    }
-    l.b[1] = mode == TWO ? r.x.x + (size_t)r.list[min(g + 8, r.n - 1)] * 64 + t4 * 16 : l.b[0];
-    if constexpr (!MX) {
+    const bool lo = MODE == PACK;
+    const uint32_t x = smem_address(r.x.x), c = MX ? 0 : smem_address(r.x.c);
+    auto place = [&](int col) { const int i = min(col, r.n - 1); return LIST ? (int)r.list[i] : i; };
+    l.b[0] = x + place(lo ? g & 3 : g) * 64 + t4 * 16 + (lo && g >= 4 ? NT * 64 : 0);
+    if constexpr (NC == 2) l.b[1] = x + place(g + 8) * 64 + t4 * 16;
+    l.c_step = step_c_bytes(MX, NT);
 #pragma unroll
-        for (int nc = 0; nc < 2; ++nc)
+    for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int col = mode == PACK ? (2 * t4 + e) & 3 : 8 * nc + 2 * t4 + e;
-                l.c[nc][e] = r.x.c + r.list[min(col, r.n - 1)];
-            }
+        for (int e = 0; e < 2; ++e) {
+            const int tok = place(lo ? (2 * t4 + e) & 3 : 8 * nc + 2 * t4 + e);
+            if constexpr (!MX) l.c[nc][e] = c + tok * 4;
+            l.f1[nc][e] = sc.f1[r.seg][tok];
+            l.f2[nc][e] = sc.f2[r.seg][tok];
+        }
+    if constexpr (!MX && lo) {
+        if (t4 >= 2) {
+            l.c[0][0] = l.c[0][1] = smem_address(&sc.zero);
+            l.c_step = 0;
+        }
     }
 }
 
-template <bool MX, int PARTS, int MODE>
-__device__ __forceinline__ void do_step(const Unit<MX> (&u)[2], Lane & l, int lane, float (&acc)[2][2][4]) {
+// One unit. NT == 1: every MMA column is the one token, and only the even ones are kept.
+template <bool MX, int PARTS, int MODE, int NT, bool LIST>
+__device__ __forceinline__ void do_step(uint32_t words, uint32_t scale_at, uint32_t b_at, uint32_t c_at, const Lane & l, float (&acc)[2][2][4]) {
     constexpr int NC = MODE == TWO ? 2 : 1;
     constexpr int NP = MODE == PACK ? 1 : PARTS;
+    Unit<MX> u;
+    read_unit<MX>(words, scale_at, u);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         uint4 b[NC][NP];
@@ -326,152 +413,161 @@ __device__ __forceinline__ void do_step(const Unit<MX> (&u)[2], Lane & l, int la
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p) b[nc][p] = *reinterpret_cast<const uint4 *>(l.b[nc] + h * l.b_group + p * l.b_part);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                start[nc][e] = 0.f;
-                if constexpr (!MX) {
-                    start[nc][e] = l.c[nc][e][h * l.c_group];
-                    if (MODE == PACK && (lane & 2)) start[nc][e] = 0.f;      // the lo columns carry no offset
-                }
+            for (int p = 0; p < NP; ++p) b[nc][p] = shared_u4(l.b[nc] + b_at + (h * PARTS + p) * (NT * 64));
+            start[nc][0] = start[nc][1] = 0.f;
+            if constexpr (!MX) {
+                const int c_group = MODE == PACK ? 0 : h * NT * 4;      // PACK: the zero has no groups, so h is part of c_at there
+                const uint32_t hh = MODE == PACK ? h * (l.c_step >> 1) : 0;
+                start[nc][0] = __uint_as_float(shared_u1(l.c[nc][0] + c_at + c_group + hh));
+                start[nc][1] = NT == 1 ? start[nc][0] : __uint_as_float(shared_u1(l.c[nc][1] + c_at + c_group + hh));
             }
         }
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
             float c[NC][4];
-#pragma unroll
-            for (int nc = 0; nc < NC; ++nc) { c[nc][0] = c[nc][2] = start[nc][0]; c[nc][1] = c[nc][3] = start[nc][1]; }
             uint32_t a[4];
-            if (h == 0) decode<MX, 0, 0>(u[tile].q, a); else decode<MX, 1, 0>(u[tile].q, a);
+            if (h == 0) decode<MX, 0, 0>(u.q[tile], a); else decode<MX, 1, 0>(u.q[tile], a);
 #pragma unroll
-            for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-                for (int p = 0; p < NP; ++p) mma(c[nc], a, b[nc][p].x, b[nc][p].y);
-            if (h == 0) decode<MX, 0, 1>(u[tile].q, a); else decode<MX, 1, 1>(u[tile].q, a);
+            for (int nc = 0; nc < NC; ++nc) {
+                mma_start(c[nc], a, b[nc][0].x, b[nc][0].y, start[nc][0], start[nc][1]);
+                if constexpr (NP == 2) mma(c[nc], a, b[nc][NP - 1].x, b[nc][NP - 1].y);
+            }
+            if (h == 0) decode<MX, 0, 1>(u.q[tile], a); else decode<MX, 1, 1>(u.q[tile], a);
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
                 for (int p = 0; p < NP; ++p) mma(c[nc], a, b[nc][p].z, b[nc][p].w);
             float d0, d1;
-            if (h == 0) scales<MX, 0>(u[tile].s, d0, d1); else scales<MX, 1>(u[tile].s, d0, d1);
+            if (h == 0) scales<MX, 0>(u.s[tile], d0, d1); else scales<MX, 1>(u.s[tile], d0, d1);
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
                 acc[tile][nc][0] += d0 * c[nc][0];
-                acc[tile][nc][1] += d0 * c[nc][1];
                 acc[tile][nc][2] += d1 * c[nc][2];
-                acc[tile][nc][3] += d1 * c[nc][3];
-            }
-        }
-    }
-#pragma unroll
-    for (int nc = 0; nc < NC; ++nc) {
-        l.b[nc] += l.b_step;
-        if constexpr (!MX) { l.c[nc][0] += l.c_step; l.c[nc][1] += l.c_step; }
-    }
-}
-
-// Calls put(row 0..31 of the pair, column, sum) for every column of the run this lane holds.
-template <class Put>
-__device__ __forceinline__ void end_run(int mode, int n, int lane, float (&acc)[2][2][4], Put put) {
-    const int g = lane >> 2, t4 = lane & 3;
-#pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
-#pragma unroll
-        for (int nc = 0; nc < 2; ++nc) {
-            if (nc == 1 && mode != TWO) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v = acc[tile][nc][i];
-                if (mode == PACK) v += __shfl_xor_sync(0xffffffffu, v, 2);      // hi column + lo column
-                const int col = 8 * nc + 2 * t4 + (i & 1);
-                if (col < n && !(mode == PACK && t4 >= 2)) put(tile * 16 + g + (i >> 1) * 8, col, v);
-            }
-        }
-#pragma unroll
-        for (int nc = 0; nc < 2; ++nc)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[tile][nc][i] = 0.f;
-    }
-}
-
-// A warp's sequence of runs: items warp, warp + kWarps, ... below n_items, each with n_segs runs (some may be empty).
-// Source: int len(item, seg); Run run(item, seg); put(item, seg, row, column, sum). MODES: the modes that occur.
-template <bool MX, int PARTS, int MODES, class Source>
-struct Stream {
-    Source & src;
-    const int n_items, n_segs, lane;
-    Unit<MX> buf[kDepth][2];
-    struct Cursor { int item, seg, rem; } ld, cp;
-    const uint8_t * p0, * p1;
-
-    __device__ __forceinline__ Stream(Source & s, int items, int segs) : src(s), n_items(items), n_segs(segs), lane(threadIdx.x & 31) {
-        ld = {(int)(threadIdx.x >> 5), -1, 0};
-        next(ld);
-        cp = ld;
-        if (ld.item < n_items) point();
-    }
-    __device__ __forceinline__ void next(Cursor & c) {
-        do {
-            if (++c.seg == n_segs) { c.seg = 0; c.item += kWarps; }
-            if (c.item >= n_items) return;
-            c.rem = src.len(c.item, c.seg);
-        } while (c.rem == 0);
-    }
-    __device__ __forceinline__ void point() {
-        const Run r = src.run(ld.item, ld.seg);
-        p0 = r.p0;
-        p1 = r.p1;
-    }
-    __device__ __forceinline__ void fetch(int d) {
-        if (ld.item >= n_items) return;
-        load_unit<MX>(buf[d][0], p0, lane);
-        load_unit<MX>(buf[d][1], p1, lane);
-        p0 += w4_unit_bytes(MX);
-        p1 += w4_unit_bytes(MX);
-        if (--ld.rem == 0) {
-            next(ld);
-            if (ld.item < n_items) point();
-        }
-    }
-    // The first units of the sequence; needs nothing but the weights.
-    __device__ __forceinline__ void prefetch() {
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) fetch(d);
-    }
-    __device__ __forceinline__ void work() {
-        if (cp.item >= n_items) return;
-        float acc[2][2][4] = {};
-        Lane l;
-        Run r = src.run(cp.item, cp.seg);
-        int mode = mode_of(r.n, PARTS);
-        begin_run<MX, PARTS>(r, mode, lane, l);
-        while (cp.item < n_items) {
-#pragma unroll
-            for (int d = 0; d < kDepth; ++d) {
-                if (cp.item >= n_items) break;
-                if constexpr (MODES & (1 << PACK)) if (MODES == (1 << PACK) || mode == PACK) do_step<MX, PARTS, PACK>(buf[d], l, lane, acc);
-                if constexpr (MODES & (1 << ONE)) if (MODES == (1 << ONE) || mode == ONE) do_step<MX, PARTS, ONE>(buf[d], l, lane, acc);
-                if constexpr (MODES & (1 << TWO)) if (MODES == (1 << TWO) || mode == TWO) do_step<MX, PARTS, TWO>(buf[d], l, lane, acc);
-                fetch(d);
-                if (--cp.rem == 0) {
-                    end_run(mode, r.n, lane, acc, [&](int row, int col, float v) { src.put(cp.item, cp.seg, row, col, v); });
-                    next(cp);
-                    if (cp.item < n_items) {
-                        r = src.run(cp.item, cp.seg);
-                        mode = mode_of(r.n, PARTS);
-                        begin_run<MX, PARTS>(r, mode, lane, l);
-                    }
+                if constexpr (NT > 1) {
+                    acc[tile][nc][1] += d0 * c[nc][1];
+                    acc[tile][nc][3] += d1 * c[nc][3];
                 }
             }
         }
     }
+}
+
+// Hands a run's sums to put(row 0..31 of the block, column, sum) and clears them.
+template <int MODE, int NT, class Put>
+__device__ __forceinline__ void end_run(int n, int lane, const Lane & l, float (&acc)[2][2][4], Put put) {
+    const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+        for (int nc = 0; nc < (MODE == TWO ? 2 : 1); ++nc)
+#pragma unroll
+            for (int i = 0; i < 4; i += NT > 1 ? 1 : 2) {
+                float v = acc[tile][nc][i];
+                if constexpr (MODE == PACK) v += __shfl_xor_sync(0xffffffffu, v, 2);      // hi column + lo column
+                const int col = 8 * nc + 2 * t4 + (i & 1);
+                if (col < n && !(MODE == PACK && t4 >= 2)) put(tile * 16 + g + (i >> 1) * 8, col, v * l.f1[nc][i & 1] * l.f2[nc][i & 1]);
+                acc[tile][nc][i] = 0.f;
+            }
+}
+
+// Where a warp is in its sequence of runs.
+struct Cursor {
+    const uint8_t * p;          // the next unit
+    int rem;                    // units left in the run
+    int group, job;             // the Source's
+    bool live;
 };
 
-// Parts of the columns the warps split an item into: as few as keep the warps evenly loaded. The cost counts steps of the
-// busiest warp and two steps' time for every partial sum it writes.
-__host__ __device__ inline int split_columns(int jobs, int steps) {
+// Runs a warp's sequence. Source: first(Cursor &) and next(Cursor &) move to a run (never an empty one) and set everything;
+// group(const Cursor &) describes the activations; put(const Cursor &, row, column, sum) takes the sums.
+template <bool MX, class Source> struct Stream {
+    const Source & src;
+    const int lane;
+    const uint32_t ring;
+    Cursor ld, cp;
+    uint32_t fill, at;          // ring offsets of the stage to fill and the stage to multiply
+
+    __device__ __forceinline__ Stream(const Source & s, uint8_t * rings)
+        : src(s), lane(threadIdx.x & 31), ring(smem_address(rings) + (threadIdx.x >> 5) * (kStages * w4_unit_bytes(MX))), fill(0), at(0) {
+        src.first(ld);
+        cp = ld;
+    }
+    __device__ __forceinline__ void fetch() {
+        if (ld.live) {
+            const uint32_t dst = ring + fill + lane * 16;
+            const uint8_t * p = ld.p + lane * 16;
+            copy16(dst, p);
+            copy16(dst + 512, p + 512);
+            if (lane < (MX ? 4 : 8)) copy16(dst + 1024, p + 1024);
+            ld.p += w4_unit_bytes(MX);
+            if (--ld.rem == 0) src.next(ld);
+        }
+        fill = fill == (kStages - 1) * w4_unit_bytes(MX) ? 0 : fill + w4_unit_bytes(MX);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // The first units of the sequence; needs nothing but the weights. The ring must be free: a barrier lies between its last reads and this.
+    __device__ __forceinline__ void prefetch() {
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) fetch();
+    }
+    // All runs of the cursor's group whose job is below `limit`.
+    template <int PARTS, int MODE, int NT, bool LIST> __device__ __forceinline__ void work_group(const Group & r, const Scratch & sc, int limit = 0x7fffffff) {
+        float acc[2][2][4] = {};
+        Lane l;
+        begin_group<MX, PARTS, MODE, NT, LIST>(r, lane, sc, l);
+        const int group = cp.group;
+        const uint32_t words = ring + lane * 16, scale_at = ring + 1024 + (lane >> 2) * (MX ? 4 : 8);
+        do {
+            uint32_t b_at = 0, c_at = 0;
+            for (int n = cp.rem; n > 0; --n) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                __syncwarp();           // every lane's copies of this unit have landed, and the stage read last is free
+                fetch();
+                do_step<MX, PARTS, MODE, NT, LIST>(words + at, scale_at + at, b_at, c_at, l, acc);
+                at = at == (kStages - 1) * w4_unit_bytes(MX) ? 0 : at + w4_unit_bytes(MX);
+                b_at += step_x_bytes(PARTS, NT);
+                c_at += l.c_step;
+            }
+            end_run<MODE, NT>(r.n, lane, l, acc, [&](int row, int col, float v) { src.put(cp, row, col, v); });
+            src.next(cp);
+        } while (cp.live && cp.group == group && cp.job < limit);
+    }
+    // The runs of jobs below `limit`. Token sets staged with room for NT tokens, whose groups hold up to `NT` of them.
+    template <int PARTS, int NT, bool LIST> __device__ __forceinline__ void work(const Scratch & sc, int limit) {
+        while (cp.live && cp.job < limit) {
+            const Group r = src.group(cp);
+            if constexpr (!LIST) work_group<PARTS, mode_of(NT, PARTS), NT, LIST>(r, sc, limit);
+            else {
+                const int mode = mode_of(r.n, PARTS);
+                if (PARTS == 2 && mode == PACK) work_group<PARTS, PARTS == 2 ? PACK : ONE, NT, LIST>(r, sc, limit);
+                if constexpr (NT > (PARTS == 2 ? 4 : 0)) if (mode == ONE) work_group<PARTS, ONE, NT, LIST>(r, sc, limit);
+                if constexpr (NT > 8) if (mode == TWO) work_group<PARTS, TWO, NT, LIST>(r, sc, limit);
+            }
+        }
+    }
+    // Token sets staged with room for 1, 2, 4, 8 or 16, whichever holds them; none above MOST.
+    template <int PARTS, int MOST> __device__ __forceinline__ void work_sized(const Scratch & sc) {
+        while (cp.live) {
+            const Group r = src.group(cp);
+            if (r.n == 1) work_group<PARTS, mode_of(1, PARTS), 1, false>(r, sc);
+            if constexpr (MOST > 1) if (r.n == 2) work_group<PARTS, mode_of(2, PARTS), 2, false>(r, sc);
+            if constexpr (MOST > 2) if (r.n > 2 && r.n <= 4) work_group<PARTS, mode_of(4, PARTS), 4, false>(r, sc);
+            if constexpr (MOST > 4) if (r.n > 4 && r.n <= 8) work_group<PARTS, mode_of(8, PARTS), 8, false>(r, sc);
+            if constexpr (MOST > 8) if (r.n > 8) work_group<PARTS, mode_of(16, PARTS), 16, false>(r, sc);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+};
+
+// Room a set of n tokens is staged with.
+__host__ __device__ constexpr int room_for(int n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16; }
+
+// Parts (a power of two) the warps split the columns of a job into: as few as keep the warps evenly loaded, and at most `most`.
+// Warp w takes part w % ks of jobs w / ks, w / ks + kWarps / ks, ... The cost counts steps of the busiest warp and two steps' time
+// for every partial sum it writes.
+__host__ __device__ inline int split_columns(int jobs, int steps, int most) {
     int best = 1, best_cost = 0x7fffffff;
-    for (int ks = 1; ks <= kWarps; ks *= 2) {
+    for (int ks = 1; ks <= kWarps && ks <= most; ks *= 2) {
         if (ks > 1 && ks > steps) break;
         const int rounds = (jobs * ks + kWarps - 1) / kWarps;
         const int cost = rounds * ((steps + ks - 1) / ks + 2);
@@ -481,14 +577,47 @@ __host__ __device__ inline int split_columns(int jobs, int steps) {
 }
 
 // Range `part` of `parts` nearly equal ranges of [0, n).
-__host__ __device__ inline int part_begin(int n, int part, int parts) { return (int)((int64_t)n * part / parts); }
+__host__ __device__ inline int part_begin(int n, int part, int parts) {
+    const unsigned each = (unsigned)n / (unsigned)parts, more = (unsigned)n - each * parts;
+    return (int)(part * each + min((unsigned)part, more));
+}
 
 // ---- y = W x, and y = silu(W x) * (U x)
+
+// The inbox of a CTA: for each (row block, token) it owns, the sums of 32 rows from every (CTA, part of the columns) of the
+// cluster; with the gate, of gate and of up. Unit u of a round, block * tokens + token, belongs to CTA u % C. Rounds use two
+// inboxes in turn: whoever writes round r + 2's has met everyone after they read round r's.
+struct Inbox {
+    uint32_t base;              // shared-memory address
+    int bytes;                  // of one of the two
+    int rank, log_c, ks, per;   // per: matrices of a block
+
+    __device__ __forceinline__ void put(int round, int unit, int which, int sub, int row, float v) const {
+        const int from = (((unit >> log_c) * per + which) << log_c | rank) * ks + sub;
+        remote_store(remote_address(base + (round & 1) * bytes + (from * 32 + row) * 4, unit & ((1 << log_c) - 1)), v);
+    }
+    // Row `lane` of the sum over the cluster for the CTA's own unit number `mine`, in the order of the columns.
+    __device__ __forceinline__ float sum(int round, int mine, int which) const {
+        const int n = ks << log_c;
+        const uint32_t at = base + (round & 1) * bytes + ((mine * per + which) * n * 32 + (threadIdx.x & 31)) * 4;
+        float v = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) v += __uint_as_float(shared_u1(at + i * 128));
+        return v;
+    }
+};
+// Bytes of one inbox for `units` units of a round.
+__host__ __device__ inline int64_t inbox_bytes(int64_t units, int C, int ks, int per) { return (units + C - 1) / C * per * C * ks * 128; }
+// Row blocks a round can take with `room` bytes for one inbox; at least one.
+__host__ __device__ inline int blocks_per_round(int room, int tokens, int C, int ks, int per) {
+    const int units = room / (per * C * ks * 128) * C;      // whole units in every CTA
+    return max(1, units / tokens);
+}
 
 struct ProductArgs {
     const uint8_t * w, * u;
     Act x;
-    int T, n_in, n_out, tiles, steps;
+    int T, n_in, n_out, steps;
     const float * norm;
     float eps;
     const float * bias;
@@ -497,106 +626,90 @@ struct ProductArgs {
     void * y;
     uint32_t y_type;
     int64_t ld_y;
-    int jobs, clusters;             // a job is a pair of row tiles; with the gate, one tile of each matrix
-    int x_bytes, c_bytes, slots;    // shared memory: staged activations, start values, partial slots of T * kSlotCol floats
+    int blocks, clusters;           // row blocks, of gate and up together as of one matrix
+    int x_bytes, c_bytes, inbox;    // shared memory: staged activations, start values, one inbox
+    int ks;                         // parts of the columns, the same in every cluster: one inbox may have to do
 };
 
-template <bool MX, bool GLU> struct ProductSource {
+// Jobs: a row block; with the gate, block j of gate and of up are jobs 2 j and 2 j + 1.
+template <bool MX, int PARTS, bool GLU, int NT> struct ProductSource {
     const ProductArgs & a;
-    const uint8_t * list;
-    Staged x;
-    float * partial;
-    const Scratch & sc;
-    int job0, s0, n_steps, ks;
+    Staged x;                   // from this warp's columns on
+    Inbox inbox;
+    int job0, jobs, ks;         // jobs job0 .. job0 + jobs - 1
+    int sub, step, len;         // this warp's columns
+    int round, round0;          // the round, and its first job
 
-    __device__ __forceinline__ int len(int item, int) const {
-        const int sub = item % ks;
-        return part_begin(n_steps, sub + 1, ks) - part_begin(n_steps, sub, ks);
+    __device__ __forceinline__ void point(Cursor & c) const {
+        c.live = c.job < jobs;
+        const int job = job0 + c.job;
+        const size_t block = GLU ? job >> 1 : job;
+        c.p = (GLU && (job & 1) ? a.u : a.w) + (block * a.steps + step) * w4_unit_bytes(MX);
+        c.rem = len;
     }
-    __device__ __forceinline__ Run run(int item, int) const {
-        const int job = job0 + item / ks, sub = item % ks;
-        const int s = part_begin(n_steps, sub, ks);
-        const int t0 = GLU ? job : 2 * job, t1 = GLU ? job : min(2 * job + 1, a.tiles - 1);
-        Run r;
-        r.p0 = a.w + ((size_t)t0 * a.steps + s0 + s) * w4_unit_bytes(MX);
-        r.p1 = (GLU ? a.u : a.w) + ((size_t)t1 * a.steps + s0 + s) * w4_unit_bytes(MX);
-        r.len = 0;
-        r.x = {x.x + (size_t)s * (x.n * 64) * b_rows, MX ? nullptr : x.c + (size_t)s * 2 * x.n, x.n};
-        r.list = list;
-        r.n = a.T;
-        return r;
+    __device__ __forceinline__ void first(Cursor & c) const {
+        c.group = 0;
+        c.job = (threadIdx.x >> 5) / ks;
+        point(c);
     }
-    int b_rows;     // 2 * PARTS
-    __device__ __forceinline__ void put(int item, int, int row, int col, float v) const {
-        partial[((size_t)item * a.T + col) * kSlotCol + row] = v * sc.f1[0][col] * sc.f2[0][col];
+    __device__ __forceinline__ void next(Cursor & c) const {
+        c.job += kWarps / ks;
+        point(c);
+    }
+    __device__ __forceinline__ Group group(const Cursor &) const { return {x, nullptr, a.T, 0}; }
+    __device__ __forceinline__ void put(const Cursor & c, int row, int col, float v) const {
+        const int job = c.job - round0;
+        inbox.put(round, (GLU ? job >> 1 : job) * a.T + col, GLU ? job & 1 : 0, sub, row, v);
     }
 };
 
-template <bool MX, int PARTS, bool GLU, int MODE>
-__global__ void __launch_bounds__(kThreads, 2) w4_product_kernel(ProductArgs a) {
+template <bool MX, int PARTS, bool GLU, int NT>
+__global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_product_kernel(ProductArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Scratch sc;
-    __shared__ uint8_t list[kRowList];
+    constexpr int kPer = GLU ? 2 : 1;           // jobs of a row block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), C = (int)cluster_size();
     const int cluster = blockIdx.x / C;
+    cluster_arrive();
     const int s0 = part_begin(a.steps, rank, C), n_steps = part_begin(a.steps, rank + 1, C) - s0;
-    const int j_begin = part_begin(a.jobs, cluster, a.clusters), j_end = part_begin(a.jobs, cluster + 1, a.clusters);
-    const int ks = min(split_columns(j_end - j_begin, a.steps / C), a.slots);
-    const int per_round = max(1, a.slots / ks);
-    Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes), a.T};
-    float * partial = reinterpret_cast<float *>(smem + a.x_bytes + a.c_bytes);
-    if (threadIdx.x < kRowList) list[threadIdx.x] = (uint8_t)threadIdx.x;
+    const int b_begin = part_begin(a.blocks, cluster, a.clusters), blocks = part_begin(a.blocks, cluster + 1, a.clusters) - b_begin;
+    const int ks = a.ks;
+    const int per_round = blocks_per_round(a.inbox, a.T, C, ks, kPer);
+    uint8_t * const rings = smem + a.x_bytes + a.c_bytes;
+    const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
+    const Inbox inbox{smem_address(rings + ring_bytes(MX)), a.inbox, rank, __ffs(C) - 1, ks, kPer};
+    const int sub = warp % ks, step = part_begin(n_steps, sub, ks), len = part_begin(n_steps, sub + 1, ks) - step;
+    const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
+    if (threadIdx.x == 0) sc.zero = 0;
 
-    for (int j0 = j_begin; j0 < j_end; j0 += per_round) {
-        const int jobs = min(per_round, j_end - j0);
-        ProductSource<MX, GLU> src{a, list, x, partial, sc, j0, s0, n_steps, ks, 2 * PARTS};
-        Stream<MX, PARTS, 1 << MODE, ProductSource<MX, GLU>> stream(src, jobs * ks, 1);
-        stream.prefetch();
-        if (j0 == j_begin) {
-            // the weights above are the library's own; everything below is the caller's
-            pdl_trigger();
-            pdl_wait();
-            stage<MX, PARTS>(a.x, [](int t) { return (int64_t)t; }, a.T, s0 * 64, n_steps, a.n_in, a.norm, x, sc, 0);
-            __syncthreads();
-        }
-        stream.work();
+    ProductSource<MX, PARTS, GLU, NT> src{a, x_warp, inbox, b_begin * kPer, blocks * kPer, ks, sub, s0 + step, len, 0, 0};
+    Stream<MX, ProductSource<MX, PARTS, GLU, NT>> stream(src, rings);
+    stream.prefetch();
+    // the weights above are the library's own; everything below is the caller's
+    pdl_trigger();
+    pdl_wait();
+    stage_tokens<MX, PARTS>(a.x, a.T, NT, s0, n_steps, a.n_in, a.norm, x, sc, rank, C);
+    __syncthreads();
+    for (int b0 = 0; b0 < blocks; b0 += per_round, ++src.round) {
+        const int now = min(per_round, blocks - b0);
+        src.round0 = b0 * kPer;
+        stream.template work<PARTS, NT, false>(sc, (b0 + now) * kPer);
         cluster_sync();
-        // 32 rows of one token at a time: the cluster's partial sums in the order of the columns
-        const uint32_t base = smem_address(partial);
-        for (int u = rank + C * warp; u < jobs * a.T; u += C * kWarps) {
-            const int job = u / a.T, t = u % a.T;
-            float v = 0.f;
-            for (int c = 0; c < C; ++c) {
-                const uint32_t at = remote_address(base, c) + (((size_t)job * ks * a.T + t) * kSlotCol + lane) * 4;
-                for (int i = 0; i < ks; ++i) v += remote_load(at + (uint32_t)(i * a.T * kSlotCol * 4));
-            }
-            if (a.norm) {
-                float ss = lane < C ? remote_load(remote_address(smem_address(&sc.ss[t]), lane)) : 0.f;
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                ss = __shfl_sync(0xffffffffu, ss, 0);
-                v *= rsqrtf(ss / (float)a.n_in + a.eps);
-            }
-            int row;
-            if constexpr (GLU) {
-                const float up = __shfl_down_sync(0xffffffffu, v, 16);
-                v = v / (1.f + expf(-v)) * up;
-                row = lane < 16 ? (j0 + job) * 16 + lane : a.n_out;
-            } else {
-                row = (j0 + job) * 32 + lane;
-            }
+        // 32 rows of one token at a time
+        for (int i = warp; i * C + rank < now * a.T; i += kWarps) {
+            const int unit = i * C + rank, b = unit / a.T, t = unit - b * a.T;
+            float v = inbox.sum(src.round, i, 0);
+            const float factor = a.norm ? rms_factor(sc, t, C, a.n_in, a.eps) : 1.f;
+            v *= factor;
+            if constexpr (GLU) v = v / (1.f + expf(-v)) * (inbox.sum(src.round, i, 1) * factor);
+            const int row = (b_begin + b0 + b) * 32 + lane;
             if (row < a.n_out) {
                 if (a.bias) v += a.bias[row];
                 if (a.residual) v += load1(Act{a.residual, a.ld_residual, a.y_type, false}, t, row);
                 store1(a.y, a.y_type, t * a.ld_y + row, v);
             }
         }
-        cluster_sync();     // nobody reuses or leaves the slots that others still read
-    }
-    if (j_begin >= j_end) {
-        pdl_trigger();
-        pdl_wait();
     }
 }
 
@@ -608,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_product_kernel(ProductArgs a) 
 // experts' down matrices as one long reduction: a cluster owns a range of y's rows, its CTAs divide the experts' concatenated columns,
 // and the sum over experts is part of the sum over the cluster.
 
-struct MoeMeta {                        // in the workspace, in front of h
+struct alignas(16) MoeMeta {                     // in the workspace, in front of h
     int32_t n;                          // chosen experts
     int32_t pad[3];
     uint16_t expert[kW4MaxExperts];     // ascending
@@ -622,7 +735,7 @@ struct MoeArgs {
     const float * router;
     Act x;
     int T, E, k, d, ff;
-    int tiles_ff, steps_d, tiles_d, steps_ff;
+    int blocks_ff, steps_d, blocks_d, steps_ff;
     bool normalise;
     const float * norm;
     float eps;
@@ -636,7 +749,7 @@ struct MoeArgs {
     MoeMeta * meta;
     float * h;
     int64_t ld_h;
-    int clusters, x_bytes, c_bytes, logit_bytes, partial_floats;
+    int clusters, x_bytes, c_bytes, logit_bytes, inbox, partial;        // shared memory, in bytes
 };
 
 struct Picks {
@@ -646,52 +759,59 @@ struct Picks {
     uint16_t unique[kW4MaxExperts];
     uint8_t count[kW4MaxExperts];                   // of unique[i]
     uint8_t token[kW4MaxExperts][kRowList];
-    int warp_unique[kWarps];
+    uint16_t pair[kW4MaxExperts][kRowList];         // token * n_used + rank of the expert among the token's
+    uint32_t mask[kW4MaxExperts];                   // by expert: the tokens that chose it
+    uint8_t rank[kW4MaxExperts][kRowList];
+    int warp_unique[kWarps], warp_most[kWarps];
     int n, most;                                    // unique experts, largest count
 };
+
+// Sums each of the 16 values of a lane over the warp; lane i ends up with value i >> 1 (lanes 2 i and 2 i + 1 alike).
+__device__ __forceinline__ float warp_sums16(float (&v)[16]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int half = 8; half > 0; half >>= 1) {
+        const bool upper = lane & (2 * half);
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float send = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2 * half);
+        }
+    }
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+}
 
 // The CTA's columns' part of every (token, expert) logit.
 __device__ void partial_logits(const MoeArgs & a, int k0, int k1, float * out) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int EB = 4, TB = 4;       // experts and tokens a warp takes at once
     const Act router{a.router, a.d, GGML_F32, (uintptr_t)a.router % 16 == 0};
-    for (int e0 = warp * EB; e0 < a.E; e0 += kWarps * EB) {
-        for (int t0 = 0; t0 < a.T; t0 += TB) {
-            float acc[EB][TB] = {};
-            for (int k = k0 + lane * 4; k < k1; k += 128) {
-                float g[4] = {1.f, 1.f, 1.f, 1.f};
-                if (a.norm) {
+    const int groups_t = (a.T + TB - 1) / TB, items = (a.E + EB - 1) / EB * groups_t;
+    for (int item = warp; item < items; item += kWarps) {
+        const int e0 = item / groups_t * EB, t0 = item % groups_t * TB;
+        float acc[EB * TB] = {};
+        for (int k = k0 + lane * 4; k < k1; k += 128) {
+            float r[EB][4], v[TB][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) g[i] = a.norm[k + i];
-                }
-                float r[EB][4];
-#pragma unroll
-                for (int e = 0; e < EB; ++e) load4(router, min(e0 + e, a.E - 1), k, r[e]);
-#pragma unroll
-                for (int t = 0; t < TB; ++t) {
-                    if (t0 + t >= a.T) break;
-                    float v[4];
-                    load4(a.x, t0 + t, k, v);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float f = v[i] * g[i];
-#pragma unroll
-                        for (int e = 0; e < EB; ++e) acc[e][t] += r[e][i] * f;
-                    }
-                }
-            }
+            for (int e = 0; e < EB; ++e) load4(router, min(e0 + e, a.E - 1), k, r[e]);
 #pragma unroll
             for (int t = 0; t < TB; ++t) {
-                if (t0 + t >= a.T) break;
-#pragma unroll
-                for (int e = 0; e < EB; ++e) {
-                    float v = acc[e][t];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    if (lane == 0 && e0 + e < a.E) out[(t0 + t) * a.E + e0 + e] = v;
+                v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.f;
+                if (t0 + t < a.T) {
+                    load4(a.x, t0 + t, k, v[t]);
+                    if (a.norm) scale4(v[t], a.norm + k);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < EB; ++e)
+#pragma unroll
+                    for (int t = 0; t < TB; ++t) acc[e * TB + t] += r[e][i] * v[t][i];
         }
+        const float sum = warp_sums16(acc);
+        const int e = e0 + (lane >> 1) / TB, t = t0 + (lane >> 1) % TB;
+        if (!(lane & 1) && e < a.E && t < a.T) out[t * a.E + e] = sum;
     }
 }
 
@@ -718,26 +838,32 @@ __device__ void pick_experts(const float * logits, int E, int k, bool normalise,
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    uint32_t taken = 0;
+    // key: the probability's bits, which order like the probabilities, plus one; a NaN behind every number, taken ones at zero
+    uint32_t key[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        p[j] /= sum;
+        key[j] = lane + 32 * j < E ? (p[j] >= 0.f ? __float_as_uint(p[j]) + 2u : 1u) : 0u;
+    }
     float chosen = 0.f;
     for (int pick = 0; pick < k; ++pick) {
-        float best = -2.f, value = 0.f;
-        int at = 0x7fffffff;
+        uint32_t best = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) best = max(best, key[j]);
+        best = __reduce_max_sync(0xffffffffu, best);
+        uint32_t at = 0xffffffffu;
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j) if (key[j] == best) at = lane + 32 * j;
+        at = __reduce_min_sync(0xffffffffu, at);
+        float value = 0.f;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int e = lane + 32 * j;
-            if (e >= E || (taken >> j & 1)) continue;
-            const float v = p[j] / sum;
-            const float key = v >= 0.f ? v : -1.f;      // NaN behind every number
-            if (key > best) { best = key; value = v; at = e; }
+            if (at == (uint32_t)(lane + 32 * j)) {
+                value = p[j];
+                key[j] = 0;
+            }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ob = __shfl_xor_sync(0xffffffffu, best, o), ov = __shfl_xor_sync(0xffffffffu, value, o);
-            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-            if (ob > best || (ob == best && oa < at)) { best = ob; value = ov; at = oa; }
-        }
-        if ((at & 31) == lane) taken |= 1u << (at >> 5);
+        value = __shfl_sync(0xffffffffu, value, at & 31);
         if (lane == 0) { expert[pick] = (uint16_t)at; weight[pick] = value; }
         chosen += value;
     }
@@ -747,110 +873,118 @@ __device__ void pick_experts(const float * logits, int E, int k, bool normalise,
     }
 }
 
-// The chosen experts in ascending order with their tokens, from the picks of all tokens.
+// The chosen experts in ascending order with their tokens, from the picks of all tokens. Picks::mask is zero before.
 __device__ void group_picks(const MoeArgs & a, Picks & p, MoeMeta * meta) {
     const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
-    uint32_t mask = 0;                  // tokens that chose expert e
-    if (e < a.E) {
-        for (int i = 0; i < a.T * a.k; ++i)
-            if (p.expert[i] == e) mask |= 1u << (i / a.k);
+    for (int i = e; i < a.T * a.k; i += kThreads) {
+        const int t = i / a.k, expert = p.expert[i];
+        atomicOr(&p.mask[expert], 1u << t);
+        p.rank[expert][t] = (uint8_t)(i - t * a.k);
     }
-    const uint32_t chosen = __ballot_sync(0xffffffffu, mask != 0);
-    if (lane == 0) p.warp_unique[warp] = __popc(chosen);
-    if (e == 0) p.most = 1;
     __syncthreads();
-    int before = 0, all = 0;
+    const uint32_t mask = p.mask[e];                // tokens that chose expert e
+    const uint32_t chosen = __ballot_sync(0xffffffffu, mask != 0);
+    const int n = __popc(mask);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, (uint32_t)n);
+    if (lane == 0) { p.warp_unique[warp] = __popc(chosen); p.warp_most[warp] = (int)most; }
+    __syncthreads();
+    int before = 0, all = 0, top = 1;
     for (int w = 0; w < kWarps; ++w) {
         if (w < warp) before += p.warp_unique[w];
         all += p.warp_unique[w];
+        top = max(top, p.warp_most[w]);
     }
     if (mask) {
         const int u = before + __popc(chosen & ((1u << lane) - 1u));
-        const int n = __popc(mask);
         p.unique[u] = (uint16_t)e;
         p.count[u] = (uint8_t)n;
-        atomicMax(&p.most, n);
-        int at = 0;
-        for (uint32_t m = mask; m; m &= m - 1) p.token[u][at++] = (uint8_t)(__ffs(m) - 1);
+        int i = 0;
+        for (uint32_t m = mask; m; m &= m - 1, ++i) {
+            const int t = __ffs(m) - 1;
+            p.token[u][i] = (uint8_t)t;
+            p.pair[u][i] = (uint16_t)(t * a.k + p.rank[e][t]);
+            if (meta) meta->pair[u][i] = p.pair[u][i];
+        }
         if (meta) {
             meta->expert[u] = (uint16_t)e;
             meta->count[u] = (uint16_t)n;
-            for (int i = 0; i < n; ++i) {
-                const int t = p.token[u][i];
-                int j = 0;
-                while (j < a.k - 1 && p.expert[t * a.k + j] != e) ++j;
-                meta->pair[u][i] = (uint16_t)(t * a.k + j);
-            }
         }
     }
     if (e == 0) {
         p.n = all;
+        p.most = top;
         if (meta) meta->n = all;
     }
     __syncthreads();
 }
 
-template <bool MX, int PARTS> struct GateUpSource {
+// Jobs: block j of an expert's gate and of its up matrix are jobs 2 j and 2 j + 1, experts one behind the other.
+template <bool MX, int PARTS, int NT> struct GateUpSource {
     const MoeArgs & a;
     const Picks & p;
     Staged x;
-    float * partial;
-    const Scratch & sc;
-    int job0, s0, n_steps, ks, most;
+    Inbox inbox;
+    int job0, jobs, ks, most;
+    int sub, step, len;
+    int round, round0;
 
-    __device__ __forceinline__ int len(int item, int) const {
-        const int sub = item % ks;
-        return part_begin(n_steps, sub + 1, ks) - part_begin(n_steps, sub, ks);
+    // Cursor::group is the expert's place among the chosen ones.
+    __device__ __forceinline__ void point(Cursor & c) const {
+        c.live = c.job < jobs;
+        if (!c.live) return;
+        const int job = job0 + c.job, block = job >> 1;
+        c.group = block / a.blocks_ff;
+        const int e = p.unique[c.group];
+        c.p = (job & 1 ? a.up + e * a.up_expert : a.gate + e * a.gate_expert) + ((size_t)(block - c.group * a.blocks_ff) * a.steps_d + step) * w4_unit_bytes(MX);
+        c.rem = len;
     }
-    __device__ __forceinline__ Run run(int item, int) const {
-        const int job = job0 + item / ks, s = part_begin(n_steps, item % ks, ks);
-        const int u = job / a.tiles_ff, tile = job % a.tiles_ff;
-        const size_t at = ((size_t)tile * a.steps_d + s0 + s) * w4_unit_bytes(MX);
-        const int e = p.unique[u];
-        Run r;
-        r.p0 = a.gate + e * a.gate_expert + at;
-        r.p1 = a.up + e * a.up_expert + at;
-        r.x = {x.x + (size_t)s * (2 * PARTS * 64) * x.n, MX ? nullptr : x.c + (size_t)s * 2 * x.n, x.n};
-        r.list = p.token[u];
-        r.n = p.count[u];
-        return r;
+    __device__ __forceinline__ void first(Cursor & c) const {
+        c.job = (threadIdx.x >> 5) / ks;
+        point(c);
     }
-    __device__ __forceinline__ void put(int item, int, int row, int col, float v) const {
-        const int tok = p.token[(job0 + item / ks) / a.tiles_ff][col];
-        partial[((size_t)item * most + col) * kSlotCol + row] = v * sc.f1[0][tok] * sc.f2[0][tok];
+    __device__ __forceinline__ void next(Cursor & c) const {
+        c.job += kWarps / ks;
+        point(c);
+    }
+    __device__ __forceinline__ Group group(const Cursor & c) const { return {x, p.token[c.group], p.count[c.group], 0}; }
+    __device__ __forceinline__ void put(const Cursor & c, int row, int col, float v) const {
+        const int job = c.job - round0;
+        inbox.put(round, (job >> 1) * most + col, job & 1, sub, row, v);
     }
 };
 
-template <bool MX, int PARTS, int MODES>
-__global__ void __launch_bounds__(kThreads, 2) w4_moe_gate_up_kernel(MoeArgs a) {
+template <bool MX, int PARTS, int NT>
+__global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_moe_gate_up_kernel(MoeArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Scratch sc;
     __shared__ Picks picks;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), C = (int)cluster_size();
     const int cluster = blockIdx.x / C;
+    cluster_arrive();
     const int s0 = part_begin(a.steps_d, rank, C), n_steps = part_begin(a.steps_d, rank + 1, C) - s0;
-    Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes), a.T};
+    const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
     float * mine = reinterpret_cast<float *>(smem + a.x_bytes + a.c_bytes);         // this CTA's part of the logits
     float * logits = mine + a.logit_bytes / 4;
-    float * partial = logits + a.logit_bytes / 4;
+    uint8_t * const rings = smem + a.x_bytes + a.c_bytes + 2 * a.logit_bytes;
+    if (threadIdx.x == 0) sc.zero = 0;
+    picks.mask[threadIdx.x] = 0;
 
     pdl_trigger();
     pdl_wait();
-    stage<MX, PARTS>(a.x, [](int t) { return (int64_t)t; }, a.T, s0 * 64, n_steps, a.d, a.norm, x, sc, 0);
     partial_logits(a, s0 * 64, min(a.d, (s0 + n_steps) * 64), mine);
+    stage_tokens<MX, PARTS>(a.x, a.T, NT, s0, n_steps, a.d, a.norm, x, sc, rank, C);
     cluster_sync();
-    if (threadIdx.x < a.T) {
-        float ss = 0.f;
-        for (int c = 0; c < C; ++c) ss += remote_load(remote_address(smem_address(&sc.ss[threadIdx.x]), c));
-        picks.rstd[threadIdx.x] = a.norm ? rsqrtf(ss / (float)a.d + a.eps) : 1.f;
-    }
-    __syncthreads();
     for (int i = threadIdx.x; i < a.T * a.E; i += kThreads) {
+        float part[kMaxCluster];
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) part[c] = c < C ? remote_load(remote_address(smem_address(mine + i), c)) : 0.f;
         float v = 0.f;
-        for (int c = 0; c < C; ++c) v += remote_load(remote_address(smem_address(mine), c) + i * 4);
-        logits[i] = v * picks.rstd[i / a.E];
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) v += part[c];
+        logits[i] = a.norm ? v * rms_factor(sc, i / a.E, C, a.d, a.eps) : v;
     }
+    if (threadIdx.x < a.T) picks.rstd[threadIdx.x] = a.norm ? rms_factor(sc, threadIdx.x, C, a.d, a.eps) : 1.f;
     __syncthreads();
     for (int t = warp; t < a.T; t += kWarps) pick_experts(logits + t * a.E, a.E, a.k, a.normalise, picks.expert + t * a.k, picks.weight + t * a.k);
     __syncthreads();
@@ -863,154 +997,188 @@ __global__ void __launch_bounds__(kThreads, 2) w4_moe_gate_up_kernel(MoeArgs a) 
         }
     }
 
-    const int total = picks.n * a.tiles_ff, most = picks.most;
-    const int j_begin = part_begin(total, cluster, a.clusters), j_end = part_begin(total, cluster + 1, a.clusters);
-    const int slots = a.partial_floats / (most * kSlotCol);
-    const int ks = min(split_columns(j_end - j_begin, a.steps_d / C), slots);
-    const int per_round = slots / ks;
-    for (int j0 = j_begin; j0 < j_end; j0 += per_round) {
-        const int jobs = min(per_round, j_end - j0);
-        GateUpSource<MX, PARTS> src{a, picks, x, partial, sc, j0, s0, n_steps, ks, most};
-        Stream<MX, PARTS, MODES, GateUpSource<MX, PARTS>> stream(src, jobs * ks, 1);
-        stream.prefetch();
-        stream.work();
+    const int total = picks.n * a.blocks_ff, most = picks.most;
+    const int b_begin = part_begin(total, cluster, a.clusters), blocks = part_begin(total, cluster + 1, a.clusters) - b_begin;
+    const int ks = split_columns(blocks * 2, a.steps_d / C, (int)(a.inbox / inbox_bytes(most, C, 1, 2)));
+    const int per_round = blocks_per_round(a.inbox, most, C, ks, 2);
+    const int sub = warp % ks, step = part_begin(n_steps, sub, ks), len = part_begin(n_steps, sub + 1, ks) - step;
+    const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
+    const Inbox inbox{smem_address(rings + ring_bytes(MX)), a.inbox, rank, __ffs(C) - 1, ks, 2};
+    GateUpSource<MX, PARTS, NT> src{a, picks, x_warp, inbox, 2 * b_begin, 2 * blocks, ks, most, sub, s0 + step, len, 0, 0};
+    Stream<MX, GateUpSource<MX, PARTS, NT>> stream(src, rings);
+    stream.prefetch();
+    for (int b0 = 0; b0 < blocks; b0 += per_round, ++src.round) {
+        const int now = min(per_round, blocks - b0);
+        src.round0 = 2 * b0;
+        stream.template work<PARTS, NT, (NT > 1)>(sc, 2 * (b0 + now));
         cluster_sync();
-        const uint32_t base = smem_address(partial);
-        for (int i = rank + C * warp; i < jobs * most; i += C * kWarps) {
-            const int job = i / most, col = i % most;
-            const int u = (j0 + job) / a.tiles_ff, tile = (j0 + job) % a.tiles_ff;
+        for (int i = warp; i * C + rank < now * most; i += kWarps) {
+            const int unit = i * C + rank, b = unit / most, col = unit - b * most;
+            const int u = (b_begin + b0 + b) / a.blocks_ff, row = ((b_begin + b0 + b) - u * a.blocks_ff) * 32 + lane;
             if (col >= picks.count[u]) continue;
-            float v = 0.f;
-            for (int c = 0; c < C; ++c) {
-                const uint32_t at = remote_address(base, c) + (((size_t)job * ks * most + col) * kSlotCol + lane) * 4;
-                for (int s = 0; s < ks; ++s) v += remote_load(at + (uint32_t)(s * most * kSlotCol * 4));
-            }
-            const int t = picks.token[u][col];
-            v *= picks.rstd[t];
-            const float b = __shfl_down_sync(0xffffffffu, v, 16);
-            int j = 0;
-            while (j < a.k - 1 && picks.expert[t * a.k + j] != picks.unique[u]) ++j;
-            const int pair = t * a.k + j, row = tile * 16 + lane;
-            if (lane < 16 && row < a.ff) a.h[pair * a.ld_h + row] = picks.weight[pair] * (v / (1.f + expf(-v)) * b);
+            const int t = picks.token[u][col], pair = picks.pair[u][col];
+            const float v = inbox.sum(src.round, i, 0) * picks.rstd[t], up = inbox.sum(src.round, i, 1) * picks.rstd[t];
+            if (row < a.ff) a.h[pair * a.ld_h + row] = picks.weight[pair] * (v / (1.f + expf(-v)) * up);
         }
-        cluster_sync();
     }
-    cluster_sync();     // nobody leaves while its logits are read
+    if (blocks == 0) cluster_sync();        // nobody leaves while its logits are read
 }
 
+// Consecutive steps of one chosen expert.
 struct Seg {
-    int u, s0, len, x_off, c_off, n;
+    int u, expert, s0, len, x_off, c_off, n, row0;      // row0: tokens of the segments before
 };
 struct DownTable {
     Seg seg[kMaxSegs];
-    int n;
+    uint8_t token[kMaxSegs][kRowList];
+    int n, rows;
     int next;           // the step behind the chunk
 };
+
+// The segments from step p on, as many as `room` bytes of shared memory for activations hold. By one warp.
+template <bool MX> __device__ void cut_segments(const MoeArgs & a, const MoeMeta & meta, int p, int end, int room, DownTable & table) {
+    const int lane = threadIdx.x & 31;
+    const int u = p / a.steps_ff + lane;
+    const int from = max(p, u * a.steps_ff), whole = lane < kMaxSegs ? max(0, min(end, (u + 1) * a.steps_ff) - from) : 0;
+    const int tokens = whole > 0 ? meta.count[u] : 0, nt = room_for(tokens);
+    const int bytes = (whole * step_bytes(MX, 2, nt) + 15) / 16 * 16;
+    int used = bytes, rows = tokens;        // inclusive sums over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int b = __shfl_up_sync(0xffffffffu, used, o), r = __shfl_up_sync(0xffffffffu, rows, o);
+        if (lane >= o) { used += b; rows += r; }
+    }
+    used -= bytes;
+    rows -= tokens;
+    const int len = max(0, min(whole, (room - used) / step_bytes(MX, 2, nt)));
+    // the first segment that does not fit ends the chunk; room for one step of the first is always there
+    const uint32_t cut = __ballot_sync(0xffffffffu, len < whole);
+    const int last = cut ? __ffs(cut) - 1 : 31;
+    const uint32_t kept = __ballot_sync(0xffffffffu, len > 0 && lane <= last);
+    const int n = __popc(kept);
+    if (kept >> lane & 1) {
+        const int x_bytes = len * step_x_bytes(2, nt);
+        table.seg[lane] = {u, meta.expert[u], from - u * a.steps_ff, len, used, used + x_bytes, tokens, rows};
+        for (int i = 0; i < tokens; ++i) table.token[lane][i] = (uint8_t)(meta.pair[u][i] / a.k);
+        if (lane == n - 1) {
+            table.n = n;
+            table.rows = rows + tokens;
+            table.next = from + len;
+        }
+    }
+}
 
 template <bool MX> struct DownSource {
     const MoeArgs & a;
     const DownTable & table;
     uint8_t * smem;
     float * partial;
-    const Scratch & sc;
-    const uint8_t * identity;
-    int job0, ks;
+    int job0, jobs, ks, sub;
 
-    __device__ __forceinline__ int len(int item, int seg) const {
-        const int n = table.seg[seg].len, sub = item % ks;
-        return part_begin(n, sub + 1, ks) - part_begin(n, sub, ks);
+    // Cursor::group is the segment: all jobs of one, then the next.
+    __device__ __forceinline__ void point(Cursor & c) const {
+        while (true) {
+            c.live = c.group < table.n;
+            if (!c.live) return;
+            const Seg & g = table.seg[c.group];
+            const int s = part_begin(g.len, sub, ks);
+            c.rem = part_begin(g.len, sub + 1, ks) - s;
+            if (c.job < jobs && c.rem > 0) {
+                c.p = a.down + g.expert * a.down_expert + ((size_t)(job0 + c.job) * a.steps_ff + g.s0 + s) * w4_unit_bytes(MX);
+                return;
+            }
+            ++c.group;
+            c.job = (threadIdx.x >> 5) / ks;
+        }
     }
-    __device__ __forceinline__ Run run(int item, int seg) const {
-        const Seg & g = table.seg[seg];
-        const int job = job0 + item / ks, s = part_begin(g.len, item % ks, ks);
-        const uint8_t * e = a.down + a.meta->expert[g.u] * a.down_expert;
-        Run r;
-        r.p0 = e + ((size_t)(2 * job) * a.steps_ff + g.s0 + s) * w4_unit_bytes(MX);
-        r.p1 = e + ((size_t)min(2 * job + 1, a.tiles_d - 1) * a.steps_ff + g.s0 + s) * w4_unit_bytes(MX);
-        r.x = {smem + g.x_off + (size_t)s * (2 * 2 * 64) * g.n, MX ? nullptr : reinterpret_cast<float *>(smem + g.c_off) + (size_t)s * 2 * g.n, g.n};
-        r.list = identity;
-        r.n = g.n;
-        return r;
+    __device__ __forceinline__ void first(Cursor & c) const {
+        c.group = 0;
+        c.job = (threadIdx.x >> 5) / ks;
+        point(c);
     }
-    __device__ __forceinline__ void put(int item, int seg, int row, int col, float v) const {
-        const int tok = a.meta->pair[table.seg[seg].u][col] / a.k;
-        partial[((size_t)item * a.T + tok) * kSlotCol + row] += v * sc.f1[seg][col] * sc.f2[seg][col];
+    __device__ __forceinline__ void next(Cursor & c) const {
+        c.job += kWarps / ks;
+        point(c);
+    }
+    __device__ __forceinline__ Group group(const Cursor & c) const {
+        const Seg & g = table.seg[c.group];
+        const int s = part_begin(g.len, sub, ks), nt = room_for(g.n);
+        return {{smem + g.x_off + s * step_x_bytes(2, nt), reinterpret_cast<float *>(smem + g.c_off + s * step_c_bytes(MX, nt))}, nullptr, g.n, c.group};
+    }
+    __device__ __forceinline__ void put(const Cursor & c, int row, int col, float v) const {
+        partial[((c.job * ks + sub) * a.T + table.token[c.group][col]) * kSlotCol + row] += v;
     }
 };
 
-template <bool MX, int MODES>
-__global__ void __launch_bounds__(kThreads, 2) w4_moe_down_kernel(MoeArgs a) {
+template <bool MX, int MOST>
+__global__ void __launch_bounds__(kThreads, MOST > 8 ? 2 : 3) w4_moe_down_kernel(MoeArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Scratch sc;
     __shared__ DownTable table;
-    __shared__ uint8_t identity[kRowList];
+    __shared__ MoeMeta meta;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), C = (int)cluster_size();
     const int cluster = blockIdx.x / C;
-    float * partial = reinterpret_cast<float *>(smem + a.x_bytes);
-    if (threadIdx.x < kRowList) identity[threadIdx.x] = (uint8_t)threadIdx.x;
+    cluster_arrive();
+    uint8_t * const rings = smem + a.x_bytes;
+    float * partial = reinterpret_cast<float *>(rings + ring_bytes(MX));
+    const Inbox inbox{smem_address(rings + ring_bytes(MX) + a.partial), a.inbox, rank, __ffs(C) - 1, 1, 1};
+    const int j_begin = part_begin(a.blocks_d, cluster, a.clusters), j_end = part_begin(a.blocks_d, cluster + 1, a.clusters);
+    if (threadIdx.x == 0) sc.zero = 0;
     pdl_trigger();
     pdl_wait();
-    const int total = a.meta->n * a.steps_ff;       // the chosen experts' columns, one behind the other
+    {
+        const int4 * from = reinterpret_cast<const int4 *>(a.meta);
+        int4 * to = reinterpret_cast<int4 *>(&meta);
+        const int reach = min(a.E, a.T * a.k);
+        for (int i = threadIdx.x; i < (int)((offsetof(MoeMeta, pair) + sizeof(meta.pair[0]) * reach) / 16); i += kThreads) to[i] = from[i];
+    }
+    cluster_wait();
+    __syncthreads();
+    const int total = meta.n * a.steps_ff;          // the chosen experts' columns, one behind the other
     const int begin = part_begin(total, rank, C), end = part_begin(total, rank + 1, C);
-    const int jobs_all = (a.tiles_d + 1) / 2;
-    const int j_begin = part_begin(jobs_all, cluster, a.clusters), j_end = part_begin(jobs_all, cluster + 1, a.clusters);
-    const int slots = a.partial_floats / (a.T * kSlotCol);
-    const int ks = min(split_columns(j_end - j_begin, max(1, total / C)), slots);
-    const int per_round = slots / ks;
+    const int slot = a.T * kSlotCol * 4;
+    const int ks = split_columns(j_end - j_begin, max(1, total / C), a.partial / slot);
+    const int per_round = min(a.partial / (slot * ks), blocks_per_round(a.inbox, a.T, C, 1, 1));
     const Act h{a.h, a.ld_h, GGML_F32, true};
-    for (int j0 = j_begin; j0 < j_end; j0 += per_round) {
+    int round = 0;
+    for (int j0 = j_begin; j0 < j_end; j0 += per_round, ++round) {
         const int jobs = min(per_round, j_end - j0);
         for (int i = threadIdx.x; i < jobs * ks * a.T * kSlotCol; i += kThreads) partial[i] = 0.f;
-        for (int p = begin; p < end;) {
-            if (threadIdx.x == 0) {
-                // as many steps as fit into the shared memory for activations
-                int n = 0, used = 0, at = p;
-                while (at < end && n < kMaxSegs) {
-                    const int u = at / a.steps_ff, off = at % a.steps_ff, tokens = a.meta->count[u];
-                    const int each = staged_x_bytes(1, 2, tokens) + staged_c_bytes(MX, 1, tokens);
-                    const int len = min(min(a.steps_ff - off, end - at), (a.x_bytes - used - 16) / each);
-                    if (len <= 0) break;
-                    const int x_bytes = staged_x_bytes(len, 2, tokens);
-                    table.seg[n] = {u, off, len, used, used + x_bytes, tokens};
-                    used += (x_bytes + staged_c_bytes(MX, len, tokens) + 15) / 16 * 16;
-                    at += len;
-                    ++n;
-                }
-                table.n = n;
-                table.next = at;
-            }
+        for (int p = begin; p < end; p = table.next) {
+            __syncthreads();            // the table, the activations and the slots are free (or cleared)
+            if (warp == 0) cut_segments<MX>(a, meta, p, end, a.x_bytes - 16, table);
             __syncthreads();
-            DownSource<MX> src{a, table, smem, partial, sc, identity, j0, ks};
-            Stream<MX, 2, MODES, DownSource<MX>> stream(src, jobs * ks, table.n);
+            const DownSource<MX> src{a, table, smem, partial, j0, jobs, ks, warp % ks};
+            Stream<MX, DownSource<MX>> stream(src, rings);
             stream.prefetch();
-            for (int i = 0; i < table.n; ++i) {
-                const Seg & g = table.seg[i];
-                const uint16_t * pair = a.meta->pair[g.u];
-                stage<MX, 2>(h, [pair](int t) { return (int64_t)pair[t]; }, g.n, g.s0 * 64, g.len, a.ff, nullptr,
-                             Staged{smem + g.x_off, reinterpret_cast<float *>(smem + g.c_off), g.n}, sc, i);
-            }
+            stage_rows<MX, 2, false>(h, table.rows, a.ff, nullptr, sc, [&](int i) {
+                int n = 0;
+                while (n + 1 < table.n && i >= table.seg[n + 1].row0) ++n;
+                const Seg & g = table.seg[n];
+                return StageRow{(int64_t)meta.pair[g.u][i - g.row0], g.s0 * 64, g.len, room_for(g.n), i - g.row0, n,
+                                Staged{smem + g.x_off, reinterpret_cast<float *>(smem + g.c_off)}};
+            }, [](int, float) {});
             __syncthreads();
-            stream.work();
-            p = table.next;
-            __syncthreads();
+            stream.template work_sized<2, MOST>(sc);
+        }
+        __syncthreads();
+        for (int unit = warp; unit < jobs * a.T; unit += kWarps) {
+            const int job = unit / a.T, t = unit - job * a.T;
+            float v = 0.f;
+            for (int i = 0; i < ks; ++i) v += partial[((job * ks + i) * a.T + t) * kSlotCol + lane];
+            inbox.put(round, unit, 0, 0, lane, v);
         }
         cluster_sync();
-        const uint32_t base = smem_address(partial);
-        for (int u = rank + C * warp; u < jobs * a.T; u += C * kWarps) {
-            const int job = u / a.T, t = u % a.T;
-            float v = 0.f;
-            for (int c = 0; c < C; ++c) {
-                const uint32_t at = remote_address(base, c) + (((size_t)job * ks * a.T + t) * kSlotCol + lane) * 4;
-                for (int i = 0; i < ks; ++i) v += remote_load(at + (uint32_t)(i * a.T * kSlotCol * 4));
-            }
+        for (int i = warp; i * C + rank < jobs * a.T; i += kWarps) {
+            const int unit = i * C + rank, job = unit / a.T, t = unit - job * a.T;
+            float v = inbox.sum(round, i, 0);
             const int row = (j0 + job) * 32 + lane;
             if (row < a.d) {
                 if (a.residual) v += load1(Act{a.residual, a.ld_residual, a.y_type, false}, t, row);
                 store1(a.y, a.y_type, t * a.ld_y + row, v);
             }
         }
-        cluster_sync();
     }
 }
 
@@ -1020,18 +1188,18 @@ __global__ void __launch_bounds__(kThreads, 2) w4_moe_down_kernel(MoeArgs a) {
 // s = 0, 1, groups h = 0, 1 and halves e = 0, 1 of the word. Q4_0: the nibble at bit 16 e + 8 s + 4 h. MXFP4: inside half
 // e, (sign, magnitude) at bits (15, 11..9), (12, 8..6), (14, 5..3), (13, 2..0) for (h, s) = (0,0), (0,1), (1,0), (1,1).
 template <bool MX>
-__global__ void w4_retile_kernel(const uint8_t * rows, uint32_t n_out, uint32_t n_in, uint32_t tiles, uint32_t steps, uint8_t * units, int * max_scale) {
+__global__ void w4_retile_kernel(const uint8_t * rows, uint32_t n_out, uint32_t n_in, uint32_t row_blocks, uint32_t steps, uint8_t * units, int * max_scale) {
     constexpr uint32_t kBlock = MX ? 17 : 18;
     const uint32_t blocks = n_in / 32;
     const size_t unit = blockIdx.x;
     const uint32_t step = (uint32_t)(unit % steps);
-    const size_t tile_of_all = unit / steps;
-    const uint32_t tile = (uint32_t)(tile_of_all % tiles);
-    const size_t expert = tile_of_all / tiles;
+    const size_t block_of_all = unit / steps;
+    const uint32_t row_block = (uint32_t)(block_of_all % row_blocks);
+    const size_t expert = block_of_all / row_blocks;
     uint8_t * dst = units + unit * w4_unit_bytes(MX);
-    const uint32_t lane = threadIdx.x >> 2, j = threadIdx.x & 3;
+    const uint32_t tile = threadIdx.x >> 7, lane = (threadIdx.x & 127) >> 2, j = threadIdx.x & 3;
     const uint32_t g = lane >> 2, t = lane & 3;
-    const uint32_t row = tile * 16 + g + 8 * (j & 1);
+    const uint32_t row = row_block * 32 + tile * 16 + g + 8 * (j & 1);
     uint32_t word = 0;
     for (uint32_t h = 0; h < 2; ++h) {
         const uint32_t block = step * 2 + h;
@@ -1050,20 +1218,21 @@ __global__ void w4_retile_kernel(const uint8_t * rows, uint32_t n_out, uint32_t 
                 }
             }
     }
-    *reinterpret_cast<uint32_t *>(dst + lane * 16 + j * 4) = word;
-    if (threadIdx.x < 32) {
-        // scales of (g, group), then of (g + 8, group), for g = 0..7
-        const uint32_t sg = threadIdx.x >> 2, upper = (threadIdx.x >> 1) & 1, h = threadIdx.x & 1;
-        const uint32_t srow = tile * 16 + sg + 8 * upper, block = step * 2 + h;
+    *reinterpret_cast<uint32_t *>(dst + tile * 512 + lane * 16 + j * 4) = word;
+    if (threadIdx.x < 64) {
+        // scales of (g, group), then of (g + 8, group), for g = 0..7, of each tile
+        const uint32_t st = threadIdx.x >> 5, sg = (threadIdx.x & 31) >> 2, upper = (threadIdx.x >> 1) & 1, h = threadIdx.x & 1;
+        const uint32_t srow = row_block * 32 + st * 16 + sg + 8 * upper, block = step * 2 + h;
         const bool live = srow < n_out && block < blocks;
         const uint8_t * b = rows + ((expert * n_out + srow) * blocks + block) * kBlock;
         if (MX) {
             // kept as s + 8, so that the smallest scale 2^-127 is a normal f32 as well; 2^-8 is part of the rows' final factor
             const int s = live ? b[0] : 0;
-            if (live) atomicMax(max_scale, s);
-            dst[512 + sg * 4 + upper * 2 + h] = live ? (uint8_t)min(s + 8, 255) : 0;
+            const uint32_t warp_max = __reduce_max_sync(0xffffffffu, (uint32_t)s);
+            if ((threadIdx.x & 31) == 0) atomicMax(max_scale, (int)warp_max);
+            dst[1024 + st * 32 + sg * 4 + upper * 2 + h] = live ? (uint8_t)min(s + 8, 255) : 0;
         } else {
-            reinterpret_cast<uint16_t *>(dst + 512)[sg * 4 + upper * 2 + h] = live ? (uint16_t)(b[0] | b[1] << 8) : 0;
+            reinterpret_cast<uint16_t *>(dst + 1024 + st * 64)[sg * 4 + upper * 2 + h] = live ? (uint16_t)(b[0] | b[1] << 8) : 0;
         }
     }
 }
@@ -1100,25 +1269,31 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), int grid, int cluster, size
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-template <bool MX, int PARTS, bool GLU, int MODE>
-cudaError_t launch_product(const ProductArgs & a, int C, size_t smem, cudaStream_t stream) {
-    static PerDeviceOnce once;
-    if (once.first()) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_product_kernel<MX, PARTS, GLU, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-        if (e != cudaSuccess) return e;
-    }
-    return launch_cluster(w4_product_kernel<MX, PARTS, GLU, MODE>, a.clusters * C, C, smem, stream, a);
+template <typename... KArgs> cudaError_t allow_smem(PerDeviceOnce & once, void (*kernel)(KArgs...)) {
+    return once.first() ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) : cudaSuccess;
 }
+
+template <bool MX, int PARTS, bool GLU, int NT> cudaError_t launch_product(const ProductArgs & a, int C, size_t smem, cudaStream_t stream) {
+    static PerDeviceOnce once;
+    const cudaError_t e = allow_smem(once, w4_product_kernel<MX, PARTS, GLU, NT>);
+    return e != cudaSuccess ? e : launch_cluster(w4_product_kernel<MX, PARTS, GLU, NT>, a.clusters * C, C, smem, stream, a);
+}
+
+// Room the kernels that take whole calls of n tokens stage them with: those sizes they are built for.
+int product_room(int n, int parts) { return n == 1 ? 1 : n <= 4 && parts == 2 ? 4 : n <= 8 ? 8 : 16; }
 
 template <bool MX, bool GLU>
 cudaError_t launch_product_of(const ProductArgs & a, int parts, int C, size_t smem, cudaStream_t stream) {
+    const int nt = product_room(a.T, parts);
     if (parts == 2) {
-        if (a.T <= 4) return launch_product<MX, 2, GLU, PACK>(a, C, smem, stream);
-        if (a.T <= 8) return launch_product<MX, 2, GLU, ONE>(a, C, smem, stream);
-        return launch_product<MX, 2, GLU, TWO>(a, C, smem, stream);
+        if (nt == 1) return launch_product<MX, 2, GLU, 1>(a, C, smem, stream);
+        if (nt == 4) return launch_product<MX, 2, GLU, 4>(a, C, smem, stream);
+        if (nt == 8) return launch_product<MX, 2, GLU, 8>(a, C, smem, stream);
+        return launch_product<MX, 2, GLU, 16>(a, C, smem, stream);
     }
-    if (a.T <= 8) return launch_product<MX, 1, GLU, ONE>(a, C, smem, stream);
-    return launch_product<MX, 1, GLU, TWO>(a, C, smem, stream);
+    if (nt == 1) return launch_product<MX, 1, GLU, 1>(a, C, smem, stream);
+    if (nt == 8) return launch_product<MX, 1, GLU, 8>(a, C, smem, stream);
+    return launch_product<MX, 1, GLU, 16>(a, C, smem, stream);
 }
 
 size_t type_bytes(uint32_t type) { return type == GGML_F32 ? 4 : 2; }
@@ -1132,47 +1307,46 @@ const void * row_at(const void * p, uint32_t type, int64_t ld, int64_t row) {
     return p ? static_cast<const uint8_t *>(p) + row * ld * (int64_t)type_bytes(type) : nullptr;
 }
 
-template <bool MX, int PARTS, int MODES> cudaError_t launch_gate_up(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
+template <bool MX, int PARTS, int NT> cudaError_t launch_gate_up(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
     static PerDeviceOnce once;
-    if (once.first()) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_moe_gate_up_kernel<MX, PARTS, MODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-        if (e != cudaSuccess) return e;
-    }
-    return launch_cluster(w4_moe_gate_up_kernel<MX, PARTS, MODES>, a.clusters * C, C, smem, stream, a);
+    const cudaError_t e = allow_smem(once, w4_moe_gate_up_kernel<MX, PARTS, NT>);
+    return e != cudaSuccess ? e : launch_cluster(w4_moe_gate_up_kernel<MX, PARTS, NT>, a.clusters * C, C, smem, stream, a);
 }
 
-template <bool MX, int MODES> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
+template <bool MX, int MOST> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
     static PerDeviceOnce once;
-    if (once.first()) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_moe_down_kernel<MX, MODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-        if (e != cudaSuccess) return e;
-    }
-    return launch_cluster(w4_moe_down_kernel<MX, MODES>, a.clusters * C, C, smem, stream, a);
+    const cudaError_t e = allow_smem(once, w4_moe_down_kernel<MX, MOST>);
+    return e != cudaSuccess ? e : launch_cluster(w4_moe_down_kernel<MX, MOST>, a.clusters * C, C, smem, stream, a);
 }
 
-// The kernels are built for the modes that calls of up to 4, 8 and 16 tokens reach.
 template <bool MX> cudaError_t launch_gate_up_of(const MoeArgs & a, int parts, int C, size_t smem, cudaStream_t stream) {
+    const int nt = product_room(a.T, parts);
     if (parts == 2) {
-        if (a.T <= 4) return launch_gate_up<MX, 2, 1 << PACK>(a, C, smem, stream);
-        if (a.T <= 8) return launch_gate_up<MX, 2, 1 << PACK | 1 << ONE>(a, C, smem, stream);
-        return launch_gate_up<MX, 2, 1 << PACK | 1 << ONE | 1 << TWO>(a, C, smem, stream);
+        if (nt == 1) return launch_gate_up<MX, 2, 1>(a, C, smem, stream);
+        if (nt == 4) return launch_gate_up<MX, 2, 4>(a, C, smem, stream);
+        if (nt == 8) return launch_gate_up<MX, 2, 8>(a, C, smem, stream);
+        return launch_gate_up<MX, 2, 16>(a, C, smem, stream);
     }
-    if (a.T <= 8) return launch_gate_up<MX, 1, 1 << ONE>(a, C, smem, stream);
-    return launch_gate_up<MX, 1, 1 << ONE | 1 << TWO>(a, C, smem, stream);
+    if (nt == 1) return launch_gate_up<MX, 1, 1>(a, C, smem, stream);
+    if (nt == 8) return launch_gate_up<MX, 1, 8>(a, C, smem, stream);
+    return launch_gate_up<MX, 1, 16>(a, C, smem, stream);
 }
 
 template <bool MX> cudaError_t launch_down_of(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
-    if (a.T <= 4) return launch_down<MX, 1 << PACK>(a, C, smem, stream);
-    if (a.T <= 8) return launch_down<MX, 1 << PACK | 1 << ONE>(a, C, smem, stream);
-    return launch_down<MX, 1 << PACK | 1 << ONE | 1 << TWO>(a, C, smem, stream);
+    if (a.T == 1) return launch_down<MX, 1>(a, C, smem, stream);
+    if (a.T <= 4) return launch_down<MX, 4>(a, C, smem, stream);
+    if (a.T <= 8) return launch_down<MX, 8>(a, C, smem, stream);
+    return launch_down<MX, 16>(a, C, smem, stream);
 }
+
+int up_to(int x, int unit) { return (x + unit - 1) / unit * unit; }
 
 int64_t moe_ld_h(uint32_t ff) { return ((int64_t)ff + 3) / 4 * 4; }
 
 } // namespace
 
 size_t w4_bytes(uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert) {
-    return (size_t)n_expert * ((n_out + 15) / 16) * ((n_in + 63) / 64) * w4_unit_bytes(type == GGML_MXFP4);
+    return (size_t)n_expert * ((n_out + 31) / 32) * ((n_in + 63) / 64) * w4_unit_bytes(type == GGML_MXFP4);
 }
 
 W4View w4_view(const uint8_t * units, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert) {
@@ -1182,34 +1356,66 @@ W4View w4_view(const uint8_t * units, uint32_t type, uint32_t n_out, uint32_t n_
     v.n_out = n_out;
     v.n_in = n_in;
     v.n_expert = n_expert;
-    v.tiles = (n_out + 15) / 16;
+    v.blocks = (n_out + 31) / 32;
     v.steps = (n_in + 63) / 64;
-    v.expert_bytes = (size_t)v.tiles * v.steps * w4_unit_bytes(type == GGML_MXFP4);
+    v.expert_bytes = (size_t)v.blocks * v.steps * w4_unit_bytes(type == GGML_MXFP4);
     return v;
 }
 
 void launch_w4_retile(const uint8_t * rows, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert, uint8_t * units, int * max_scale,
                       cudaStream_t stream) {
     const W4View v = w4_view(units, type, n_out, n_in, n_expert);
-    const size_t n = (size_t)n_expert * v.tiles * v.steps;
-    if (type == GGML_MXFP4) w4_retile_kernel<true><<<(unsigned)n, 128, 0, stream>>>(rows, n_out, n_in, v.tiles, v.steps, units, max_scale);
-    else w4_retile_kernel<false><<<(unsigned)n, 128, 0, stream>>>(rows, n_out, n_in, v.tiles, v.steps, units, max_scale);
+    const size_t n = (size_t)n_expert * v.blocks * v.steps;
+    if (type == GGML_MXFP4) w4_retile_kernel<true><<<(unsigned)n, 256, 0, stream>>>(rows, n_out, n_in, v.blocks, v.steps, units, max_scale);
+    else w4_retile_kernel<false><<<(unsigned)n, 256, 0, stream>>>(rows, n_out, n_in, v.blocks, v.steps, units, max_scale);
+}
+
+// How a product is cut: CTAs of a cluster, clusters, and the shared memory of a CTA.
+struct Cut {
+    int C = 0, clusters = 0, resident = 0;
+    double cost = 0;
+};
+
+// Chooses the cluster size for `blocks` row blocks of `per` matrices and `steps` column steps whose activations take `each` bytes of
+// shared memory a step. The estimate is in clocks: the weight stream at the SM's share of the memory bandwidth, but no faster
+// than the copies in flight of the CTAs on the busiest SM allow; the conversion of the CTA's share of the activations; and the sums it
+// receives; `step_clocks` is what else a column step costs a CTA.
+Cut choose_cut(int blocks, int per, int steps, int n, int each, int ring, int fixed, double step_clocks, int unit, int sms) {
+    Cut best;
+    for (int C = 1; C <= kMaxCluster && C <= steps; C *= 2) {
+        const int s = (steps + C - 1) / C;
+        const int64_t inbox = 2 * inbox_bytes(n, C, 1, per);
+        const int64_t smem = s * each + ring + fixed + inbox + 4096;
+        if (smem > kMaxSmem) continue;
+        Cut c;
+        c.C = C;
+        c.resident = (int)std::min<int64_t>(n > 8 ? 2 : 3, 226 * 1024 / smem);
+        const int most = std::max(1, c.resident * sms / C), blocks_each = (blocks + most - 1) / most;
+        c.clusters = (blocks + blocks_each - 1) / blocks_each;
+        const int busy = (c.clusters * C + sms - 1) / sms;
+        const double in_flight = (double)busy * ring * (kStages - 1) / kStages;
+        const double stream = std::max((double)blocks * per * steps * unit / (23.5 * sms), (double)busy * blocks_each * per * s * unit / std::min(46.0, in_flight / 1600.0));
+        const double convert = busy * s * (n * 64 * 0.12 + step_clocks) + 800, sums = busy * (double)blocks_each * per * n * 8;
+        c.cost = stream + convert + sums;
+        if (!best.C || c.cost < best.cost) best = c;
+    }
+    return best;
 }
 
 cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
     const bool mx = p.w.type == GGML_MXFP4, glu = p.up != nullptr;
     const int parts = p.x_type == GGML_F32 || p.norm ? 2 : 1;
     const int sms = device_sms();
-    const int jobs = glu ? (int)p.w.tiles : ((int)p.w.tiles + 1) / 2;
-    const int steps = (int)p.w.steps;
+    const int blocks = (int)p.w.blocks, per = glu ? 2 : 1, steps = (int)p.w.steps;
     for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
-        // the smallest cluster that fills the GPU, and whose share of the activations is small beside its share of the weights
-        int C = 1;
-        auto staged = [&](int c) { const int s = (steps + c - 1) / c; return staged_x_bytes(s, parts, n) + staged_c_bytes(mx, s, n); };
-        while (C < 8 && 2 * C <= steps && ((int64_t)jobs * C < 2 * sms || (int64_t)n * sms * 8 > (int64_t)jobs * C * C * 4)) C *= 2;
-        while (C < 8 && 2 * C <= steps && staged(C) > 96 * 1024) C *= 2;
-        while (n > 1 && staged(C) > 160 * 1024) n = (n + 1) / 2;
+        Cut cut;
+        for (;; n = (n + 1) / 2) {
+            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), ring_bytes(mx), 0, 0, (int)w4_unit_bytes(mx), sms);
+            if (cut.C || n == 1) break;
+        }
+        if (!cut.C) return cudaErrorInvalidValue;       // rows this long are refused when the handle is made
+        const int C = cut.C, nt = product_room(n, parts), s = (steps + C - 1) / C;
         ProductArgs a{};
         a.w = p.w.units;
         a.u = glu ? p.up->units : nullptr;
@@ -1217,7 +1423,6 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         a.T = n;
         a.n_in = (int)p.w.n_in;
         a.n_out = (int)p.w.n_out;
-        a.tiles = (int)p.w.tiles;
         a.steps = steps;
         a.norm = p.norm;
         a.eps = p.eps;
@@ -1227,19 +1432,18 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         a.y = const_cast<void *>(row_at(p.y, p.y_type, p.ld_y, t0));
         a.y_type = p.y_type;
         a.ld_y = p.ld_y;
-        a.jobs = jobs;
-        const int most = std::max(1, 2 * sms / C);
-        const int per = (jobs + most - 1) / most;
-        a.clusters = (jobs + per - 1) / per;
-        const int s = (steps + C - 1) / C;
-        a.x_bytes = (staged_x_bytes(s, parts, n) + 127) / 128 * 128;
-        a.c_bytes = (staged_c_bytes(mx, s, n) + 127) / 128 * 128;
-        a.jobs = jobs;
-        const int slot = n * kSlotCol * 4;
-        const int wanted = per * split_columns(per, steps / C);
-        const int room = std::max(kWarps * slot, std::min(100 * 1024 - a.x_bytes - a.c_bytes, kMaxSmem - a.x_bytes - a.c_bytes));
-        a.slots = std::max(1, std::min(wanted, room / slot));
-        const size_t smem = (size_t)a.x_bytes + a.c_bytes + (size_t)a.slots * slot;
+        a.blocks = blocks;
+        a.clusters = cut.clusters;
+        a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
+        a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
+        // two inboxes in what is left of the CTA's share of the shared memory; one, if everything fits into it
+        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx);
+        const int blocks_each = (blocks + cut.clusters - 1) / cut.clusters;
+        const int room = std::min(226 * 1024 / cut.resident - 4096, kMaxSmem) - fixed;
+        a.ks = split_columns(blocks_each * per, steps / C, (int)std::max<int64_t>(1, room / 2 / inbox_bytes(n, C, 1, per)));
+        const int64_t whole = inbox_bytes((int64_t)blocks_each * n, C, a.ks, per);
+        a.inbox = (int)(whole <= room ? whole : std::max<int64_t>(room / 2 / 128 * 128, inbox_bytes(n, C, a.ks, per)));
+        const size_t smem = (size_t)fixed + (whole <= room ? 1 : 2) * (size_t)a.inbox;
         cudaError_t e;
         if (mx) e = glu ? launch_product_of<true, true>(a, parts, C, smem, stream) : launch_product_of<true, false>(a, parts, C, smem, stream);
         else e = glu ? launch_product_of<false, true>(a, parts, C, smem, stream) : launch_product_of<false, false>(a, parts, C, smem, stream);
@@ -1259,13 +1463,19 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
     const int sms = device_sms();
     const int E = (int)p.gate.n_expert, d = (int)p.gate.n_in, ff = (int)p.gate.n_out;
     const int steps_d = (int)p.gate.steps, steps_ff = (int)p.down.steps;
-    auto up_to = [](int x, int unit) { return (x + unit - 1) / unit * unit; };
     for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
-        int C = 8;
-        while (C > steps_d) C /= 2;
-        auto staged = [&] { const int s = (steps_d + C - 1) / C; return staged_x_bytes(s, parts, n) + staged_c_bytes(mx, s, n); };
-        while (n > 1 && staged() > 120 * 1024) n = (n + 1) / 2;
+        // first kernel: n tokens choose at most `reach` experts, a little fewer if they choose independently
+        int reach = 0;
+        Cut cut;
+        for (;; n = (n + 1) / 2) {
+            reach = (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n)));
+            cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), ring_bytes(mx),
+                             2 * up_to(n * E * 4, 128) + 24 * 1024, n * E * 0.65 + E * 8, (int)w4_unit_bytes(mx), sms);
+            if (cut.C || n == 1) break;
+        }
+        if (!cut.C) return cudaErrorInvalidValue;
+        int C = cut.C;
         MoeArgs a{};
         a.gate = p.gate.units;
         a.up = p.up.units;
@@ -1280,9 +1490,9 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.k = p.n_used;
         a.d = d;
         a.ff = ff;
-        a.tiles_ff = (int)p.gate.tiles;
+        a.blocks_ff = (int)p.gate.blocks;
         a.steps_d = steps_d;
-        a.tiles_d = (int)p.down.tiles;
+        a.blocks_d = (int)p.down.blocks;
         a.steps_ff = steps_ff;
         a.normalise = p.normalise;
         a.norm = p.norm;
@@ -1298,30 +1508,29 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.h = reinterpret_cast<float *>(static_cast<uint8_t *>(p.workspace) + (sizeof(MoeMeta) + 255) / 256 * 256);
         a.ld_h = moe_ld_h((uint32_t)ff);
 
-        // first kernel: at most `reach` experts are chosen
-        const int reach = std::min(E, n * p.n_used);
-        const int s = (steps_d + C - 1) / C;
-        a.x_bytes = up_to(staged_x_bytes(s, parts, n), 128);
-        a.c_bytes = up_to(staged_c_bytes(mx, s, n), 128);
+        const int s = (steps_d + C - 1) / C, nt = product_room(n, parts);
+        a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
+        a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
         a.logit_bytes = up_to(n * E * 4, 128);
-        a.clusters = std::max(1, (int)std::min<int64_t>(2 * sms / C, (int64_t)reach * a.tiles_ff));
-        const int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes;
-        a.partial_floats = std::max(kWarps * n * kSlotCol, (88 * 1024 - fixed) / 4);
-        cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, C, (size_t)fixed + a.partial_floats * 4, stream)
-                           : launch_gate_up_of<false>(a, parts, C, (size_t)fixed + a.partial_floats * 4, stream);
+        a.clusters = cut.clusters;
+        int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx);
+        a.inbox = (int)std::max<int64_t>((std::min(226 * 1024 / cut.resident - 28 * 1024, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, C, 1, 2));
+        cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, C, (size_t)fixed + 2 * a.inbox, stream) : launch_gate_up_of<false>(a, parts, C, (size_t)fixed + 2 * a.inbox, stream);
         if (e != cudaSuccess) return e;
 
         // second kernel
-        C = 8;
+        C = kMaxCluster;
         while (C > steps_ff * p.n_used) C /= 2;
-        const int jobs = (a.tiles_d + 1) / 2;
-        const int most = std::max(1, 2 * sms / C), per = (jobs + most - 1) / most;
-        a.clusters = (jobs + per - 1) / per;
-        a.x_bytes = 64 * 1024;
+        const int resident = n > 8 ? 2 : 3;
+        const int most = std::max(1, resident * sms / C), per = (a.blocks_d + most - 1) / most;
+        a.clusters = (a.blocks_d + per - 1) / per;
+        a.x_bytes = (n > 8 ? 32 : n > 1 ? 16 : 12) * 1024;
         a.c_bytes = a.logit_bytes = 0;
-        a.partial_floats = std::max(kWarps * n * kSlotCol, std::min(per * kWarps * n * kSlotCol, (100 * 1024 - a.x_bytes) / 4));
-        e = mx_down ? launch_down_of<true>(a, C, (size_t)a.x_bytes + a.partial_floats * 4, stream)
-                    : launch_down_of<false>(a, C, (size_t)a.x_bytes + a.partial_floats * 4, stream);
+        const int slot = n * kSlotCol * 4, down_fixed = a.x_bytes + ring_bytes(mx_down);
+        a.inbox = (int)inbox_bytes(std::min(per, kWarps) * n, C, 1, 1);
+        a.partial = std::max(kWarps * slot, std::min(per * kWarps * slot, 226 * 1024 / resident - 18 * 1024 - down_fixed - 2 * a.inbox) / slot * slot);
+        const size_t smem = (size_t)down_fixed + a.partial + 2 * a.inbox;
+        e = mx_down ? launch_down_of<true>(a, C, smem, stream) : launch_down_of<false>(a, C, smem, stream);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

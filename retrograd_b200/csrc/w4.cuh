@@ -15,20 +15,18 @@ constexpr uint32_t kW4MaxExperts = 256;
 constexpr uint32_t kW4MaxUsed = 32;          // experts per token
 constexpr uint32_t kW4MaxScaleByte = 223;    // MXFP4: weight scales up to 2^96, so that a row's scaled sum stays inside f32
 
-// Device layout: units of 16 rows x 64 columns, a row tile's units consecutive over the columns, row tiles consecutive,
-// experts consecutive. A unit is 32 x 16 bytes, one 16-byte word per lane of the warp that multiplies it (the lane's share
-// of the A fragments of four m16n8k16 products), then the 16 rows' two scales: 64 bytes of f16 or 32 bytes. Rows and
+// Device layout: units of 32 rows x 64 columns, a row block's units consecutive over the columns, row blocks consecutive,
+// experts consecutive. A unit is, for each of its two 16-row tiles, 32 x 16 bytes, one 16-byte word per lane of the warp that multiplies it (the lane's share
+// of the A fragments of four m16n8k16 products), then for each tile the 16 rows' two scales: 64 bytes of f16 or 32 bytes. Rows and
 // columns beyond the matrix have scale zero. The bit order inside a word is described at w4_retile_kernel.
-constexpr uint32_t kW4UnitRows = 16;
-constexpr uint32_t kW4UnitCols = 64;
-__host__ __device__ constexpr uint32_t w4_unit_bytes(bool mxfp4) { return mxfp4 ? 544u : 576u; }
+__host__ __device__ constexpr uint32_t w4_unit_bytes(bool mxfp4) { return mxfp4 ? 1088u : 1152u; }
 
 struct W4View {
     const uint8_t * units = nullptr;
     uint32_t type = 0;              // GGML_Q4_0 or GGML_MXFP4
     uint32_t n_out = 0, n_in = 0;
     uint32_t n_expert = 1;
-    uint32_t tiles = 0;             // 16-row tiles of one expert
+    uint32_t blocks = 0;            // 32-row blocks of one expert
     uint32_t steps = 0;             // 64-column steps
     size_t expert_bytes = 0;
 };
