@@ -14,7 +14,7 @@
 // it converts only its share of the activations. Its warps take (row block, part of the CTA's columns) runs, and
 // write every (row block, token)'s sums into the shared memory of the CTA that owns it, which adds them in a fixed order after one
 // cluster barrier (no workspace, no atomics: results are the same in every run) and applies bias, residual or the gate's
-// activation. Every warp streams its units through a ring of its own in shared memory by asynchronous copies, kStages - 1 units
+// activation. Every warp streams its units through a ring of its own in shared memory by asynchronous copies, three or five units
 // ahead, so that no registers are held by loads in flight and three CTAs fit on an SM.
 
 #include "kernels.cuh"
@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 4;          // units in a warp's ring
 constexpr int kSlotCol = 36;        // floats per (partial slot, token): 32 rows, padded so that a warp's stores meet no bank twice
 constexpr int kMaxSegs = 16;
 constexpr int kMaxCluster = 8;
@@ -121,7 +120,9 @@ template <bool MX> struct Unit {
     uint2 s[2];     // MXFP4 uses .x only
 };
 
-__host__ __device__ constexpr int ring_bytes(bool mx) { return kWarps * kStages * (int)w4_unit_bytes(mx); }
+// Units in a warp's ring; fewer beside the activations of many tokens.
+__host__ __device__ constexpr int stages_for(int n) { return n > 4 ? 4 : 6; }
+__host__ __device__ constexpr int ring_bytes(bool mx, int n) { return kWarps * stages_for(n) * (int)w4_unit_bytes(mx); }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t * src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -271,24 +272,37 @@ __device__ void stage_rows(const Act & act, int n, int n_in, const float * norm,
         uint32_t top = 0;
         float squares = 0.f;
         float held[kHeld][4];
-        auto look = [&](int i, float (&v)[4]) {
-            v[0] = v[1] = v[2] = v[3] = 0.f;
-            if (i < count) {
-                load4(act, r.row, r.k0 + 4 * i, v);
-                if constexpr (NORM) {
+        // loads of kHeld chunks are in flight together; a row that is no longer than them is read once
+        auto load = [&](int it0) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) squares += v[e] * v[e];
-                    scale4(v, norm + r.k0 + 4 * i);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+            for (int it = 0; it < kHeld; ++it) {
+                const int i = first + (it0 + it) * shared * 32;
+                held[it][0] = held[it][1] = held[it][2] = held[it][3] = 0.f;
+                if (it0 + it < trips && i < count) load4(act, r.row, r.k0 + 4 * i, held[it]);
             }
         };
-        if (trips <= kHeld) {
+        auto weigh = [&](int it0) {
+            if constexpr (NORM) {
 #pragma unroll
-            for (int it = 0; it < kHeld; ++it) if (it < trips) look(first + it * shared * 32, held[it]);
-        } else {
-            for (int it = 0; it < trips; ++it) look(first + it * shared * 32, held[0]);
+                for (int it = 0; it < kHeld; ++it) {
+                    const int i = first + (it0 + it) * shared * 32;
+                    if (it0 + it < trips && i < count) scale4(held[it], norm + r.k0 + 4 * i);
+                }
+            }
+        };
+        for (int it0 = 0; it0 < trips; it0 += kHeld) {
+            load(it0);
+            if constexpr (NORM) {
+#pragma unroll
+                for (int it = 0; it < kHeld; ++it)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) squares += held[it][e] * held[it][e];
+            }
+            weigh(it0);
+#pragma unroll
+            for (int it = 0; it < kHeld; ++it)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(held[it][e]) & 0x7fffffffu);
         }
         top = __reduce_max_sync(0xffffffffu, top);
         if constexpr (NORM) {
@@ -313,19 +327,13 @@ __device__ void stage_rows(const Act & act, int n, int n_in, const float * norm,
             sc.f2[r.seg][r.place] = __uint_as_float((uint32_t)(down - down / 2 + 127) << 23);
             if constexpr (NORM) put_squares(i0, squares);
         }
-        if (trips <= kHeld) {
-#pragma unroll
-            for (int it = 0; it < kHeld; ++it) if (it < trips) stage_chunk<MX, PARTS>(r, first + it * shared * 32, held[it], up);
-        } else {
-            for (int it = 0; it < trips; ++it) {
-                const int i = first + it * shared * 32;
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (i < count) {
-                    load4(act, r.row, r.k0 + 4 * i, v);
-                    if constexpr (NORM) scale4(v, norm + r.k0 + 4 * i);
-                }
-                stage_chunk<MX, PARTS>(r, i, v, up);
+        for (int it0 = 0; it0 < trips; it0 += kHeld) {
+            if (trips > kHeld) {
+                load(it0);
+                weigh(it0);
             }
+#pragma unroll
+            for (int it = 0; it < kHeld; ++it) if (it0 + it < trips) stage_chunk<MX, PARTS>(r, first + (it0 + it) * shared * 32, held[it], up);
         }
         if (shared > 1) break;      // that many warps share a row only when one round holds all rows
     }
@@ -480,7 +488,7 @@ struct Cursor {
 
 // Runs a warp's sequence. Source: first(Cursor &) and next(Cursor &) move to a run (never an empty one) and set everything;
 // group(const Cursor &) describes the activations; put(const Cursor &, row, column, sum) takes the sums.
-template <bool MX, class Source> struct Stream {
+template <bool MX, int STAGES, class Source> struct Stream {
     const Source & src;
     const int lane;
     const uint32_t ring;
@@ -488,7 +496,7 @@ template <bool MX, class Source> struct Stream {
     uint32_t fill, at;          // ring offsets of the stage to fill and the stage to multiply
 
     __device__ __forceinline__ Stream(const Source & s, uint8_t * rings)
-        : src(s), lane(threadIdx.x & 31), ring(smem_address(rings) + (threadIdx.x >> 5) * (kStages * w4_unit_bytes(MX))), fill(0), at(0) {
+        : src(s), lane(threadIdx.x & 31), ring(smem_address(rings) + (threadIdx.x >> 5) * (STAGES * w4_unit_bytes(MX))), fill(0), at(0) {
         src.first(ld);
         cp = ld;
     }
@@ -502,13 +510,13 @@ template <bool MX, class Source> struct Stream {
             ld.p += w4_unit_bytes(MX);
             if (--ld.rem == 0) src.next(ld);
         }
-        fill = fill == (kStages - 1) * w4_unit_bytes(MX) ? 0 : fill + w4_unit_bytes(MX);
+        fill = fill == (STAGES - 1) * w4_unit_bytes(MX) ? 0 : fill + w4_unit_bytes(MX);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
     // The first units of the sequence; needs nothing but the weights. The ring must be free: a barrier lies between its last reads and this.
     __device__ __forceinline__ void prefetch() {
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) fetch();
+        for (int i = 0; i < STAGES - 1; ++i) fetch();
     }
     // All runs of the cursor's group whose job is below `limit`.
     template <int PARTS, int MODE, int NT, bool LIST> __device__ __forceinline__ void work_group(const Group & r, const Scratch & sc, int limit = 0x7fffffff) {
@@ -520,11 +528,11 @@ template <bool MX, class Source> struct Stream {
         do {
             uint32_t b_at = 0, c_at = 0;
             for (int n = cp.rem; n > 0; --n) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
                 __syncwarp();           // every lane's copies of this unit have landed, and the stage read last is free
                 fetch();
                 do_step<MX, PARTS, MODE, NT, LIST>(words + at, scale_at + at, b_at, c_at, l, acc);
-                at = at == (kStages - 1) * w4_unit_bytes(MX) ? 0 : at + w4_unit_bytes(MX);
+                at = at == (STAGES - 1) * w4_unit_bytes(MX) ? 0 : at + w4_unit_bytes(MX);
                 b_at += step_x_bytes(PARTS, NT);
                 c_at += l.c_step;
             }
@@ -582,6 +590,11 @@ __host__ __device__ inline int part_begin(int n, int part, int parts) {
     return (int)(part * each + min((unsigned)part, more));
 }
 
+// The same for 2^log_parts parts.
+__device__ __forceinline__ int part_begin2(int n, int part, int log_parts) {
+    return part * (n >> log_parts) + min(part, n & ((1 << log_parts) - 1));
+}
+
 // ---- y = W x, and y = silu(W x) * (U x)
 
 // The inbox of a CTA: for each (row block, token) it owns, the sums of 32 rows from every (CTA, part of the columns) of the
@@ -626,9 +639,9 @@ struct ProductArgs {
     void * y;
     uint32_t y_type;
     int64_t ld_y;
-    int blocks, clusters;           // row blocks, of gate and up together as of one matrix
+    int each, more, clusters;       // row blocks of a cluster (one more in the first `more`), of gate and up together as of one matrix
     int x_bytes, c_bytes, inbox;    // shared memory: staged activations, start values, one inbox
-    int ks;                         // parts of the columns, the same in every cluster: one inbox may have to do
+    int ks, per_round;              // parts of the columns and blocks of a round, the same in every cluster: one inbox may have to do
 };
 
 // Jobs: a row block; with the gate, block j of gate and of up are jobs 2 j and 2 j + 1.
@@ -649,11 +662,11 @@ template <bool MX, int PARTS, bool GLU, int NT> struct ProductSource {
     }
     __device__ __forceinline__ void first(Cursor & c) const {
         c.group = 0;
-        c.job = (threadIdx.x >> 5) / ks;
+        c.job = (threadIdx.x >> 5) >> (__ffs(ks) - 1);
         point(c);
     }
     __device__ __forceinline__ void next(Cursor & c) const {
-        c.job += kWarps / ks;
+        c.job += kWarps >> (__ffs(ks) - 1);
         point(c);
     }
     __device__ __forceinline__ Group group(const Cursor &) const { return {x, nullptr, a.T, 0}; }
@@ -672,19 +685,20 @@ __global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_product_kernel(Pr
     const int rank = (int)cluster_rank(), C = (int)cluster_size();
     const int cluster = blockIdx.x / C;
     cluster_arrive();
-    const int s0 = part_begin(a.steps, rank, C), n_steps = part_begin(a.steps, rank + 1, C) - s0;
-    const int b_begin = part_begin(a.blocks, cluster, a.clusters), blocks = part_begin(a.blocks, cluster + 1, a.clusters) - b_begin;
-    const int ks = a.ks;
-    const int per_round = blocks_per_round(a.inbox, a.T, C, ks, kPer);
+    const int log_c = __ffs(C) - 1;
+    const int s0 = part_begin2(a.steps, rank, log_c), n_steps = part_begin2(a.steps, rank + 1, log_c) - s0;
+    const int b_begin = cluster * a.each + min(cluster, a.more), blocks = a.each + (cluster < a.more);
+    const int ks = a.ks, log_ks = __ffs(ks) - 1;
+    const int per_round = a.per_round;
     uint8_t * const rings = smem + a.x_bytes + a.c_bytes;
     const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
-    const Inbox inbox{smem_address(rings + ring_bytes(MX)), a.inbox, rank, __ffs(C) - 1, ks, kPer};
-    const int sub = warp % ks, step = part_begin(n_steps, sub, ks), len = part_begin(n_steps, sub + 1, ks) - step;
+    const Inbox inbox{smem_address(rings + ring_bytes(MX, NT)), a.inbox, rank, log_c, ks, kPer};
+    const int sub = warp & (ks - 1), step = part_begin2(n_steps, sub, log_ks), len = part_begin2(n_steps, sub + 1, log_ks) - step;
     const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
     if (threadIdx.x == 0) sc.zero = 0;
 
     ProductSource<MX, PARTS, GLU, NT> src{a, x_warp, inbox, b_begin * kPer, blocks * kPer, ks, sub, s0 + step, len, 0, 0};
-    Stream<MX, ProductSource<MX, PARTS, GLU, NT>> stream(src, rings);
+    Stream<MX, stages_for(NT), ProductSource<MX, PARTS, GLU, NT>> stream(src, rings);
     stream.prefetch();
     // the weights above are the library's own; everything below is the caller's
     pdl_trigger();
@@ -733,6 +747,7 @@ struct MoeArgs {
     const uint8_t * gate, * up, * down;
     size_t gate_expert, up_expert, down_expert;     // bytes of one expert
     const float * router;
+    bool router_vec;            // sixteen bytes of it may be read at once
     Act x;
     int T, E, k, d, ff;
     int blocks_ff, steps_d, blocks_d, steps_ff;
@@ -759,9 +774,8 @@ struct Picks {
     uint16_t unique[kW4MaxExperts];
     uint8_t count[kW4MaxExperts];                   // of unique[i]
     uint8_t token[kW4MaxExperts][kRowList];
-    uint16_t pair[kW4MaxExperts][kRowList];         // token * n_used + rank of the expert among the token's
     uint32_t mask[kW4MaxExperts];                   // by expert: the tokens that chose it
-    uint8_t rank[kW4MaxExperts][kRowList];
+    uint8_t rank[kW4MaxExperts][kRowList];          // of the expert among the token's
     int warp_unique[kWarps], warp_most[kWarps];
     int n, most;                                    // unique experts, largest count
 };
@@ -781,37 +795,74 @@ __device__ __forceinline__ float warp_sums16(float (&v)[16]) {
     return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
 }
 
-// The CTA's columns' part of every (token, expert) logit.
-__device__ void partial_logits(const MoeArgs & a, int k0, int k1, float * out) {
+// Columns of the router that fit into `room` bytes for all experts: whole groups of 32.
+__device__ __forceinline__ int router_columns(int E, int room) { return room / (E * 128) * 32; }
+
+// Copies columns [k, k + n) of all router rows to shared memory, row e at e * n. The caller commits, waits and synchronises.
+__device__ __forceinline__ void fetch_router(const MoeArgs & a, int k, int n, uint8_t * to) {
+    const uint32_t dst = smem_address(to);
+    if (a.router_vec) {
+        const int chunks = n / 4;
+        for (int i = threadIdx.x; i < a.E * chunks; i += kThreads) {
+            const int e = i / chunks, c = i - e * chunks;
+            copy16(dst + i * 16, reinterpret_cast<const uint8_t *>(a.router + (size_t)e * a.d + k + c * 4));
+        }
+    } else {
+        for (int i = threadIdx.x; i < a.E * n; i += kThreads) {
+            const int e = i / n, c = i - e * n;
+            reinterpret_cast<float *>(to)[i] = a.router[(size_t)e * a.d + k + c];
+        }
+    }
+}
+
+// The CTA's columns' part of every (token, expert) logit, from the staged activations and, piece by piece, the router in
+// `room` (the first piece is already on its way). The sums are in the staged activations' scale.
+template <bool MX, int PARTS, int NT> __device__ void partial_logits(const MoeArgs & a, int k0, int k1, const Staged & x, uint8_t * room, int room_bytes, float * out) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int EB = 4, TB = 4;       // experts and tokens a warp takes at once
-    const Act router{a.router, a.d, GGML_F32, (uintptr_t)a.router % 16 == 0};
+    constexpr int EB = 4, TB = NT == 1 ? 1 : 4;         // experts and tokens a warp takes at once
+    const int width = router_columns(a.E, room_bytes);
     const int groups_t = (a.T + TB - 1) / TB, items = (a.E + EB - 1) / EB * groups_t;
-    for (int item = warp; item < items; item += kWarps) {
-        const int e0 = item / groups_t * EB, t0 = item % groups_t * TB;
-        float acc[EB * TB] = {};
-        for (int k = k0 + lane * 4; k < k1; k += 128) {
-            float r[EB][4], v[TB][4];
+    for (int k = k0; k < k1; k += width) {
+        const int n = min(width, k1 - k);
+        if (k > k0) {
+            __syncthreads();
+            fetch_router(a, k, n, room);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        const float * r = reinterpret_cast<const float *>(room);
+        for (int item = warp; item < items; item += kWarps) {
+            const int e0 = item / groups_t * EB, t0 = (item - item / groups_t * groups_t) * TB;
+            float acc[16] = {};
+            for (int c = lane * 4; c < n; c += 128) {
+                const int at = k - k0 + c, step = at >> 6, group = (at >> 5) & 1;
+                float4 w[EB];
 #pragma unroll
-            for (int e = 0; e < EB; ++e) load4(router, min(e0 + e, a.E - 1), k, r[e]);
+                for (int e = 0; e < EB; ++e) w[e] = *reinterpret_cast<const float4 *>(r + min(e0 + e, a.E - 1) * n + c);
+                const float factor = !MX && group ? 16.f : 1.f;
 #pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.f;
-                if (t0 + t < a.T) {
-                    load4(a.x, t0 + t, k, v[t]);
-                    if (a.norm) scale4(v[t], a.norm + k);
+                for (int t = 0; t < TB; ++t) {
+                    const uint8_t * p = x.x + ((step * 2 + group) * PARTS * NT + min(t0 + t, a.T - 1)) * 64 + (at & 31) * 2;
+                    const uint2 h = *reinterpret_cast<const uint2 *>(p);
+                    float2 v0 = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), v1 = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+                    if constexpr (PARTS == 2) {
+                        const uint2 l = *reinterpret_cast<const uint2 *>(p + NT * 64);
+                        const float2 l0 = __half22float2(*reinterpret_cast<const __half2 *>(&l.x)), l1 = __half22float2(*reinterpret_cast<const __half2 *>(&l.y));
+                        v0.x += l0.x; v0.y += l0.y; v1.x += l1.x; v1.y += l1.y;
+                    }
+#pragma unroll
+                    for (int e = 0; e < EB; ++e)
+                        acc[e * TB + t] += factor * (w[e].x * v0.x + w[e].y * v0.y + w[e].z * v1.x + w[e].w * v1.y);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < EB; ++e)
-#pragma unroll
-                    for (int t = 0; t < TB; ++t) acc[e * TB + t] += r[e][i] * v[t][i];
+            const float sum = warp_sums16(acc);
+            const int i = lane >> 1, e = e0 + i / TB, t = t0 + i % TB;
+            if (!(lane & 1) && i < EB * TB && e < a.E && t < a.T) {
+                if (k == k0) out[t * a.E + e] = sum;
+                else out[t * a.E + e] += sum;
+            }
         }
-        const float sum = warp_sums16(acc);
-        const int e = e0 + (lane >> 1) / TB, t = t0 + (lane >> 1) % TB;
-        if (!(lane & 1) && e < a.E && t < a.T) out[t * a.E + e] = sum;
     }
 }
 
@@ -826,13 +877,14 @@ __device__ void pick_experts(const float * logits, int E, int k, bool normalise,
     for (int j = 0; j < PER; ++j) {
         const int e = lane + 32 * j;
         p[j] = e < E ? logits[e] : -INFINITY;
-        mx = fmaxf(mx, p[j]);
+        if (32 * j < E) mx = fmaxf(mx, p[j]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
+        if (32 * j >= E) break;
         p[j] = lane + 32 * j < E ? expf(p[j] - mx) : 0.f;
         sum += p[j];
     }
@@ -842,6 +894,8 @@ __device__ void pick_experts(const float * logits, int E, int k, bool normalise,
     uint32_t key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
+        key[j] = 0;
+        if (32 * j >= E) continue;
         p[j] /= sum;
         key[j] = lane + 32 * j < E ? (p[j] >= 0.f ? __float_as_uint(p[j]) + 2u : 1u) : 0u;
     }
@@ -849,16 +903,16 @@ __device__ void pick_experts(const float * logits, int E, int k, bool normalise,
     for (int pick = 0; pick < k; ++pick) {
         uint32_t best = 0;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) best = max(best, key[j]);
+        for (int j = 0; j < PER; ++j) if (32 * j < E) best = max(best, key[j]);
         best = __reduce_max_sync(0xffffffffu, best);
         uint32_t at = 0xffffffffu;
 #pragma unroll
-        for (int j = PER - 1; j >= 0; --j) if (key[j] == best) at = lane + 32 * j;
+        for (int j = PER - 1; j >= 0; --j) if (32 * j < E && key[j] == best) at = lane + 32 * j;
         at = __reduce_min_sync(0xffffffffu, at);
         float value = 0.f;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            if (at == (uint32_t)(lane + 32 * j)) {
+            if (32 * j < E && at == (uint32_t)(lane + 32 * j)) {
                 value = p[j];
                 key[j] = 0;
             }
@@ -902,8 +956,7 @@ __device__ void group_picks(const MoeArgs & a, Picks & p, MoeMeta * meta) {
         for (uint32_t m = mask; m; m &= m - 1, ++i) {
             const int t = __ffs(m) - 1;
             p.token[u][i] = (uint8_t)t;
-            p.pair[u][i] = (uint16_t)(t * a.k + p.rank[e][t]);
-            if (meta) meta->pair[u][i] = p.pair[u][i];
+            if (meta) meta->pair[u][i] = (uint16_t)(t * a.k + p.rank[e][t]);
         }
         if (meta) {
             meta->expert[u] = (uint16_t)e;
@@ -939,11 +992,11 @@ template <bool MX, int PARTS, int NT> struct GateUpSource {
         c.rem = len;
     }
     __device__ __forceinline__ void first(Cursor & c) const {
-        c.job = (threadIdx.x >> 5) / ks;
+        c.job = (threadIdx.x >> 5) >> (__ffs(ks) - 1);
         point(c);
     }
     __device__ __forceinline__ void next(Cursor & c) const {
-        c.job += kWarps / ks;
+        c.job += kWarps >> (__ffs(ks) - 1);
         point(c);
     }
     __device__ __forceinline__ Group group(const Cursor & c) const { return {x, p.token[c.group], p.count[c.group], 0}; }
@@ -962,7 +1015,8 @@ __global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_moe_gate_up_kerne
     const int rank = (int)cluster_rank(), C = (int)cluster_size();
     const int cluster = blockIdx.x / C;
     cluster_arrive();
-    const int s0 = part_begin(a.steps_d, rank, C), n_steps = part_begin(a.steps_d, rank + 1, C) - s0;
+    const int log_c = __ffs(C) - 1;
+    const int s0 = part_begin2(a.steps_d, rank, log_c), n_steps = part_begin2(a.steps_d, rank + 1, log_c) - s0;
     const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
     float * mine = reinterpret_cast<float *>(smem + a.x_bytes + a.c_bytes);         // this CTA's part of the logits
     float * logits = mine + a.logit_bytes / 4;
@@ -972,8 +1026,15 @@ __global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_moe_gate_up_kerne
 
     pdl_trigger();
     pdl_wait();
-    partial_logits(a, s0 * 64, min(a.d, (s0 + n_steps) * 64), mine);
+    const int k0 = s0 * 64, k1 = min(a.d, (s0 + n_steps) * 64);
+    fetch_router(a, k0, min(k1 - k0, router_columns(a.E, ring_bytes(MX, NT))), rings);      // the rings are idle until the experts are known
+    asm volatile("cp.async.commit_group;" ::: "memory");
     stage_tokens<MX, PARTS>(a.x, a.T, NT, s0, n_steps, a.d, a.norm, x, sc, rank, C);
+    __syncthreads();
+    partial_logits<MX, PARTS, NT>(a, k0, k1, x, rings, ring_bytes(MX, NT), mine);
+    // out of the activations' scale: a token's factors without the weights' constant
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.T * a.E; i += kThreads) mine[i] = mine[i] * sc.f1[0][i / a.E] * sc.f2[0][i / a.E] * (MX ? 0.015625f : 5.9604644775390625e-8f);
     cluster_sync();
     for (int i = threadIdx.x; i < a.T * a.E; i += kThreads) {
         float part[kMaxCluster];
@@ -1001,11 +1062,12 @@ __global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_moe_gate_up_kerne
     const int b_begin = part_begin(total, cluster, a.clusters), blocks = part_begin(total, cluster + 1, a.clusters) - b_begin;
     const int ks = split_columns(blocks * 2, a.steps_d / C, (int)(a.inbox / inbox_bytes(most, C, 1, 2)));
     const int per_round = blocks_per_round(a.inbox, most, C, ks, 2);
-    const int sub = warp % ks, step = part_begin(n_steps, sub, ks), len = part_begin(n_steps, sub + 1, ks) - step;
+    const int log_ks = __ffs(ks) - 1;
+    const int sub = warp & (ks - 1), step = part_begin2(n_steps, sub, log_ks), len = part_begin2(n_steps, sub + 1, log_ks) - step;
     const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
-    const Inbox inbox{smem_address(rings + ring_bytes(MX)), a.inbox, rank, __ffs(C) - 1, ks, 2};
+    const Inbox inbox{smem_address(rings + ring_bytes(MX, NT)), a.inbox, rank, log_c, ks, 2};
     GateUpSource<MX, PARTS, NT> src{a, picks, x_warp, inbox, 2 * b_begin, 2 * blocks, ks, most, sub, s0 + step, len, 0, 0};
-    Stream<MX, GateUpSource<MX, PARTS, NT>> stream(src, rings);
+    Stream<MX, stages_for(NT), GateUpSource<MX, PARTS, NT>> stream(src, rings);
     stream.prefetch();
     for (int b0 = 0; b0 < blocks; b0 += per_round, ++src.round) {
         const int now = min(per_round, blocks - b0);
@@ -1016,7 +1078,7 @@ __global__ void __launch_bounds__(kThreads, NT > 8 ? 2 : 3) w4_moe_gate_up_kerne
             const int unit = i * C + rank, b = unit / most, col = unit - b * most;
             const int u = (b_begin + b0 + b) / a.blocks_ff, row = ((b_begin + b0 + b) - u * a.blocks_ff) * 32 + lane;
             if (col >= picks.count[u]) continue;
-            const int t = picks.token[u][col], pair = picks.pair[u][col];
+            const int t = picks.token[u][col], pair = t * a.k + picks.rank[picks.unique[u]][t];
             const float v = inbox.sum(src.round, i, 0) * picks.rstd[t], up = inbox.sum(src.round, i, 1) * picks.rstd[t];
             if (row < a.ff) a.h[pair * a.ld_h + row] = picks.weight[pair] * (v / (1.f + expf(-v)) * up);
         }
@@ -1081,28 +1143,28 @@ template <bool MX> struct DownSource {
             c.live = c.group < table.n;
             if (!c.live) return;
             const Seg & g = table.seg[c.group];
-            const int s = part_begin(g.len, sub, ks);
-            c.rem = part_begin(g.len, sub + 1, ks) - s;
+            const int log_ks = __ffs(ks) - 1, s = part_begin2(g.len, sub, log_ks);
+            c.rem = part_begin2(g.len, sub + 1, log_ks) - s;
             if (c.job < jobs && c.rem > 0) {
                 c.p = a.down + g.expert * a.down_expert + ((size_t)(job0 + c.job) * a.steps_ff + g.s0 + s) * w4_unit_bytes(MX);
                 return;
             }
             ++c.group;
-            c.job = (threadIdx.x >> 5) / ks;
+            c.job = (threadIdx.x >> 5) >> (__ffs(ks) - 1);
         }
     }
     __device__ __forceinline__ void first(Cursor & c) const {
         c.group = 0;
-        c.job = (threadIdx.x >> 5) / ks;
+        c.job = (threadIdx.x >> 5) >> (__ffs(ks) - 1);
         point(c);
     }
     __device__ __forceinline__ void next(Cursor & c) const {
-        c.job += kWarps / ks;
+        c.job += kWarps >> (__ffs(ks) - 1);
         point(c);
     }
     __device__ __forceinline__ Group group(const Cursor & c) const {
         const Seg & g = table.seg[c.group];
-        const int s = part_begin(g.len, sub, ks), nt = room_for(g.n);
+        const int s = part_begin2(g.len, sub, __ffs(ks) - 1), nt = room_for(g.n);
         return {{smem + g.x_off + s * step_x_bytes(2, nt), reinterpret_cast<float *>(smem + g.c_off + s * step_c_bytes(MX, nt))}, nullptr, g.n, c.group};
     }
     __device__ __forceinline__ void put(const Cursor & c, int row, int col, float v) const {
@@ -1121,8 +1183,8 @@ __global__ void __launch_bounds__(kThreads, MOST > 8 ? 2 : 3) w4_moe_down_kernel
     const int cluster = blockIdx.x / C;
     cluster_arrive();
     uint8_t * const rings = smem + a.x_bytes;
-    float * partial = reinterpret_cast<float *>(rings + ring_bytes(MX));
-    const Inbox inbox{smem_address(rings + ring_bytes(MX) + a.partial), a.inbox, rank, __ffs(C) - 1, 1, 1};
+    float * partial = reinterpret_cast<float *>(rings + ring_bytes(MX, MOST));
+    const Inbox inbox{smem_address(rings + ring_bytes(MX, MOST) + a.partial), a.inbox, rank, __ffs(C) - 1, 1, 1};
     const int j_begin = part_begin(a.blocks_d, cluster, a.clusters), j_end = part_begin(a.blocks_d, cluster + 1, a.clusters);
     if (threadIdx.x == 0) sc.zero = 0;
     pdl_trigger();
@@ -1136,7 +1198,7 @@ __global__ void __launch_bounds__(kThreads, MOST > 8 ? 2 : 3) w4_moe_down_kernel
     cluster_wait();
     __syncthreads();
     const int total = meta.n * a.steps_ff;          // the chosen experts' columns, one behind the other
-    const int begin = part_begin(total, rank, C), end = part_begin(total, rank + 1, C);
+    const int begin = part_begin2(total, rank, __ffs(C) - 1), end = part_begin2(total, rank + 1, __ffs(C) - 1);
     const int slot = a.T * kSlotCol * 4;
     const int ks = split_columns(j_end - j_begin, max(1, total / C), a.partial / slot);
     const int per_round = min(a.partial / (slot * ks), blocks_per_round(a.inbox, a.T, C, 1, 1));
@@ -1150,7 +1212,7 @@ __global__ void __launch_bounds__(kThreads, MOST > 8 ? 2 : 3) w4_moe_down_kernel
             if (warp == 0) cut_segments<MX>(a, meta, p, end, a.x_bytes - 16, table);
             __syncthreads();
             const DownSource<MX> src{a, table, smem, partial, j0, jobs, ks, warp % ks};
-            Stream<MX, DownSource<MX>> stream(src, rings);
+            Stream<MX, stages_for(MOST), DownSource<MX>> stream(src, rings);
             stream.prefetch();
             stage_rows<MX, 2, false>(h, table.rows, a.ff, nullptr, sc, [&](int i) {
                 int n = 0;
@@ -1370,6 +1432,36 @@ void launch_w4_retile(const uint8_t * rows, uint32_t type, uint32_t n_out, uint3
     else w4_retile_kernel<false><<<(unsigned)n, 256, 0, stream>>>(rows, n_out, n_in, v.blocks, v.steps, units, max_scale);
 }
 
+// Clusters of a size that are on the GPU together, with `resident` CTAs on an SM: a cluster lies within one of the GPU's processing
+// clusters, whose SM counts are no multiples of it. Asked once per device.
+int resident_clusters(int log_c, int resident) {
+    struct Table { std::atomic<int> n[4][3]; };
+    static Table tables[64];
+    int device = 0;
+    cudaGetDevice(&device);
+    std::atomic<int> & known = tables[device & 63].n[log_c][resident - 1];
+    int n = known.load();
+    if (n) return n;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << log_c;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1u << log_c);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = std::min(kMaxSmem, 226 * 1024 / resident - 4096);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static PerDeviceOnce once;
+    auto kernel = w4_product_kernel<false, 2, false, 1>;
+    if (allow_smem(once, kernel) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = std::max(1, resident * device_sms() >> log_c);
+    }
+    known.store(n);
+    return n;
+}
+
 // How a product is cut: CTAs of a cluster, clusters, and the shared memory of a CTA.
 struct Cut {
     int C = 0, clusters = 0, resident = 0;
@@ -1390,10 +1482,13 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, int ring, int fi
         Cut c;
         c.C = C;
         c.resident = (int)std::min<int64_t>(n > 8 ? 2 : 3, 226 * 1024 / smem);
-        const int most = std::max(1, c.resident * sms / C), blocks_each = (blocks + most - 1) / most;
+        if (const char * e = std::getenv("W4_RES")) c.resident = std::min(c.resident, atoi(e));
+        if (const char * e = std::getenv("W4_C")) if (C != atoi(e)) continue;
+        const int log_c = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
+        const int most = resident_clusters(log_c, c.resident), blocks_each = (blocks + most - 1) / most;
         c.clusters = (blocks + blocks_each - 1) / blocks_each;
         const int busy = (c.clusters * C + sms - 1) / sms;
-        const double in_flight = (double)busy * ring * (kStages - 1) / kStages;
+        const double in_flight = (double)busy * ring * (stages_for(n) - 1) / stages_for(n);
         const double stream = std::max((double)blocks * per * steps * unit / (23.5 * sms), (double)busy * blocks_each * per * s * unit / std::min(46.0, in_flight / 1600.0));
         const double convert = busy * s * (n * 64 * 0.12 + step_clocks) + 800, sums = busy * (double)blocks_each * per * n * 8;
         c.cost = stream + convert + sums;
@@ -1411,7 +1506,7 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
         Cut cut;
         for (;; n = (n + 1) / 2) {
-            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), ring_bytes(mx), 0, 0, (int)w4_unit_bytes(mx), sms);
+            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), ring_bytes(mx, product_room(n, parts)), 0, 0, (int)w4_unit_bytes(mx), sms);
             if (cut.C || n == 1) break;
         }
         if (!cut.C) return cudaErrorInvalidValue;       // rows this long are refused when the handle is made
@@ -1432,17 +1527,19 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         a.y = const_cast<void *>(row_at(p.y, p.y_type, p.ld_y, t0));
         a.y_type = p.y_type;
         a.ld_y = p.ld_y;
-        a.blocks = blocks;
+        a.each = blocks / cut.clusters;
+        a.more = blocks % cut.clusters;
         a.clusters = cut.clusters;
         a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
         // two inboxes in what is left of the CTA's share of the shared memory; one, if everything fits into it
-        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx);
+        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx, nt);
         const int blocks_each = (blocks + cut.clusters - 1) / cut.clusters;
         const int room = std::min(226 * 1024 / cut.resident - 4096, kMaxSmem) - fixed;
         a.ks = split_columns(blocks_each * per, steps / C, (int)std::max<int64_t>(1, room / 2 / inbox_bytes(n, C, 1, per)));
         const int64_t whole = inbox_bytes((int64_t)blocks_each * n, C, a.ks, per);
         a.inbox = (int)(whole <= room ? whole : std::max<int64_t>(room / 2 / 128 * 128, inbox_bytes(n, C, a.ks, per)));
+        a.per_round = blocks_per_round(a.inbox, n, C, a.ks, per);
         const size_t smem = (size_t)fixed + (whole <= room ? 1 : 2) * (size_t)a.inbox;
         cudaError_t e;
         if (mx) e = glu ? launch_product_of<true, true>(a, parts, C, smem, stream) : launch_product_of<true, false>(a, parts, C, smem, stream);
@@ -1470,8 +1567,8 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         Cut cut;
         for (;; n = (n + 1) / 2) {
             reach = (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n)));
-            cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), ring_bytes(mx),
-                             2 * up_to(n * E * 4, 128) + 24 * 1024, n * E * 0.65 + E * 8, (int)w4_unit_bytes(mx), sms);
+            cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), ring_bytes(mx, product_room(n, parts)),
+                             2 * up_to(n * E * 4, 128) + 16 * 1024, n * E * 0.65 + E * 8, (int)w4_unit_bytes(mx), sms);
             if (cut.C || n == 1) break;
         }
         if (!cut.C) return cudaErrorInvalidValue;
@@ -1484,6 +1581,7 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.up_expert = p.up.expert_bytes;
         a.down_expert = p.down.expert_bytes;
         a.router = p.router;
+        a.router_vec = (uintptr_t)p.router % 16 == 0;
         a.x = make_act(row_at(p.x, p.x_type, p.ld_x, t0), p.ld_x, p.x_type);
         a.T = n;
         a.E = E;
@@ -1513,20 +1611,20 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
         a.logit_bytes = up_to(n * E * 4, 128);
         a.clusters = cut.clusters;
-        int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx);
-        a.inbox = (int)std::max<int64_t>((std::min(226 * 1024 / cut.resident - 28 * 1024, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, C, 1, 2));
+        int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx, nt);
+        a.inbox = (int)std::max<int64_t>((std::min(226 * 1024 / cut.resident - 20 * 1024, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, C, 1, 2));
         cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, C, (size_t)fixed + 2 * a.inbox, stream) : launch_gate_up_of<false>(a, parts, C, (size_t)fixed + 2 * a.inbox, stream);
         if (e != cudaSuccess) return e;
 
         // second kernel
         C = kMaxCluster;
         while (C > steps_ff * p.n_used) C /= 2;
-        const int resident = n > 8 ? 2 : 3;
-        const int most = std::max(1, resident * sms / C), per = (a.blocks_d + most - 1) / most;
+        const int resident = 2;
+        const int most = resident_clusters(C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3, resident), per = (a.blocks_d + most - 1) / most;
         a.clusters = (a.blocks_d + per - 1) / per;
-        a.x_bytes = (n > 8 ? 32 : n > 1 ? 16 : 12) * 1024;
+        a.x_bytes = (n > 8 ? 24 : n > 1 ? 20 : 12) * 1024;
         a.c_bytes = a.logit_bytes = 0;
-        const int slot = n * kSlotCol * 4, down_fixed = a.x_bytes + ring_bytes(mx_down);
+        const int slot = n * kSlotCol * 4, down_fixed = a.x_bytes + ring_bytes(mx_down, n == 1 ? 1 : n <= 4 ? 4 : 8);
         a.inbox = (int)inbox_bytes(std::min(per, kWarps) * n, C, 1, 1);
         a.partial = std::max(kWarps * slot, std::min(per * kWarps * slot, 226 * 1024 / resident - 18 * 1024 - down_fixed - 2 * a.inbox) / slot * slot);
         const size_t smem = (size_t)down_fixed + a.partial + 2 * a.inbox;
