@@ -498,7 +498,7 @@ int retro_b200_gemm_q4k_noalloc(const uint8_t * d_w, uint32_t n_out, uint32_t n_
  *
  * retro_b200_w4_new lays `rows` ([n_expert][n_out][n_in / 32 blocks], host or device memory, read before the call returns) out on
  * the current device, in about the same number of bytes; n_expert is 1 for a plain matrix. NULL and a message when the type is another one,
- * n_in is no multiple of 32 or above 262144, n_expert is above 256, or an MXFP4 scale is above 2^96. The handle is immutable: calls
+ * n_in is no multiple of 32 or above 262144, n_expert is above 256, or an MXFP4 scale is above 2^80. The handle is immutable: calls
  * from several threads and streams may use it at once. Free it when no call that uses it is pending.
  *
  * The calls below take DEVICE pointers on the handle's device, whichever device is current, enqueue on `stream` (a cudaStream_t of that device,

@@ -13,13 +13,14 @@ constexpr int kW4PassTokens = 16;            // tokens one launch serves; longer
 constexpr uint32_t kW4MaxColumns = 262144;   // longest row: one token's activations of an eighth of it fit in shared memory
 constexpr uint32_t kW4MaxExperts = 256;
 constexpr uint32_t kW4MaxUsed = 32;          // experts per token
-constexpr uint32_t kW4MaxScaleByte = 223;    // MXFP4: weight scales up to 2^96, so that a row's scaled sum stays inside f32
+constexpr uint32_t kW4MaxScaleByte = 207;    // MXFP4: weight scales up to 2^80, so that a row's scaled sum stays inside f32
 
-// Device layout: units of 32 rows x 64 columns, a row block's units consecutive over the columns, row blocks consecutive,
-// experts consecutive. A unit is, for each of its two 16-row tiles, 32 x 16 bytes, one 16-byte word per lane of the warp that multiplies it (the lane's share
-// of the A fragments of four m16n8k16 products), then for each tile the 16 rows' two scales: 64 bytes of f16 or 32 bytes. Rows and
-// columns beyond the matrix have scale zero. The bit order inside a word is described at w4_retile_kernel.
-__host__ __device__ constexpr uint32_t w4_unit_bytes(bool mxfp4) { return mxfp4 ? 1088u : 1152u; }
+// Device layout: units of 32 rows x 128 columns, a row block's units consecutive over the columns, row blocks consecutive,
+// experts consecutive. A unit is, for each 64-column half and 16-row tile, 32 x 16 bytes, one 16-byte word per lane of the warp that
+// multiplies it (the lane's share of the A fragments of four m16n8k16 products), then for each tile the 16 rows' four
+// scales: 128 bytes of f16 or 64 bytes. Rows and columns beyond the matrix have scale zero. The bit order inside a word is described at
+// w4_retile_kernel.
+__host__ __device__ constexpr uint32_t w4_unit_bytes(bool mxfp4) { return mxfp4 ? 2176u : 2304u; }
 
 struct W4View {
     const uint8_t * units = nullptr;
@@ -27,7 +28,7 @@ struct W4View {
     uint32_t n_out = 0, n_in = 0;
     uint32_t n_expert = 1;
     uint32_t blocks = 0;            // 32-row blocks of one expert
-    uint32_t steps = 0;             // 64-column steps
+    uint32_t steps = 0;             // 128-column steps
     size_t expert_bytes = 0;
 };
 

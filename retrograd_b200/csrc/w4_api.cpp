@@ -105,7 +105,7 @@ retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_
         if (n_out == 0 || n_in == 0 || n_in % 32 != 0) return refuse(op, "n_out must be at least 1 and n_in a multiple of 32");
         if (n_in > kW4MaxColumns) return refuse(op, "n_in is larger than 262144");
         if (n_expert == 0 || n_expert > kW4MaxExperts) return refuse(op, "n_expert must be 1 to 256");
-        if ((uint64_t)n_expert * (((uint64_t)n_out + 31) / 32) * ((n_in + 63) / 64) > 0x7fffffffull) return refuse(op, "the bank is too large");
+        if ((uint64_t)n_expert * (((uint64_t)n_out + 31) / 32) * ((n_in + 127) / 128) > 0x7fffffffull) return refuse(op, "the bank is too large");
         auto w = std::make_unique<retro_b200_w4>();
         RB_CUDA(cudaGetDevice(&w->device));
         w->bytes = w4_bytes(ggml_type, n_out, n_in, n_expert);
@@ -126,7 +126,7 @@ retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_
         int h_max = 0;
         RB_CUDA(cudaMemcpyAsync(&h_max, d_max, sizeof h_max, cudaMemcpyDeviceToHost, raw.s));
         RB_CUDA(cudaStreamSynchronize(raw.s));
-        if (h_max > (int)kW4MaxScaleByte) return refuse(op, "an MXFP4 scale byte is above 223 (2^96)");
+        if (h_max > (int)kW4MaxScaleByte) return refuse(op, "an MXFP4 scale byte is above 207 (2^80)");
         made = w.release();
         return STATUS_OK;
     });
