@@ -208,16 +208,17 @@ struct Staged {
 };
 
 template <int WARPS> struct Scratch {
-    float f1[kRowList], f2[kRowList];           // a token's sums times f1 times f2 are in the activations' own scale
+    float factor[kRowList];                     // a token's sums times it are in the activations' own scale
     float ss[kMaxCluster][kRowList];            // sums of squares of each CTA's columns
     uint32_t top[WARPS];
     float squares[WARPS];
     uint64_t zero;                              // start values of PACK's lo columns
 };
 
-// 2^shift brings the magnitude with these bits into [2^13, 2^14), as far as it is an f32 itself (below 2^-113 the values only come
-// near). Rows with an infinity or a NaN are left as they are: their own sums become NaN, those of the other tokens stay what they are.
-__device__ __forceinline__ int shift_for(uint32_t top) { return top > 0 && top < 0x7f800000u ? min(126, 140 - (int)(top >> 23)) : 0; }
+// 2^shift brings the magnitude with these bits into [2^13, 2^14), as far as it and the factor that takes it back are f32 (below 2^-113 the
+// values only come near; above 2^113 they count as infinite). Rows with an infinity or a NaN are left as they are: their own
+// sums become NaN, those of the other tokens stay what they are.
+__device__ __forceinline__ int shift_for(uint32_t top) { return top > 0 && top < 0x7f800000u ? max(-100, min(126, 140 - (int)(top >> 23))) : 0; }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // The power of two a sum is short of: of the weights' f16 form, and of MXFP4's scale bytes (kept plus 8).
 __host__ __device__ constexpr int weight_shift(bool mx) { return mx ? -8 : 24; }
@@ -300,9 +301,7 @@ __device__ void stage_rows(const Act & act, int n, int nt, int k0, int steps, in
     const int shift = shift_for(top);
     const float up = power(shift);
     if (part == 0 && lane == 0) {
-        const int down = weight_shift(MX) - shift;
-        sc.f1[row] = power(down / 2);
-        sc.f2[row] = power(down - down / 2);
+        sc.factor[row] = power(weight_shift(MX) - shift);
         if constexpr (NORM) put_squares(row, squares);
     }
     for (int it0 = 0; it0 < trips; it0 += kHeld) {
@@ -365,7 +364,7 @@ struct Group {
 struct Lane {
     uint32_t b[2], c[2][2];             // shared-memory addresses at the group's first step
     uint32_t c_step, c_group;
-    float f1[2][2], f2[2][2];
+    float factor[2][2];
 };
 
 // OWN: every group of columns has factors of its own (see Staged).
@@ -386,10 +385,7 @@ __device__ __forceinline__ void begin_group(const Group & r, int lane, const S &
         for (int e = 0; e < 2; ++e) {
             const int tok = place(lo ? (2 * t4 + e) & 3 : 8 * nc + 2 * t4 + e);
             l.c[nc][e] = c + tok * (OWN ? 8 : 4);
-            if constexpr (!OWN) {
-                l.f1[nc][e] = sc.f1[tok];
-                l.f2[nc][e] = sc.f2[tok];
-            }
+            if constexpr (!OWN) l.factor[nc][e] = sc.factor[tok];
         }
     if constexpr (!MX && lo && !OWN) {
         if (t4 >= 2) {              // the lo columns carry no offset
@@ -484,26 +480,33 @@ __device__ __forceinline__ void do_step(uint32_t words, uint32_t scale_at, uint3
     do_group<MX, PARTS, MODE, NT, OWN, 3>(u, sc, b_at, c_at, l, lane, acc);
 }
 
-// Hands a run's sums to put(row 0..31 of the block, column, sum) and clears them.
-template <int MODE, int NT, bool OWN, class Put>
-__device__ __forceinline__ void end_run(int n, int lane, const Lane & l, float (&acc)[2][2][4], Put put) {
-    const int g = lane >> 2, t4 = lane & 3;
+// Hands on a run's sums and clears them: begin(column), then put(row - lane / 4, sum) for the lane's four rows of the block.
+template <int MODE, int NT, bool OWN, class Begin, class Put>
+__device__ __forceinline__ void end_run(int n, int lane, const Lane & l, float (&acc)[2][2][4], Begin begin, Put put) {
+    const int t4 = lane & 3;
 #pragma unroll
     for (int nc = 0; nc < (MODE == TWO ? 2 : 1); ++nc)
 #pragma unroll
         for (int e = 0; e < (NT > 1 ? 2 : 1); ++e) {
             const int col = 8 * nc + 2 * t4 + e;
             const bool mine = col < n && !(MODE == PACK && t4 >= 2);
+            if constexpr (MODE == PACK) {
 #pragma unroll
-            for (int tile = 0; tile < 2; ++tile)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float & a = acc[tile][nc][e + 2 * half];
-                    float v = a;
-                    if constexpr (MODE == PACK) v += __shfl_xor_sync(0xffffffffu, v, 2);      // hi column + lo column
-                    if (mine) put(tile * 16 + g + half * 8, col, OWN ? v : v * l.f1[nc][e] * l.f2[nc][e]);
-                    a = 0.f;
+                for (int i = 0; i < 4; ++i) {
+                    float & a = acc[i >> 1][nc][e + 2 * (i & 1)];
+                    a += __shfl_xor_sync(0xffffffffu, a, 2);        // hi column + lo column
                 }
+            }
+            if (mine) {
+                begin(col);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = acc[i >> 1][nc][e + 2 * (i & 1)];
+                    put(i * 8, OWN ? a : a * l.factor[nc][e]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i >> 1][nc][e + 2 * (i & 1)] = 0.f;
         }
 }
 
@@ -516,7 +519,7 @@ struct Cursor {
 };
 
 // Runs a warp's sequence. Source: first(Cursor &) and next(Cursor &) move to a run (never an empty one) and set everything;
-// group(const Cursor &) describes the activations; put(const Cursor &, row, column, sum) takes the sums.
+// group(const Cursor &) describes the activations; column(const Cursor &, column) is the cluster address that takes 32 rows' sums.
 // LIST: groups name their tokens.
 template <bool MX, class Source> struct Stream {
     static constexpr uint32_t kUnit = w4_unit_bytes(MX);
@@ -566,7 +569,8 @@ template <bool MX, class Source> struct Stream {
                 b_at += OWN ? step_h_bytes(NT) : step_x_bytes(PARTS, NT);
                 c_at += l.c_step;
             }
-            end_run<MODE, NT, OWN>(r.n, lane, l, acc, [&](int row, int col, float v) { src.put(cp, row, col, v); });
+            uint32_t to = 0;
+            end_run<MODE, NT, OWN>(r.n, lane, l, acc, [&](int col) { to = src.column(cp, col) + (lane >> 2) * 4; }, [&](int row, float v) { remote_store(to + row * 4, v); });
             src.next(cp);
         } while (cp.live && cp.group == group && cp.job < limit);
     }
@@ -620,9 +624,10 @@ struct Inbox {
     int bytes;                  // of one of the two
     int rank, log_c, ks, per;   // per: matrices of a block
 
-    __device__ __forceinline__ void put(int round, int unit, int which, int sub, int row, float v) const {
+    // The cluster address of 32 rows' sums.
+    __device__ __forceinline__ uint32_t slot(int round, int unit, int which, int sub) const {
         const int from = (((unit >> log_c) * per + which) << log_c | rank) * ks + sub;
-        remote_store(remote_address(base + (round & 1) * bytes + (from * 32 + row) * 4, unit & ((1 << log_c) - 1)), v);
+        return remote_address(base + (round & 1) * bytes + from * 128, unit & ((1 << log_c) - 1));
     }
     // Row `lane` of the sum over the cluster for the CTA's own unit number `mine`, in the order of the columns.
     __device__ __forceinline__ float sum(int round, int mine, int which) const {
@@ -687,9 +692,9 @@ template <bool MX, int PARTS, bool GLU, int NT> struct ProductSource {
         point(c);
     }
     __device__ __forceinline__ Group group(const Cursor &) const { return {x, nullptr, a.T}; }
-    __device__ __forceinline__ void put(const Cursor & c, int row, int col, float v) const {
+    __device__ __forceinline__ uint32_t column(const Cursor & c, int col) const {
         const int job = c.job - round0;
-        inbox.put(round, (GLU ? job >> 1 : job) * a.T + col, GLU ? job & 1 : 0, sub, row, v);
+        return inbox.slot(round, (GLU ? job >> 1 : job) * a.T + col, GLU ? job & 1 : 0, sub);
     }
 };
 
@@ -806,8 +811,10 @@ struct Picks {
     uint32_t mask[kW4MaxExperts];                   // by expert: the tokens that chose it
     uint8_t rank[kW4MaxExperts][kRowList];          // of the expert among the token's
     int sums[3][8];
-    int most[8];
-    int n, widest;                                  // unique experts, largest count
+    int n;                                          // unique experts
+
+    // Units are the (block, token) results of the chosen experts' blocks, one behind the other: the first of a block.
+    __device__ __forceinline__ int unit(int u, int block, int blocks) const { return before[u] * blocks + block * count[u]; }
 };
 
 // Sums each of the 16 values of a lane over the warp; lane i ends up with value i >> 1 (lanes 2 i and 2 i + 1 alike).
@@ -980,19 +987,16 @@ __device__ void group_picks(const MoeArgs & a, Picks & p, MoeMeta * meta) {
             if (lane >= o) sum[i] += v;
         }
     }
-    const uint32_t most = __reduce_max_sync(0xffffffffu, (uint32_t)n);
     if (warp < 8 && lane == 31) {
 #pragma unroll
         for (int i = 0; i < 3; ++i) p.sums[i][warp] = sum[i];
-        p.most[warp] = (int)most;
     }
     __syncthreads();
-    int before[3] = {sum[0] - (n > 0), sum[1] - n, sum[2] - sets}, all = 0, all_sets = 0, widest = 1;
+    int before[3] = {sum[0] - (n > 0), sum[1] - n, sum[2] - sets}, all = 0, all_sets = 0;
     for (int w = 0; w < 8; ++w) {
         if (w < warp) { before[0] += p.sums[0][w]; before[1] += p.sums[1][w]; before[2] += p.sums[2][w]; }
         all += p.sums[0][w];
         all_sets += p.sums[2][w];
-        widest = max(widest, p.most[w]);
     }
     if (mask) {
         const int u = before[0];
@@ -1015,7 +1019,6 @@ __device__ void group_picks(const MoeArgs & a, Picks & p, MoeMeta * meta) {
     }
     if (e == 0) {
         p.n = all;
-        p.widest = widest;
         if (meta) meta->n = all_sets;
     }
     __syncthreads();
@@ -1029,9 +1032,8 @@ template <bool MX, int PARTS, int NT> struct GateUpSource {
     Inbox inbox;
     int job0, jobs;
     int first_job, stride;
-    int widest;
     int sub, step, len;
-    int round, round0;
+    int round, unit0;           // the round, and its first unit
 
     // Cursor::group is the expert's place among the chosen ones.
     __device__ __forceinline__ void point(Cursor & c) const {
@@ -1053,9 +1055,9 @@ template <bool MX, int PARTS, int NT> struct GateUpSource {
         point(c);
     }
     __device__ __forceinline__ Group group(const Cursor & c) const { return {x, p.token[c.group], p.count[c.group]}; }
-    __device__ __forceinline__ void put(const Cursor & c, int row, int col, float v) const {
-        const int job = c.job - round0;
-        inbox.put(round, (job >> 1) * widest + col, job & 1, sub, row, v);
+    __device__ __forceinline__ uint32_t column(const Cursor & c, int col) const {
+        const int job = job0 + c.job;
+        return inbox.slot(round, p.unit(c.group, (job >> 1) - c.group * a.blocks_ff, a.blocks_ff) - unit0 + col, job & 1, sub);
     }
 };
 
@@ -1065,7 +1067,7 @@ __device__ __forceinline__ void put_hidden(const MoeArgs & a, const Picks & p, i
     const int set = col / kSet, place = col - set * kSet, nt = min(kSet, p.count[u] - set * kSet);
     uint8_t * at = a.hidden + ((size_t)(p.before[u] + set * kSet) * a.steps_ff + (size_t)(block >> 2) * nt) * kHiddenBytes;
     const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
-    const int shift = max(-100, shift_for(top));            // so that the factor below is an f32
+    const int shift = shift_for(top);
     const int last = block == a.blocks_ff - 1 ? 3 : block & 3;
     for (int group = block & 3; group <= last; ++group) {
         if (group != (block & 3)) v = 0.f;
@@ -1112,7 +1114,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
     partial_logits<MX, PARTS, NT, kWarps>(a, k0, k1, x, rings, ring_bytes(MX, kWarps), mine);
     // out of the activations' scale: a token's factors without the weights' constant
     __syncthreads();
-    for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) mine[i] = mine[i] * sc.f1[i / a.E] * sc.f2[i / a.E] * power(-weight_shift(MX));
+    for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) mine[i] *= sc.factor[i / a.E] * power(-weight_shift(MX));
     cluster_sync();
     for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) {
         const uint32_t at = smem_address(mine + i);
@@ -1137,29 +1139,44 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
         }
     }
 
-    const int total = picks.n * a.blocks_ff, widest = picks.widest;
+    const int total = picks.n * a.blocks_ff;
     const int b_begin = part_begin(total, cluster, a.clusters), blocks = part_begin(total, cluster + 1, a.clusters) - b_begin;
-    const int ks = split_columns(blocks * 2, a.steps_d >> log_c, kWarps, (int)(a.inbox / inbox_bytes(widest, C, 1, 2))), log_ks = __ffs(ks) - 1;
-    const int per_round = blocks_per_round(a.inbox, widest, C, ks, 2, kWarps);
+    // parts of the columns: no more than the inbox has room for with every token at one expert
+    const int ks = split_columns(blocks * 2, a.steps_d >> log_c, kWarps, (int)(a.inbox / inbox_bytes(a.T, C, 1, 2))), log_ks = __ffs(ks) - 1;
+    const int room = (a.inbox >> (log_c + log_ks + 8)) << log_c;        // units of a round
     const int sub = warp & (ks - 1), step = part_begin2(n_steps, sub, log_ks), len = part_begin2(n_steps, sub + 1, log_ks) - step;
     const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
     const Inbox inbox{smem_address(rings + ring_bytes(MX, kWarps)), a.inbox, rank, log_c, ks, 2};
-    GateUpSource<MX, PARTS, NT> src{a, picks, x_warp, inbox, 2 * b_begin, 2 * blocks, warp >> log_ks, kWarps >> log_ks, widest, sub, s0 + step, len, 0, 0};
+    GateUpSource<MX, PARTS, NT> src{a, picks, x_warp, inbox, 2 * b_begin, 2 * blocks, warp >> log_ks, kWarps >> log_ks, sub, s0 + step, len, 0, 0};
     Stream<MX, GateUpSource<MX, PARTS, NT>> stream(src, rings);
     stream.prefetch();
-    for (int b0 = 0; b0 < blocks; b0 += per_round, ++src.round) {
-        const int now = min(per_round, blocks - b0);
-        src.round0 = 2 * b0;
+    int u = b_begin / a.blocks_ff, block = b_begin - u * a.blocks_ff;       // where the round begins
+    for (int b0 = 0; b0 < blocks; ++src.round) {
+        // as many blocks as the inbox has room for
+        const int u0 = u, block0 = block;
+        int now = 0, units = 0;
+        while (b0 + now < blocks) {
+            const int n = picks.count[u], more = min(min(a.blocks_ff - block, blocks - b0 - now), (room - units) / n);
+            now += more;
+            units += more * n;
+            block += more;
+            if (block < a.blocks_ff) break;
+            ++u;
+            block = 0;
+        }
+        src.unit0 = picks.unit(u0, block0, a.blocks_ff);
         stream.template work<PARTS, NT, (NT > 1)>(sc, 2 * (b0 + now));
         cluster_sync();
-        for (int i = warp; i * C + rank < now * widest; i += kWarps) {
-            const int unit = i * C + rank, b = unit / widest, col = unit - b * widest;
-            const int u = (b_begin + b0 + b) / a.blocks_ff, block = (b_begin + b0 + b) - u * a.blocks_ff;
-            if (col >= picks.count[u]) continue;
-            const int t = picks.token[u][col];
+        int v_u = u0;
+        for (int i = warp; i * C + rank < units; i += kWarps) {
+            const int unit = src.unit0 + i * C + rank;
+            while (v_u + 1 < picks.n && unit >= picks.unit(v_u + 1, 0, a.blocks_ff)) ++v_u;
+            const int n = picks.count[v_u], at = unit - picks.unit(v_u, 0, a.blocks_ff), b = at / n, col = at - b * n;
+            const int t = picks.token[v_u][col];
             const float v = inbox.sum(src.round, i, 0) * picks.rstd[t], up = inbox.sum(src.round, i, 1) * picks.rstd[t];
-            put_hidden(a, picks, u, col, block, picks.weight[t * a.k + picks.rank[picks.unique[u]][t]] * (v / (1.f + expf(-v)) * up));
+            put_hidden(a, picks, v_u, col, b, picks.weight[t * a.k + picks.rank[picks.unique[v_u]][t]] * (v / (1.f + expf(-v)) * up));
         }
+        b0 += now;
     }
     if (blocks == 0) cluster_sync();        // nobody leaves while its logits are read
 }
@@ -1254,7 +1271,7 @@ template <bool MX, int MOST> struct DownStream {
         fetch_hidden();
         fetch_weights();
     }
-    template <int NT, class Put> __device__ __forceinline__ void work_run(Put put) {
+    template <int NT, class Column> __device__ __forceinline__ void work_run(Column column) {
         float acc[2][2][4] = {};
         Lane l;
         const Group g{{hidden, nullptr}, nullptr, NT};
@@ -1269,15 +1286,17 @@ template <bool MX, int MOST> struct DownStream {
             at = at == (kStages - 1) * kUnit ? 0 : at + kUnit;
             h_at ^= kHidden;
         }
-        end_run<PACK, NT, true>(NT, lane, l, acc, put);
+        float * to = nullptr;
+        end_run<PACK, NT, true>(NT, lane, l, acc, [&](int col) { to = column(col) + (lane >> 2); }, [&](int row, float v) { to[row] += v; });
     }
-    template <class Put> __device__ __forceinline__ void work(Put put) {
+    // slot(job, token): where 32 rows' sums are added up
+    template <class Slot> __device__ __forceinline__ void work(Slot slot) {
         while (c.live) {
             const int n = meta.count[c.set];
-            auto to_slot = [&](int row, int col, float v) { put(c.job, meta.token[c.set][col], row, v); };
-            if (n == 1) work_run<1>(to_slot);
-            if constexpr (MOST > 1) if (n == 2) work_run<2>(to_slot);
-            if constexpr (MOST > 2) if (n == 3) work_run<3>(to_slot);
+            auto column = [&](int col) { return slot(c.job, meta.token[c.set][col]); };
+            if (n == 1) work_run<1>(column);
+            if constexpr (MOST > 1) if (n == 2) work_run<2>(column);
+            if constexpr (MOST > 2) if (n == 3) work_run<3>(column);
             next(c);
             if (c.live) c.left = left(c);
         }
@@ -1324,13 +1343,13 @@ __global__ void __launch_bounds__(256, MOST > 1 ? 2 : 3) w4_moe_down_kernel(MoeA
         stream.prefetch();
         for (int i = threadIdx.x; i < jobs * ks * a.T * kSlotCol; i += kWarps * 32) partial[i] = 0.f;
         __syncthreads();
-        stream.work([&](int job, int token, int row, float v) { partial[((job * ks + sub) * a.T + token) * kSlotCol + row] += v; });
+        stream.work([&](int job, int token) { return partial + ((job * ks + sub) * a.T + token) * kSlotCol; });
         __syncthreads();
         for (int unit = warp; unit < jobs * a.T; unit += kWarps) {
             const int job = unit / a.T, t = unit - job * a.T;
             float v = 0.f;
             for (int i = 0; i < ks; ++i) v += partial[((job * ks + i) * a.T + t) * kSlotCol + lane];
-            inbox.put(round, unit, 0, 0, lane, v);
+            remote_store(inbox.slot(round, unit, 0, 0) + lane * 4, v);
         }
         cluster_sync();
         for (int i = warp; i * C + rank < jobs * a.T; i += kWarps) {
@@ -1547,10 +1566,10 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int mos
         const int busy = (c.clusters * C + sms - 1) / sms;
         const int ks = split_columns(blocks_each * per, steps / C, warps, warps);
         const int runs = (blocks_each * per * ks + warps - 1) / warps;           // of the busiest warp
-        const double unit_clocks = std::max(98.0, (n > 8 ? 300.0 : n > 4 ? 220.0 : 200.0) / 2.4);
-        const double in_flight = (double)busy * warps * (kStages - 1) * unit;
-        const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms), (double)busy * runs * warps * ((s + ks - 1) / ks) * unit_clocks,
-                                        (double)busy * blocks_each * per * s * unit / (in_flight / 1800.0)});
+        const double unit_clocks = n > 8 ? 170 : n > 4 ? 130 : 98;
+        const double in_flight = (double)c.clusters * C * warps * (kStages - 1) * unit;
+        const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms) * std::max(1.0, 13e6 / in_flight),
+                                        (double)busy * runs * warps * ((s + ks - 1) / ks + (n > 8 ? 0.6 : 0.3)) * unit_clocks});
         const double convert = busy * s * (n * 128 * 0.1 + step_clocks) + 800, sums = busy * (double)blocks_each * per * n * (6 + 2 * C * ks);
         const int64_t room = std::min(kSmShare / c.resident - 4096, kMaxSmem) - fixed - ring - (int64_t)s * each;
         const double rounds = std::ceil((double)inbox_bytes((int64_t)blocks_each * n, C, ks, per) / std::max<int64_t>(room, 1024));
@@ -1656,7 +1675,7 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         for (;; n = (n + 1) / 2) {
             const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n))));
             cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), mx, product_room(n, parts) > 4 ? 1 : 2,
-                             2 * up_to(n * E * 4, 128) + kStatic, n * E * 1.2 + E * 16.0, sms);
+                             2 * up_to(n * E * 4, 128) + kStatic, n * E * 0.4 + E * 4.0, sms);
             if (cut.C || n == 1) break;
         }
         if (!cut.C) return cudaErrorInvalidValue;
@@ -1705,7 +1724,7 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         if (e != cudaSuccess) return e;
 
         // second kernel
-        int C = kMaxCluster;
+        int C = 4;                      // eight would leave a warp two units of a run at one token
         while (C > steps_ff * p.n_used) C /= 2;
         const int resident = n > 1 ? 2 : 3;
         const int most = resident_clusters(log2_of(C), resident, 256), per = (a.blocks_d + most - 1) / most;
