@@ -1551,10 +1551,10 @@ struct Cut {
 // shared memory a step. The estimate is in clocks: the weight stream at the SM's share of the memory bandwidth, but no faster
 // than the busiest SM's warps get through it or than its copies in flight allow; the conversion of the CTA's share of the activations; the sums it
 // receives; and a barrier for every round its inbox allows. `step_clocks` is what else a column step costs a CTA.
-Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int most_resident, int fixed, double step_clocks, int sms) {
+Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int most_resident, int most_c, int fixed, double step_clocks, int sms) {
     Cut best;
     const int warps = warps_for(n), ring = ring_bytes(mx, warps), unit = (int)w4_unit_bytes(mx);
-    for (int C = 1; C <= kMaxCluster && C <= steps; C *= 2) {
+    for (int C = 1; C <= most_c && C <= steps; C *= 2) {
         const int s = (steps + C - 1) / C;
         const int64_t smem = (int64_t)s * each + ring + fixed + 2 * inbox_bytes(n, C, 1, per) + 4096;
         if (smem > kMaxSmem) continue;
@@ -1566,9 +1566,9 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int mos
         const int busy = (c.clusters * C + sms - 1) / sms;
         const int ks = split_columns(blocks_each * per, steps / C, warps, warps);
         const int runs = (blocks_each * per * ks + warps - 1) / warps;           // of the busiest warp
-        const double unit_clocks = n > 8 ? 170 : n > 4 ? 130 : 98;
+        const double unit_clocks = n > 8 ? 150 : n > 4 ? 120 : 80;
         const double in_flight = (double)c.clusters * C * warps * (kStages - 1) * unit;
-        const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms) * std::max(1.0, 13e6 / in_flight),
+        const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms) * std::max(1.0, 13e6 / in_flight),     // two microseconds of latency under load
                                         (double)busy * runs * warps * ((s + ks - 1) / ks + (n > 8 ? 0.6 : 0.3)) * unit_clocks});
         const double convert = busy * s * (n * 128 * 0.1 + step_clocks) + 800, sums = busy * (double)blocks_each * per * n * (6 + 2 * C * ks);
         const int64_t room = std::min(kSmShare / c.resident - 4096, kMaxSmem) - fixed - ring - (int64_t)s * each;
@@ -1614,7 +1614,7 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
         Cut cut;
         for (;; n = (n + 1) / 2) {
-            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), mx, resident_for(product_room(n, parts)), 0, 0, device_sms());
+            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), mx, resident_for(product_room(n, parts)), kMaxCluster, 0, 0, device_sms());
             if (cut.C || n == 1) break;
         }
         if (!cut.C) return cudaErrorInvalidValue;       // rows this long are refused when the handle is made
@@ -1670,11 +1670,12 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
     constexpr int kStatic = 16 * 1024;          // the routing tables
     for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
-        // first kernel: n tokens that choose independently choose about `reach` experts
+        // first kernel: n tokens that choose independently choose about `reach` experts. Up to four tokens it runs in clusters of at most four
+        // (one token, 32 experts of 2880 x 2880: 33 us the layer, 39 us with eight), unless rows are so long that four cannot hold them.
         Cut cut;
         for (;; n = (n + 1) / 2) {
             const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n))));
-            cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), mx, product_room(n, parts) > 4 ? 1 : 2,
+            cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), mx, product_room(n, parts) > 4 ? 1 : 2, n > 4 || steps_d > 256 ? kMaxCluster : 4,
                              2 * up_to(n * E * 4, 128) + kStatic, n * E * 0.4 + E * 4.0, sms);
             if (cut.C || n == 1) break;
         }
