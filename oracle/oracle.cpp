@@ -122,13 +122,14 @@ void scale_min_k4(int j, const uint8_t * q, uint8_t & sc, uint8_t & m) {
     }
 }
 
-enum : uint32_t { T_F32 = 0, T_F16 = 1, T_Q8_0 = 8, T_Q4_K = 12, T_BF16 = 30, T_MXFP4 = 39 };
+enum : uint32_t { T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q8_0 = 8, T_Q4_K = 12, T_BF16 = 30, T_MXFP4 = 39 };
 
 bool geom(uint32_t type, size_t & elems, size_t & bytes) {
     switch (type) {
         case T_F32: elems = 1; bytes = 4; return true;
         case T_F16: elems = 1; bytes = 2; return true;
         case T_BF16: elems = 1; bytes = 2; return true;
+        case T_Q4_0: elems = 32; bytes = 18; return true;
         case T_Q8_0: elems = 32; bytes = 34; return true;
         case T_Q4_K: elems = 256; bytes = 144; return true;
         case T_MXFP4: elems = 32; bytes = 17; return true;
@@ -158,6 +159,18 @@ bool dequantize_row(uint32_t type, const uint8_t * src, size_t n, float * y) {
                 std::memcpy(&h, src + 2 * i, 2);
                 uint32_t bits = (uint32_t)h << 16;
                 std::memcpy(&y[i], &bits, 4);
+            }
+            return true;
+        case T_Q4_0:
+            for (size_t b = 0; b < nb; ++b) {
+                const uint8_t * p = src + b * 18;
+                uint16_t h;
+                std::memcpy(&h, p, 2);
+                const float scale = half_to_f32(h);
+                for (int j = 0; j < 16; ++j) {
+                    y[b * 32 + j] = scale * (float)((int)(p[2 + j] & 0x0F) - 8);
+                    y[b * 32 + j + 16] = scale * (float)((int)(p[2 + j] >> 4) - 8);
+                }
             }
             return true;
         case T_Q8_0:

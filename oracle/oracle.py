@@ -14,7 +14,7 @@ HERE = Path(__file__).resolve().parent
 LIB = HERE / "liboracle.so"
 MODELGEN = HERE / "libmodelgen.so"
 
-T_F32, T_F16, T_Q8_0, T_Q4_K, T_BF16, T_MXFP4 = 0, 1, 8, 12, 30, 39
+T_F32, T_F16, T_Q4_0, T_Q8_0, T_Q4_K, T_BF16, T_MXFP4 = 0, 1, 2, 8, 12, 30, 39
 
 
 def build(force: bool = False) -> Path:

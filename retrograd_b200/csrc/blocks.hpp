@@ -3,6 +3,7 @@
 // Block geometry follows the reference's in-tree format table
 // (crates/rir-core/src/quant_table.rs:322-360,420-440; decoders in
 // crates/rir-core/src/quant.rs:223-417):
+//   Q4_0   32 elements / 18 B : f16 d | 16 B nibbles (element i low, 16 + i high; value d (q - 8))
 //   Q8_0   32 elements / 34 B : f16 d | 32 x i8
 //   Q4_K  256 elements / 144 B: f16 d | f16 dmin | 12 B packed 6-bit scales+mins | 128 B nibbles
 //   MXFP4  32 elements / 17 B : E8M0 exponent byte | 16 B nibbles (doubled E2M1 table)
@@ -35,6 +36,7 @@ inline bool block_geom(uint32_t type, BlockGeom & out) {
         case GGML_F32:   out = {1, 4};     return true;
         case GGML_F16:   out = {1, 2};     return true;
         case GGML_BF16:  out = {1, 2};     return true;
+        case GGML_Q4_0:  out = {32, 18};   return true;
         case GGML_Q8_0:  out = {32, 34};   return true;
         case GGML_Q4_K:  out = {256, 144}; return true;
         case GGML_MXFP4: out = {32, 17};   return true;
@@ -47,6 +49,7 @@ inline const char * type_name(uint32_t type) {
         case GGML_F32: return "f32";
         case GGML_F16: return "f16";
         case GGML_BF16: return "bf16";
+        case GGML_Q4_0: return "q4_0";
         case GGML_Q8_0: return "q8_0";
         case GGML_Q4_K: return "q4_K";
         case GGML_MXFP4: return "mxfp4";

@@ -72,8 +72,29 @@ bool mxfp4_to_q8_0(const void * src, size_t bytes, std::vector<uint8_t> & out) {
     return true;
 }
 
+// Q4_0 blocks (f16 d + 16 bytes of nibbles) -> Q8_0 blocks of the same values: the same d, the int8 is q - 8.
+void q4_0_to_q8_0(const void * src, size_t bytes, std::vector<uint8_t> & out) {
+    const size_t n_blocks = bytes / 18;
+    const uint8_t * in = static_cast<const uint8_t *>(src);
+    out.resize(n_blocks * 34);
+#pragma omp parallel for
+    for (long long b = 0; b < (long long)n_blocks; ++b) {
+        const uint8_t * blk = in + b * 18;
+        uint8_t * dst = out.data() + b * 34;
+        dst[0] = blk[0];
+        dst[1] = blk[1];
+        for (int i = 0; i < 16; ++i) {
+            dst[2 + i] = (uint8_t)(int8_t)((int)(blk[2 + i] & 0xF) - 8);
+            dst[2 + 16 + i] = (uint8_t)(int8_t)((int)(blk[2 + i] >> 4) - 8);
+        }
+    }
+}
+
 void Engine::load_model(const std::string & path) {
-    if (const char * env = std::getenv("RB200_MOE")) moe_tensor_cores_ = std::string(env) != "rows";
+    if (const char * env = std::getenv("RB200_MOE")) {
+        moe_tensor_cores_ = std::string(env) != "rows";
+        moe_few_ = std::string(env) == "few";
+    }
     if (const char * env = std::getenv("RB200_LORA")) lora_tensor_cores_ = std::string(env) != "rows";
     if (const char * env = std::getenv("RB200_Q8_TC5")) q8_tc5_ = std::string(env) != "0";
     GgufFile file(path);
@@ -109,10 +130,66 @@ void Engine::load_model(const std::string & path) {
         m.weight_bytes += bytes;
         return static_cast<uint8_t *>(p);
     };
-    auto need = [&](const std::string & name) -> const GgufTensor & {
+    auto stored = [&](const std::string & name) -> const GgufTensor & {
         const GgufTensor * t = file.find(name);
         if (!t) throw std::runtime_error("failed to load model GGUF: missing tensor " + name);
         return *t;
+    };
+    // A tensor as the kernels of longer steps read it: Q4_0 as the Q8_0 blocks of the same values. The re-coded bytes
+    // are kept until the layer they belong to is uploaded.
+    struct Recoded {
+        GgufTensor tensor;
+        std::vector<uint8_t> bytes;
+    };
+    std::map<std::string, Recoded> recoded_q4_0;
+    auto need = [&](const std::string & name) -> const GgufTensor & {
+        const GgufTensor & t = stored(name);
+        if (t.type != GGML_Q4_0) return t;
+        Recoded & r = recoded_q4_0[name];
+        if (r.bytes.empty()) {
+            q4_0_to_q8_0(t.data, t.n_bytes, r.bytes);
+            r.tensor = t;
+            r.tensor.type = GGML_Q8_0;
+            r.tensor.data = r.bytes.data();
+            r.tensor.n_bytes = r.bytes.size();
+        }
+        return r.tensor;
+    };
+    // The stored rows of matrices of one 4-bit type and row length, one behind the other, as units of the few-token products.
+    auto attach_w4 = [&](WeightView & w, const std::vector<std::string> & names, uint64_t n_in, uint64_t n_out, uint32_t n_expert) {
+        const uint32_t type = stored(names[0]).type;
+        for (const std::string & name : names)
+            if (stored(name).type != type) return;
+        if ((type != GGML_Q4_0 && type != GGML_MXFP4) || n_in > kW4MaxColumns || n_expert > kW4MaxExperts) return;
+        size_t total = 0;
+        for (const std::string & name : names) total += stored(name).n_bytes;
+        struct Raw { uint8_t * p = nullptr; ~Raw() { if (p) cudaFree(p); } } raw;
+        RB_CUDA(cudaMalloc(&raw.p, align_up(total, 16) + 16));
+        size_t at = 0;
+        for (const std::string & name : names) {
+            const GgufTensor & t = stored(name);
+            RB_CUDA(cudaMemcpy(raw.p + at, t.data, t.n_bytes, cudaMemcpyHostToDevice));
+            at += t.n_bytes;
+        }
+        int * d_max = reinterpret_cast<int *>(raw.p + align_up(total, 16));
+        RB_CUDA(cudaMemset(d_max, 0, sizeof(int)));
+        void * units = nullptr;
+        const size_t bytes = w4_bytes(type, (uint32_t)n_out, (uint32_t)n_in, n_expert);
+        RB_CUDA(cudaMalloc(&units, bytes));
+        m.allocations.push_back(units);
+        RB_CUDA(cudaDeviceSynchronize());       // the blocking uploads have reached the device
+        launch_w4_retile(raw.p, type, (uint32_t)n_out, (uint32_t)n_in, n_expert, static_cast<uint8_t *>(units), d_max, stream);
+        int h_max = 0;
+        RB_CUDA(cudaMemcpyAsync(&h_max, d_max, sizeof h_max, cudaMemcpyDeviceToHost, stream));
+        RB_CUDA(cudaStreamSynchronize(stream));
+        if (h_max > (int)kW4MaxScaleByte) {     // beyond what these kernels hold: the other kernels serve every step
+            m.allocations.pop_back();
+            RB_CUDA(cudaFree(units));
+            return;
+        }
+        w.w4 = static_cast<const uint8_t *>(units);
+        w.w4_type = type;
+        m.tiled_bytes += bytes;
     };
     // the host-side check the matrix' tcgen05 kernel asks for (see WeightView::tc5_exact)
     auto tc5_check = [&](const GgufTensor & t, uint64_t n_in) {
@@ -128,12 +205,13 @@ void Engine::load_model(const std::string & path) {
         w.n_in = (uint32_t)t.ne[0];
         w.n_out = (uint32_t)rows;
         w.row_bytes = (uint32_t)row_bytes(t.type, t.ne[0]);
-        const bool wants_tiled = t.ne.size() == 2 && w.n_in % 256 == 0 &&
+        // (Q4_0 matrices have the few-token units instead of a copy for the streaming kernel)
+        const bool wants_tiled = t.ne.size() == 2 && w.n_in % 256 == 0 && stored(t.name).type != GGML_Q4_0 &&
                                  ((t.type == GGML_Q4_K && rows >= 128) || (t.type == GGML_Q8_0 && rows >= 16));
         // A blocking copy from pageable host memory may return while its last piece is still on its way
         // to the device; the regrouping kernels run on another stream, so wait for the device first.
         if (wants_tiled) RB_CUDA(cudaDeviceSynchronize());
-        if (t.type == GGML_Q4_K && t.ne.size() == 2 && w.n_in % 256 == 0 && rows >= 128) {
+        if (wants_tiled && t.type == GGML_Q4_K) {
             // second copy regrouped for the tcgen05 kernel's coalesced weight stream
             void * tiled = nullptr;
             const size_t bytes = q4k_tiled_bytes(w.n_out, w.n_in);
@@ -142,7 +220,7 @@ void Engine::load_model(const std::string & path) {
             launch_q4k_retile(dev, w.n_out, w.n_in, w.row_bytes, static_cast<uint8_t *>(tiled), stream);
             w.tiled = static_cast<const uint8_t *>(tiled);
             m.tiled_bytes += bytes;
-        } else if (t.type == GGML_Q8_0 && t.ne.size() == 2 && w.n_in % 256 == 0 && rows >= 16) {
+        } else if (wants_tiled) {
             // second copy in MMA fragment order for the decode streaming kernel
             void * tiled = nullptr;
             const size_t bytes = q8_0_tiled_bytes(w.n_out, w.n_in);
@@ -158,7 +236,9 @@ void Engine::load_model(const std::string & path) {
         const GgufTensor & t = need(name);
         if (t.ne.size() != 2 || t.ne[0] != n_in || t.ne[1] != n_out) throw std::runtime_error("failed to load model GGUF: unexpected shape of " + name);
         if (n_in % 8 != 0) throw std::runtime_error("failed to load model GGUF: row length of " + name + " is not a multiple of 8");
-        return view_of(t, upload(t.data, t.n_bytes), n_out, tc5_check(t, n_in));
+        WeightView w = view_of(t, upload(t.data, t.n_bytes), n_out, tc5_check(t, n_in));
+        if (stored(name).type == GGML_Q4_0) attach_w4(w, {name}, n_in, n_out, 1);
+        return w;
     };
     auto vector_f32 = [&](const std::string & name, uint64_t n, bool optional) -> const float * {
         const GgufTensor * t = file.find(name);
@@ -172,6 +252,8 @@ void Engine::load_model(const std::string & path) {
     // Several matrices with one row length and storage type, stacked row-wise into one allocation.
     auto fused = [&](const std::vector<std::string> & names, uint64_t n_in, const std::vector<uint64_t> & n_out, WeightView & out) -> bool {
         uint32_t type = need(names[0]).type;
+        for (const std::string & name : names)
+            if (stored(name).type != stored(names[0]).type) return false;
         size_t total = 0;
         for (size_t i = 0; i < names.size(); ++i) {
             const GgufTensor & t = need(names[i]);
@@ -194,6 +276,7 @@ void Engine::load_model(const std::string & path) {
         }
         m.weight_bytes += total;
         out = view_of(need(names[0]), static_cast<uint8_t *>(p), rows, tc5_exact);
+        if (stored(names[0]).type == GGML_Q4_0) attach_w4(out, names, n_in, rows, 1);
         return true;
     };
 
@@ -201,6 +284,8 @@ void Engine::load_model(const std::string & path) {
     hp.vocab = (uint32_t)embd.ne[1];
     if (embd.ne[0] != hp.d) throw std::runtime_error("failed to load model GGUF: token_embd width differs from embedding_length");
     m.token_embd = view_of(embd, upload(embd.data, embd.n_bytes), hp.vocab, tc5_check(embd, hp.d));
+    if (stored("token_embd.weight").type == GGML_Q4_0 && !file.find("output.weight")) attach_w4(m.token_embd, {"token_embd.weight"}, hp.d, hp.vocab, 1);
+    recoded_q4_0.clear();
 
     const uint64_t dq = hp.dq(), dkv = hp.dkv();
     m.layers.resize(hp.n_layer);
@@ -291,12 +376,19 @@ void Engine::load_model(const std::string & path) {
             bank(p + "ffn_gate_exps.weight", hp.d, hp.ff, lw.gate_exps, lw.gate_stride);
             bank(p + "ffn_up_exps.weight", hp.d, hp.ff, lw.up_exps, lw.up_stride);
             bank(p + "ffn_down_exps.weight", hp.ff, hp.d, lw.down_exps, lw.down_stride);
+            const uint32_t bank_type = stored(p + "ffn_gate_exps.weight").type;
+            if ((bank_type == GGML_Q4_0 || (bank_type == GGML_MXFP4 && moe_few_)) && hp.n_expert_used <= kW4MaxUsed &&
+                stored(p + "ffn_up_exps.weight").type == bank_type) {
+                attach_w4(lw.gate_exps, {p + "ffn_gate_exps.weight"}, hp.d, hp.ff, hp.n_expert);
+                attach_w4(lw.up_exps, {p + "ffn_up_exps.weight"}, hp.d, hp.ff, hp.n_expert);
+                attach_w4(lw.down_exps, {p + "ffn_down_exps.weight"}, hp.ff, hp.d, hp.n_expert);
+            }
             // the inventory entry of each bank, as the file holds it (retro_experts.cpp:86-131: role = the
             // name's stem without "ffn_" and "_exps")
             const char * roles[3] = {"gate", "up", "down"};
             const WeightView * views[3] = {&lw.gate_exps, &lw.up_exps, &lw.down_exps};
             for (int b = 0; b < 3; ++b) {
-                const GgufTensor & t = need(p + "ffn_" + roles[b] + "_exps.weight");
+                const GgufTensor & t = stored(p + "ffn_" + roles[b] + "_exps.weight");
                 retro_expert_bank_desc desc{};
                 desc.layer = l;
                 std::snprintf(desc.role, sizeof desc.role, "%s", roles[b]);
@@ -308,12 +400,13 @@ void Engine::load_model(const std::string & path) {
                 }
                 desc.tensor.n_bytes = t.n_bytes;
                 desc.tensor.storage_id = reinterpret_cast<uint64_t>(views[b]->data);
-                const char * type = t.type == GGML_F32 ? "F32" : t.type == GGML_F16 ? "F16" : t.type == GGML_BF16 ? "BF16" : t.type == GGML_Q8_0 ? "Q8_0"
+                const char * type = t.type == GGML_F32 ? "F32" : t.type == GGML_F16 ? "F16" : t.type == GGML_BF16 ? "BF16" : t.type == GGML_Q8_0 ? "Q8_0" : t.type == GGML_Q4_0 ? "Q4_0"
                                     : t.type == GGML_Q4_K ? "Q4_K" : t.type == GGML_MXFP4 ? "MXFP4" : "unknown";
                 std::snprintf(desc.tensor.type_name, sizeof desc.tensor.type_name, "%s", type);
                 m.expert_banks.push_back(desc);
             }
         }
+        recoded_q4_0.clear();
     }
     m.output_norm = vector_f32("output_norm.weight", hp.d, false);
     if (file.find("output.weight")) {
@@ -491,6 +584,7 @@ Engine::Engine(const std::string & path, const retro_engine_config & cfg) : conf
         moe_offsets_.ensure(hp.n_expert + 1);
         moe_sorted_.ensure(P);
         moe_w_.ensure(P);
+        w4_workspace_.ensure(w4_moe_workspace_bytes(hp.ff, kW4PassTokens, hp.n_expert_used));
         pair_gu_.ensure(P * 2 * hp.ff);
         pair_h_.ensure(P * hp.ff);
         pair_y_.ensure(P * hp.d);
@@ -564,6 +658,10 @@ bool Engine::tc5_split_preferred(const WeightView & w, int T, const SplitAct * x
 // Returns whether `tail` (the row-wise step that consumes y) was done by the GEMM's own finish kernel.
 bool Engine::linear(const WeightView & w, const float * x, int ldx, int T, float * y, int ldy, const float * bias, const float * residual,
                     int ldr, const SplitAct * xs, const FinishTail * tail) {
+    if (w4_serves(w, T)) {
+        linear_w4(w, x, ldx, T, y, ldy, bias, residual, ldr);
+        return false;
+    }
     bool tail_done = false;
     prof_.begin(K_GEMM, stream);
     if (xs && stream_gemm_ && T <= kStreamMaxTokens && !tc5_split_preferred(w, T, xs) &&
@@ -631,6 +729,84 @@ bool Engine::linear(const WeightView & w, const float * x, int ldx, int T, float
     prof_.end(K_GEMM, 1, stream);
     ++last_launches;
     return tail_done;
+}
+
+namespace {
+
+void w4_launched(cudaError_t status) {
+    if (status != cudaSuccess) throw CudaError(std::string("a few-token product failed to launch: ") + cudaGetErrorString(status));
+}
+
+W4Product w4_rows(const float * x, int ldx, int T, float * y, int ldy) {
+    W4Product p;
+    p.x = x;
+    p.x_type = GGML_F32;
+    p.ld_x = ldx;
+    p.n_tokens = T;
+    p.y = y;
+    p.y_type = GGML_F32;
+    p.ld_y = ldy;
+    return p;
+}
+
+} // namespace
+
+// y = W x (+ bias, residual) of a matrix with few-token units; with `norm`, x is normalised by these weights first.
+void Engine::linear_w4(const WeightView & w, const float * x, int ldx, int T, float * y, int ldy, const float * bias, const float * residual, int ldr,
+                       const float * norm) {
+    W4Product p = w4_rows(x, ldx, T, y, ldy);
+    p.w = w4_view(w.w4, w.w4_type, w.n_out, w.n_in, 1);
+    p.norm = norm;
+    p.eps = model->hp.eps;
+    p.bias = bias;
+    p.residual = residual;
+    p.ld_residual = ldr;
+    prof_.begin(K_GEMM, stream);
+    w4_launched(launch_w4_product(p, stream));
+    prof_.end(K_GEMM, 1, stream);
+    ++last_launches;
+}
+
+// The gated pair of a stacked [gate | up] matrix whose halves are whole row blocks.
+void Engine::glu_w4(const WeightView & gate_up, const float * x, int ldx, int T, float * y, int ldy, const float * norm) {
+    const uint32_t ff = gate_up.n_out / 2;
+    W4Product p = w4_rows(x, ldx, T, y, ldy);
+    p.w = w4_view(gate_up.w4, gate_up.w4_type, ff, gate_up.n_in, 1);
+    const W4View up = w4_view(gate_up.w4 + p.w.expert_bytes, gate_up.w4_type, ff, gate_up.n_in, 1);
+    p.up = &up;
+    p.norm = norm;
+    p.eps = model->hp.eps;
+    prof_.begin(K_GEMM, stream);
+    w4_launched(launch_w4_product(p, stream));
+    prof_.end(K_GEMM, 1, stream);
+    ++last_launches;
+}
+
+// x_ += the expert layer of x (x_ itself, normalised by `norm`, or normalised rows); the routing goes to moe_ids_ and moe_w_.
+void Engine::moe_w4(const LayerWeights & lw, const float * x, int T, const float * norm) {
+    const HParams & hp = model->hp;
+    auto bank = [&](const WeightView & w) { return w4_view(w.w4, w.w4_type, w.n_out, w.n_in, hp.n_expert); };
+    W4Moe p;
+    p.gate = bank(lw.gate_exps);
+    p.up = bank(lw.up_exps);
+    p.down = bank(lw.down_exps);
+    p.router = reinterpret_cast<const float *>(lw.router.data);
+    p.x = x;
+    p.x_type = p.y_type = GGML_F32;
+    p.ld_x = p.ld_y = p.ld_residual = hp.d;
+    p.n_tokens = T;
+    p.n_used = (int)hp.n_expert_used;
+    p.norm = norm;
+    p.eps = hp.eps;
+    p.residual = x_.ptr;
+    p.y = x_.ptr;
+    p.ids = moe_ids_.ptr;
+    p.weights = moe_w_.ptr;
+    p.workspace = w4_workspace_.ptr;
+    prof_.begin(K_MOE, stream);
+    w4_launched(launch_w4_moe(p, stream));
+    prof_.end(K_MOE, 2, stream);
+    last_launches += 2;
 }
 
 // Runs one step's device work: eagerly, or as a replayed / freshly captured CUDA graph.
@@ -705,7 +881,7 @@ void Engine::run_step_work(const std::vector<uint64_t> & sig, const std::functio
 // Whether linear() will read the split form of the activations for this weight and token count
 // (then the f32 copy of the activations need not be written at all).
 bool Engine::linear_reads_split(const WeightView & w, int ldx, int T, const SplitAct * xs) const {
-    if (!xs) return false;
+    if (!xs || w4_serves(w, T)) return false;
     if (stream_gemm_ && T <= kStreamMaxTokens &&
         (gemm_q4k_stream_supported(w, *xs, std::min(T, 8)) || gemm_q8_0_stream_supported(w, *xs, std::min(T, 8))))
         return true;
@@ -866,6 +1042,13 @@ void Engine::ep_keep_local_experts() {
         ep_local_bank_bytes_ += per * per_expert;
     };
     for (LayerWeights & lw : m.layers) {
+        for (WeightView * w : {&lw.gate_exps, &lw.up_exps, &lw.down_exps}) {        // the exchanged pairs run on the other kernels
+            if (!w->w4) continue;
+            m.tiled_bytes -= w4_bytes(w->w4_type, w->n_out, w->n_in, m.hp.n_expert);
+            m.allocations.erase(std::find(m.allocations.begin(), m.allocations.end(), (void *)w->w4));
+            RB_CUDA(cudaFree(const_cast<uint8_t *>(w->w4)));
+            w->w4 = nullptr;
+        }
         keep(lw.gate_exps, lw.gate_stride);
         keep(lw.up_exps, lw.up_stride);
         keep(lw.down_exps, lw.down_stride);
@@ -1454,13 +1637,17 @@ int Engine::step(const EffRow * rows, size_t n_rows, OutRow * out_rows, int32_t 
         const std::string p = "blk." + std::to_string(l) + ".";
         // the f32 copy of an activation is written only when something other than a split-reading GEMM consumes it
         const bool qkv_split = !any_adapter && lw.wqkv.data && linear_reads_split(lw.wqkv, d, Ti, xn_split_.get());
-        if (!norm_done)
+        // matrices with few-token units normalise their input themselves
+        const bool qkv_norms = !norm_done && !any_adapter && lw.wqkv.data && w4_serves(lw.wqkv, Ti);
+        if (!norm_done && !qkv_norms)
             RB_K(K_OTHER, 1, launch_rms_norm(x_.ptr, d, nullptr, lw.attn_norm, d, hp.eps, qkv_split ? nullptr : xn_.ptr, d, Ti, stream, xn_split_.get()));
         norm_done = false;
         const RopeStoreArgs rope_args{(int)hp.n_head, (int)hp.n_head_kv, (int)hp.head_dim, (int)hp.n_rot, hp.neox, model->inv_freq.ptr,
                                       maps.tok_pos,   maps.tok_cell,     kvl,              (int)l};
         bool roped = false;
-        if (lw.wqkv.data) {
+        if (qkv_norms) {
+            linear_w4(lw.wqkv, x_.ptr, d, Ti, qkv_.ptr, ldqkv, lw.bqkv, nullptr, 0, lw.attn_norm);
+        } else if (lw.wqkv.data) {
             // RoPE and the KV store by the projection's finish kernel when nothing else touches q, k, v in between
             FinishTail rope_tail;
             rope_tail.kind = 3;
@@ -1534,12 +1721,19 @@ int Engine::step(const EffRow * rows, size_t n_rows, OutRow * out_rows, int32_t 
         if (xn_split_.get()) ffn_norm_tail.split = *xn_split_.get();
         const bool ffn_normed = linear(lw.wo, att_.ptr, dq, Ti, x_.ptr, d, nullptr, x_.ptr, d, att_split_.get(), any_adapter ? nullptr : &ffn_norm_tail);
         if (any_adapter) lora(p + "attn_output.weight", att_.ptr, dq, Ti, x_.ptr, d);
-        if (!ffn_normed)
+        const bool ffn_glu = !any_adapter && hp.n_expert == 0 && lw.wgu.data && w4_serves(lw.wgu, Ti) && ff % 32 == 0;
+        const bool experts_w4 = hp.n_expert != 0 && !ep_comm_ && w4_serves(lw.gate_exps, Ti) && lw.up_exps.w4 && lw.down_exps.w4;
+        if (!ffn_normed && !ffn_glu && !experts_w4)
             RB_K(K_OTHER, 1, launch_rms_norm(x_.ptr, d, nullptr, lw.ffn_norm, d, hp.eps, gu_split ? nullptr : xn_.ptr, d, Ti, stream, xn_split_.get()));
         if (hp.n_expert == 0) {
             const bool down_split = !any_adapter && linear_reads_split(lw.wdown, ff, Ti, hff_split_.get());
             bool activated = false;
-            if (lw.wgu.data) {
+            if (ffn_glu) {
+                glu_w4(lw.wgu, ffn_normed ? xn_.ptr : x_.ptr, d, Ti, hff_.ptr, ff, ffn_normed ? nullptr : lw.ffn_norm);
+                if (hff_split_.get() && linear_reads_split(lw.wdown, ff, Ti, hff_split_.get()))
+                    RB_K(K_OTHER, 1, launch_split_prep(hff_.ptr, ff, ff, Ti, hff_split_.view, stream));
+                activated = true;
+            } else if (lw.wgu.data) {
                 FinishTail act_tail;
                 act_tail.kind = 2;
                 act_tail.out = down_split ? nullptr : hff_.ptr;
@@ -1571,6 +1765,11 @@ int Engine::step(const EffRow * rows, size_t n_rows, OutRow * out_rows, int32_t 
             if (any_adapter) lora(p + "ffn_down.weight", hff_.ptr, ff, Ti, x_.ptr, d);
         } else {
             const int E = (int)hp.n_expert, K = (int)hp.n_expert_used, P = Ti * K;
+            if (experts_w4) {
+                moe_w4(lw, ffn_normed ? xn_.ptr : x_.ptr, Ti, ffn_normed ? nullptr : lw.ffn_norm);
+                RB_CUDA(cudaMemcpyAsync(route_ids.ptr + (size_t)l * P, moe_ids_.ptr, (size_t)P * 4, cudaMemcpyDeviceToDevice, stream));
+                continue;
+            }
             linear(lw.router, xn_.ptr, d, Ti, router_logits_.ptr, E, nullptr, nullptr, 0);
             RB_K(K_MOE, 1, launch_moe_route(router_logits_.ptr, E, K, Ti, moe_ids_.ptr, moe_w_.ptr, stream));
             RB_CUDA(cudaMemcpyAsync(route_ids.ptr + (size_t)l * P, moe_ids_.ptr, (size_t)P * 4, cudaMemcpyDeviceToDevice, stream));

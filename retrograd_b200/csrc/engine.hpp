@@ -8,6 +8,7 @@
 #include "common.hpp"
 #include "gguf.hpp"
 #include "kernels.cuh"
+#include "w4.cuh"
 #include "ep.hpp"
 #include "kv.hpp"
 #include "grammar.hpp"
@@ -132,6 +133,8 @@ struct SplitBuffer {
     const SplitAct * get() const { return view.hi ? &view : nullptr; }
 };
 
+// Q4_0 blocks re-coded as Q8_0 blocks of the same values (see engine.cu).
+void q4_0_to_q8_0(const void * src, size_t bytes, std::vector<uint8_t> & out);
 // MXFP4 blocks re-coded as Q8_0 blocks of the same values (see engine.cu); false when a block scale does not fit an f16.
 bool mxfp4_to_q8_0(const void * src, size_t bytes, std::vector<uint8_t> & out);
 
@@ -345,6 +348,11 @@ private:
   public:
     void graph_stats(uint64_t * replays, uint64_t * cached) const { if (replays) *replays = graph_replays_; if (cached) *cached = graphs_.size(); }
   private:
+    bool w4_serves(const WeightView & w, int T) const { return w.w4 && T <= kW4PassTokens; }
+    void linear_w4(const WeightView & w, const float * x, int ldx, int T, float * y, int ldy, const float * bias, const float * residual, int ldr,
+                   const float * norm = nullptr);
+    void glu_w4(const WeightView & gate_up, const float * x, int ldx, int T, float * y, int ldy, const float * norm);
+    void moe_w4(const LayerWeights & lw, const float * x, int T, const float * norm);
     bool linear_reads_split(const WeightView & w, int ldx, int T, const SplitAct * xs) const;
     void lora(const std::string & target, const float * x, int ldx, int T, float * y, int ldy);
     void lora_group(const std::vector<std::string> & targets, const std::vector<int> & y_offsets, const float * x, int ldx, int T, float * y, int ldy);
@@ -367,6 +375,7 @@ private:
     size_t result_bytes_ = 0;
     DeviceBuffer<float> x_, xn_, qkv_, att_, gu_, hff_, hs_, router_logits_, moe_w_, pair_gu_, pair_h_, pair_y_, lora_tmp_, logits_work_;
     DeviceBuffer<int32_t> moe_ids_, d_aux_;
+    DeviceBuffer<uint8_t> w4_workspace_;               // of the few-token expert layer
     DeviceBuffer<int32_t> moe_offsets_, moe_sorted_, lora_offsets_, lora_sorted_;
     DeviceBuffer<int> device_error_;
     DeviceBuffer<int> check_word_;      // bounds-checked build: {code, value, limit, count} of the first violation
@@ -377,6 +386,7 @@ private:
     int n_sm_ = 148;
     bool stream_gemm_ = true;
     bool moe_tensor_cores_ = true;      // RB200_MOE=rows: experts stay MXFP4 on the CUDA-core row kernel
+    bool moe_few_ = false;              // RB200_MOE=few: MXFP4 experts of steps of at most sixteen tokens on the few-token kernels
     bool q8_tc5_ = true;                // RB200_Q8_TC5=0: Q8_0 above 16 tokens stays on the mma.sync kernel
     bool lora_tensor_cores_ = true;     // RB200_LORA=rows: the CUDA-core shrink / expand kernels instead
     DeviceBuffer<float> moe_xs_, moe_gu_s_, moe_y_s_;      // expert-contiguous rows: inputs, [gate | up], outputs

@@ -52,6 +52,13 @@ __device__ __forceinline__ void decode8(const uint8_t * __restrict__ row, uint32
         const uint16_t * h = reinterpret_cast<const uint16_t *>(&raw);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = __uint_as_float((uint32_t)h[i] << 16);
+    } else if constexpr (TYPE == GGML_Q4_0) {
+        const uint8_t * b = row + (size_t)(k >> 5) * 18;
+        const uint32_t in = k & 31, hi = in >> 4, l = in & 15;
+        const float d = half_bits_to_float((uint16_t)(b[0] | (b[1] << 8)));
+        const uint8_t * q = b + 2 + l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = d * (float)((int)((q[i] >> (4 * hi)) & 0xF) - 8);
     } else if constexpr (TYPE == GGML_Q8_0) {
         const uint8_t * b = row + (size_t)(k >> 5) * 34;
         const float d = half_bits_to_float((uint16_t)(b[0] | (b[1] << 8)));
@@ -910,6 +917,7 @@ template <class F> void dispatch_type(uint32_t type, F && f) {
         case GGML_F32: f(std::integral_constant<uint32_t, GGML_F32>{}); break;
         case GGML_F16: f(std::integral_constant<uint32_t, GGML_F16>{}); break;
         case GGML_BF16: f(std::integral_constant<uint32_t, GGML_BF16>{}); break;
+        case GGML_Q4_0: f(std::integral_constant<uint32_t, GGML_Q4_0>{}); break;
         case GGML_Q8_0: f(std::integral_constant<uint32_t, GGML_Q8_0>{}); break;
         case GGML_Q4_K: f(std::integral_constant<uint32_t, GGML_Q4_K>{}); break;
         case GGML_MXFP4: f(std::integral_constant<uint32_t, GGML_MXFP4>{}); break;

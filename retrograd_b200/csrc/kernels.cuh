@@ -25,6 +25,10 @@ struct WeightView {
     // zero-padded to a multiple of 128 (read by the tcgen05 kernel and the weight-streaming kernel).
     // Q8_0, optional: the layout described at kQ8TileBytes, rows padded to a multiple of 16.
     const uint8_t * tiled = nullptr;
+    // Q4_0 (and, when asked for, MXFP4 expert banks): the units of the few-token products (w4.cuh) of the same rows, of this
+    // type. `data` and `type` then are what longer steps read: Q4_0 as the Q8_0 rows of the same values.
+    const uint8_t * w4 = nullptr;
+    uint32_t w4_type = 0;
     // The matrix passed the host-side check its tcgen05 kernel needs, made once when the weights are uploaded.
     // Q4_K: every super-block lets the kernel fold the minimum term into the main accumulator (q4k_min_fold_ok).
     // Q8_0: every block scale keeps d * q inside the f16 range, so a weight is an exact f16 pair (q8_0_products_fit_f16).

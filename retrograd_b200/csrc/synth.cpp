@@ -6,7 +6,7 @@
 // reference's fixture generators (scripts/gen-tiny-fixture.py:116-133,226-374,
 // scripts/gen-tiny-moe-fixture.py:192-362). The Q8_0 quantiser is the
 // reference's (d = amax/127, round half away from zero; gen-tiny-fixture.py:173-198).
-// The Q4_K and MXFP4 encoders are this project's own: any valid encoder will do,
+// The Q4_0 quantiser is the published one of the format. The Q4_K and MXFP4 encoders are this project's own: any valid encoder will do,
 // since parity is "the same bytes decoded two ways".
 //
 // Workloads here are synthetic by construction: weights ~ N(0, std) from the
@@ -67,6 +67,24 @@ void quantize_q8_0(const float * x, size_t n, uint8_t * out) {
             double code = std::floor(std::fabs(s) + 0.5);
             if (code > 127.0) code = 127.0;
             o[2 + i] = (uint8_t)(int8_t)(s >= 0.0 ? (int)code : -(int)code);
+        }
+    }
+}
+
+// Published reference quantiser of the format: d = (the element of largest magnitude) / -8, q = trunc(x / d + 8.5).
+void quantize_q4_0(const float * x, size_t n, uint8_t * out) {
+    for (size_t b = 0; b < n / 32; ++b) {
+        const float * v = x + b * 32;
+        float top = 0.f;
+        for (int i = 0; i < 32; ++i)
+            if (std::fabs(v[i]) > std::fabs(top)) top = v[i];
+        const float d = top / -8.f, inv = d != 0.f ? 1.f / d : 0.f;
+        const uint16_t dh = float_to_half(d);
+        uint8_t * o = out + b * 18;
+        std::memcpy(o, &dh, 2);
+        for (int i = 0; i < 16; ++i) {
+            const int lo = std::min(15, (int)(int8_t)(v[i] * inv + 8.5f)), hi = std::min(15, (int)(int8_t)(v[16 + i] * inv + 8.5f));
+            o[2 + i] = (uint8_t)(lo | hi << 4);
         }
     }
 }
@@ -170,6 +188,7 @@ void encode_row(uint32_t type, const float * x, size_t n, uint8_t * out) {
                 std::memcpy(out + 2 * i, &h, 2);
             }
             break;
+        case GGML_Q4_0: quantize_q4_0(x, n, out); break;
         case GGML_Q8_0: quantize_q8_0(x, n, out); break;
         case GGML_Q4_K: quantize_q4_k(x, n, out); break;
         case GGML_MXFP4: quantize_mxfp4(x, n, out); break;
@@ -180,6 +199,7 @@ void encode_row(uint32_t type, const float * x, size_t n, uint8_t * out) {
 uint32_t parse_type(const std::string & s) {
     if (s == "f32") return GGML_F32;
     if (s == "f16") return GGML_F16;
+    if (s == "q4_0") return GGML_Q4_0;
     if (s == "q8_0") return GGML_Q8_0;
     if (s == "q4_k" || s == "q4_K") return GGML_Q4_K;
     if (s == "mxfp4") return GGML_MXFP4;
