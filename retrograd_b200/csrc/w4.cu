@@ -1,10 +1,11 @@
 // Products with 4-bit weights for at most sixteen tokens, bound by the weight stream.
 //
 // Mathematics. 16 rows x 64 columns are the A operands of four m16n8k16 products; the tokens are the columns
-// of B. The weights enter as exact f16 values that cost next to no arithmetic:
-//   Q4_0   the nibble q in the low bits of an f16 is the subnormal q 2^-24, in the next four bits 16 q 2^-24; the
-//          columns whose nibbles sit there get their activations divided by 16. The offset is the product chain's start
-//          value, -8 2^-24 times the group's sum of activations.
+// of B. The weights enter as exact f16 values that cost little arithmetic:
+//   Q4_0   the nibble q in the top four mantissa bits of an f16 is the subnormal q 2^-18: a rotation and a mask. (In the
+//          low bits it would save the rotation, but the tensor cores align products by the operands' exponents and dropped up to ten
+//          bits of such products: 1.6e-6 of the result. As the difference q - 8 it costs an addition, 64 us instead of 55 for
+//          128256 x 4096 at one token.) The offset is the product chain's start value, -8 2^-18 times the group's sum of activations.
 //   MXFP4  the conversion instruction for pairs of e2m1 values.
 // A token's activations are scaled by a power of two that brings the largest of them into [2^13, 2^14) and split into
 // hi + lo f16 (22 bits); activations that are f16 or bf16 themselves need no lo. A 32-column group is exactly two
@@ -154,7 +155,7 @@ template <bool MX, int H, int S> __device__ __forceinline__ void decode(const ui
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if constexpr (!MX) {
-            a[j] = (S ? w[j] >> 8 : w[j]) & (H ? 0x00f000f0u : 0x000f000fu);
+            a[j] = __funnelshift_r(w[j], w[j], 4 * (2 * H + S)) & 0x03c003c0u;
         } else {
             // byte 2 H + S of the word
             asm("{\n.reg .b8 b<4>;\nmov.b32 {b0, b1, b2, b3}, %1;\ncvt.rn.f16x2.e2m1x2 %0, b%2;\n}" : "=r"(a[j]) : "r"(w[j]), "n"(2 * H + S));
@@ -221,8 +222,8 @@ template <int WARPS> struct Scratch {
 __device__ __forceinline__ int shift_for(uint32_t top) { return top > 0 && top < 0x7f800000u ? max(-100, min(126, 140 - (int)(top >> 23))) : 0; }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // The power of two a sum is short of: of the weights' f16 form, and of MXFP4's scale bytes (kept plus 8).
-__host__ __device__ constexpr int weight_shift(bool mx) { return mx ? -8 : 24; }
-constexpr float kStartUnit = 5.9604644775390625e-8f;       // 2^-24
+__host__ __device__ constexpr int weight_shift(bool mx) { return mx ? -8 : 18; }
+constexpr float kStart = -8.f * 3.814697265625e-6f;        // Q4_0's offset, in units of 2^-18
 
 __device__ __forceinline__ uint32_t bits(const __half2 & h) { return *reinterpret_cast<const uint32_t *>(&h); }
 
@@ -314,14 +315,13 @@ __device__ void stage_rows(const Act & act, int n, int nt, int k0, int steps, in
             if (it0 + it >= trips) break;
             const int i = first + (it0 + it) * shared * 32;
             const int step = i >> 5, group = (i >> 3) & 3, at = (i & 7) * 4;
-            const float factor = !MX && (group & 1) ? up * 0.0625f : up;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) held[it][e] *= factor;
+            for (int e = 0; e < 4; ++e) held[it][e] *= up;
             if constexpr (!MX) {
                 float sum = (held[it][0] + held[it][1]) + (held[it][2] + held[it][3]);
 #pragma unroll
                 for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (i < padded && (lane & 7) == 0) out.c[(step * 4 + group) * nt + row] = sum * (group & 1 ? -128.f : -8.f) * kStartUnit;
+                if (i < padded && (lane & 7) == 0) out.c[(step * 4 + group) * nt + row] = sum * kStart;
             }
             if (i < padded) put_split<PARTS>(out.x + ((step * 4 + group) * PARTS * nt + row) * 64 + at * 2, nt * 64, held[it]);
         }
@@ -878,7 +878,6 @@ __device__ void partial_logits(const MoeArgs & a, int k0, int k1, const Staged &
                 float4 w[EB];
 #pragma unroll
                 for (int e = 0; e < EB; ++e) w[e] = *reinterpret_cast<const float4 *>(r + min(e0 + e, a.E - 1) * n + c);
-                const float factor = !MX && (group & 1) ? 16.f : 1.f;
 #pragma unroll
                 for (int t = 0; t < TB; ++t) {
                     const uint8_t * p = x.x + ((step * 4 + group) * PARTS * NT + min(t0 + t, a.T - 1)) * 64 + (at & 31) * 2;
@@ -891,7 +890,7 @@ __device__ void partial_logits(const MoeArgs & a, int k0, int k1, const Staged &
                     }
 #pragma unroll
                     for (int e = 0; e < EB; ++e)
-                        acc[e * TB + t] += factor * (w[e].x * v0.x + w[e].y * v0.y + w[e].z * v1.x + w[e].w * v1.y);
+                        acc[e * TB + t] += w[e].x * v0.x + w[e].y * v0.y + w[e].z * v1.x + w[e].w * v1.y;
                 }
             }
             const float sum = warp_sums16(acc);
@@ -1071,8 +1070,7 @@ __device__ __forceinline__ void put_hidden(const MoeArgs & a, const Picks & p, i
     const int last = block == a.blocks_ff - 1 ? 3 : block & 3;
     for (int group = block & 3; group <= last; ++group) {
         if (group != (block & 3)) v = 0.f;
-        const float lower = !a.down_mx && (group & 1) ? 0.0625f : 1.f;
-        const float s = v * power(shift) * lower;
+        const float s = v * power(shift);
         const __half hi = __float2half_rn(s), lo = __float2half_rn(s - __half2float(hi));
         __half * x = reinterpret_cast<__half *>(at + (group * 2 * nt + place) * 64) + lane;
         x[0] = hi;
@@ -1082,7 +1080,7 @@ __device__ __forceinline__ void put_hidden(const MoeArgs & a, const Picks & p, i
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0)
             *reinterpret_cast<float2 *>(at + step_x_bytes(2, nt) + (group * nt + place) * 8) =
-                make_float2(power(weight_shift(a.down_mx) - shift), sum * (group & 1 ? -128.f : -8.f) * kStartUnit);
+                make_float2(power(weight_shift(a.down_mx) - shift), sum * kStart);
     }
 }
 
@@ -1367,7 +1365,7 @@ __global__ void __launch_bounds__(256, MOST > 1 ? 2 : 3) w4_moe_down_kernel(MoeA
 // ---- retiling
 //
 // Word j (0..3) of lane (g, t) and half w (0, 1) of a unit's row tile holds row g + 8 (j & 1), columns 8 t + 4 s + 2 (j >> 1) + e of
-// group 2 w + h, for the products s = 0, 1, groups h = 0, 1 and e = 0, 1. Q4_0: the nibble at bit 16 e + 8 s + 4 h. MXFP4: the
+// group 2 w + h, for the products s = 0, 1, groups h = 0, 1 and e = 0, 1. Q4_0: the nibble at bit 6 + 16 e + 4 (2 h + s), modulo 32. MXFP4: the
 // nibble at bit 8 (2 h + s) + 4 e, a pair for the conversion to every byte.
 template <bool MX>
 __global__ void w4_retile_kernel(const uint8_t * rows, uint32_t n_out, uint32_t n_in, uint32_t row_blocks, uint32_t steps, uint8_t * units, int * max_scale) {
@@ -1392,7 +1390,7 @@ __global__ void w4_retile_kernel(const uint8_t * rows, uint32_t n_out, uint32_t 
                 for (uint32_t e = 0; e < 2; ++e) {
                     const uint32_t k = 8 * t + 4 * s + 2 * (j >> 1) + e;
                     const uint32_t n = (q[k & 15] >> (k >= 16 ? 4 : 0)) & 15u;
-                    word |= n << (MX ? 8 * (2 * h + s) + 4 * e : 16 * e + 8 * s + 4 * h);
+                    word |= MX ? n << (8 * (2 * h + s) + 4 * e) : __funnelshift_l(n << (6 + 16 * e), n << (6 + 16 * e), 4 * (2 * h + s));
                 }
         }
         *reinterpret_cast<uint32_t *>(dst + i * 4) = word;
