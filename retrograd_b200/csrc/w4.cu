@@ -15,7 +15,7 @@
 // it converts only its share of the activations. Its warps take (row block, part of the CTA's columns) runs, and
 // write every (row block, token)'s sums into the shared memory of the CTA that owns it, which adds them in a fixed order after one
 // cluster barrier (no workspace, no atomics: results are the same in every run) and applies bias, residual or the gate's
-// activation. Every warp streams its units through a ring of its own in shared memory by asynchronous copies, two units
+// activation. Every warp streams its units through a ring of its own in shared memory by asynchronous copies, one or two units
 // ahead, so that no registers are held by loads in flight. Up to four tokens run as three CTAs of eight warps on an SM; more
 // as one of sixteen, because all warps of a CTA share its activations.
 
@@ -32,13 +32,17 @@ namespace rb200 {
 
 namespace {
 
-constexpr int kStages = 3;          // units in a warp's ring
 constexpr int kSlotCol = 36;        // floats per (partial slot, token) of the second expert kernel: 32 rows, padded against bank conflicts
 constexpr int kRowList = kW4PassTokens;
 constexpr int kMaxCluster = 8;
 // Warps of a CTA that serves up to n tokens, and its CTAs on an SM.
 __host__ __device__ constexpr int warps_for(int n) { return n > 4 ? 16 : 8; }
 __host__ __device__ constexpr int resident_for(int n) { return n > 4 ? 1 : 3; }
+// Units in the ring of each of its warps. For products of more than eight f32 tokens the activations and the sums need the room more (14336 x
+// 4096 gated pair, sixteen tokens: 50 us with three, whose sums took seven rounds, 35 us with two); where the activations are
+// halves two is slower (4096 x 14336, eleven f16 tokens: 25 us and 20 us), and so it is for the expert layer (163 us and 149 us).
+__host__ __device__ constexpr int stages_for(int n, int parts) { return n > 8 && parts == 2 ? 2 : 3; }
+constexpr int kMoeStages = 3;
 
 struct Act {
     const void * p;
@@ -77,9 +81,17 @@ __device__ __forceinline__ void load4(const Act & a, int64_t row, int k, float (
     }
 }
 
-__device__ __forceinline__ void scale4(float (&v)[4], const float * by) {
+__device__ __forceinline__ void scale4(float (&v)[4], const float * by, bool vec) {
+    float w[4];
+    if (vec) {
+        const float4 f = *reinterpret_cast<const float4 *>(by);
+        w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= by[e];
+        for (int e = 0; e < 4; ++e) w[e] = by[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= w[e];
 }
 
 __device__ __forceinline__ void store1(void * p, uint32_t type, int64_t i, float v) {
@@ -126,7 +138,7 @@ template <bool MX> struct Scales {
     uint4 s[2];     // MXFP4 uses .x and .y only
 };
 
-__host__ __device__ constexpr int ring_bytes(bool mx, int warps) { return warps * kStages * (int)w4_unit_bytes(mx); }
+__host__ __device__ constexpr int ring_bytes(bool mx, int n, int stages) { return warps_for(n) * stages * (int)w4_unit_bytes(mx); }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t * src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -251,6 +263,7 @@ __device__ void stage_rows(const Act & act, int n, int nt, int k0, int steps, in
     const int count = min(steps * 32, (n_in - k0) / 4), padded = steps * 32;
     const int trips = (padded + shared * 32 - 1) / (shared * 32), first = part * 32 + lane;
     const bool live = row < n;          // there are as many warps as tokens, or more
+    const bool norm_vec = (reinterpret_cast<uintptr_t>(norm) & 15) == 0;
     float held[kHeld][4];
     auto load = [&](int it0) {
 #pragma unroll
@@ -265,7 +278,7 @@ __device__ void stage_rows(const Act & act, int n, int nt, int k0, int steps, in
 #pragma unroll
             for (int it = 0; it < kHeld; ++it) {
                 const int i = first + (it0 + it) * shared * 32;
-                if (it0 + it < trips && i < count) scale4(held[it], norm + k0 + 4 * i);
+                if (it0 + it < trips && i < count) scale4(held[it], norm + k0 + 4 * i, norm_vec);
             }
         }
     };
@@ -521,7 +534,8 @@ struct Cursor {
 // Runs a warp's sequence. Source: first(Cursor &) and next(Cursor &) move to a run (never an empty one) and set everything;
 // group(const Cursor &) describes the activations; column(const Cursor &, column) is the cluster address that takes 32 rows' sums.
 // LIST: groups name their tokens.
-template <bool MX, class Source> struct Stream {
+template <bool MX, int STAGES, class Source> struct Stream {
+    static constexpr int kStages = STAGES;
     static constexpr uint32_t kUnit = w4_unit_bytes(MX);
     const Source & src;
     const int lane;
@@ -713,13 +727,13 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, resident_for(NT)) w4_produ
     const int ks = a.ks, log_ks = __ffs(ks) - 1;
     uint8_t * const rings = smem + a.x_bytes + a.c_bytes;
     const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
-    const Inbox inbox{smem_address(rings + ring_bytes(MX, kWarps)), a.inbox, rank, log_c, ks, kPer};
+    const Inbox inbox{smem_address(rings + ring_bytes(MX, NT, stages_for(NT, PARTS))), a.inbox, rank, log_c, ks, kPer};
     const int sub = warp & (ks - 1), step = part_begin2(n_steps, sub, log_ks), len = part_begin2(n_steps, sub + 1, log_ks) - step;
     const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
     if (threadIdx.x == 0) sc.zero = 0;
 
     ProductSource<MX, PARTS, GLU, NT> src{a, x_warp, inbox, b_begin * kPer, blocks * kPer, warp >> log_ks, kWarps >> log_ks, sub, s0 + step, len, 0, 0};
-    Stream<MX, ProductSource<MX, PARTS, GLU, NT>> stream(src, rings);
+    Stream<MX, stages_for(NT, PARTS), ProductSource<MX, PARTS, GLU, NT>> stream(src, rings);
     stream.prefetch();
     // the weights above are the library's own; everything below is the caller's
     pdl_trigger();
@@ -1105,23 +1119,31 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
     pdl_trigger();
     pdl_wait();
     const int k0 = s0 * 128, k1 = min(a.d, (s0 + n_steps) * 128);
-    fetch_router(a, k0, min(k1 - k0, router_columns(a.E, ring_bytes(MX, kWarps))), rings);      // the rings are idle until the experts are known
+    // the rings and the first inbox are idle until the experts are known
+    const int idle = ring_bytes(MX, NT, kMoeStages) + a.inbox;
+    fetch_router(a, k0, min(k1 - k0, router_columns(a.E, idle)), rings);
     copies_commit();
     stage_tokens<MX, PARTS>(a.x, a.T, NT, k0, n_steps, a.d, a.norm, x, sc, rank, C);
     __syncthreads();
-    partial_logits<MX, PARTS, NT, kWarps>(a, k0, k1, x, rings, ring_bytes(MX, kWarps), mine);
-    // out of the activations' scale: a token's factors without the weights' constant
+    partial_logits<MX, PARTS, NT, kWarps>(a, k0, k1, x, rings, idle, mine);
+    // Out of the activations' scale (a token's factor without the weights' constant) and to every CTA of the cluster: into its second
+    // inbox, which nobody else writes before the cluster has met after the first round, where that has room.
     __syncthreads();
-    for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) mine[i] *= sc.factor[i / a.E] * power(-weight_shift(MX));
+    const int n_logits = a.T * a.E;
+    const uint32_t mail = smem_address(rings) + ring_bytes(MX, NT, kMoeStages) + a.inbox;
+    const bool posted = C * n_logits * 4 <= a.inbox;
+    for (int i = threadIdx.x; i < n_logits; i += kWarps * 32) {
+        const float v = mine[i] * (sc.factor[i / a.E] * power(-weight_shift(MX)));
+        if (posted) {
+            for (int c = 0; c < C; ++c) remote_store(remote_address(mail + (rank * n_logits + i) * 4, c), v);
+        } else {
+            mine[i] = v;
+        }
+    }
     cluster_sync();
-    for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) {
-        const uint32_t at = smem_address(mine + i);
-        float part[kMaxCluster];
-#pragma unroll
-        for (int c = 0; c < kMaxCluster; ++c) part[c] = remote_load(remote_address(at, min(c, C - 1)));
+    for (int i = threadIdx.x; i < n_logits; i += kWarps * 32) {
         float v = 0.f;
-#pragma unroll
-        for (int c = 0; c < kMaxCluster; ++c) v += c < C ? part[c] : 0.f;
+        for (int c = 0; c < C; ++c) v += posted ? shared_f1(mail + (c * n_logits + i) * 4) : remote_load(remote_address(smem_address(mine + i), c));
         logits[i] = a.norm ? v * rms_factor(sc, i / a.E, C, a.d, a.eps) : v;
     }
     if (threadIdx.x < a.T) picks.rstd[threadIdx.x] = a.norm ? rms_factor(sc, threadIdx.x, C, a.d, a.eps) : 1.f;
@@ -1144,9 +1166,9 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
     const int room = (a.inbox >> (log_c + log_ks + 8)) << log_c;        // units of a round
     const int sub = warp & (ks - 1), step = part_begin2(n_steps, sub, log_ks), len = part_begin2(n_steps, sub + 1, log_ks) - step;
     const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
-    const Inbox inbox{smem_address(rings + ring_bytes(MX, kWarps)), a.inbox, rank, log_c, ks, 2};
+    const Inbox inbox{smem_address(rings + ring_bytes(MX, NT, kMoeStages)), a.inbox, rank, log_c, ks, 2};
     GateUpSource<MX, PARTS, NT> src{a, picks, x_warp, inbox, 2 * b_begin, 2 * blocks, warp >> log_ks, kWarps >> log_ks, sub, s0 + step, len, 0, 0};
-    Stream<MX, GateUpSource<MX, PARTS, NT>> stream(src, rings);
+    Stream<MX, kMoeStages, GateUpSource<MX, PARTS, NT>> stream(src, rings);
     stream.prefetch();
     int u = b_begin / a.blocks_ff, block = b_begin - u * a.blocks_ff;       // where the round begins
     for (int b0 = 0; b0 < blocks; ++src.round) {
@@ -1182,6 +1204,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
 // The second kernel's stream: as Stream, but a unit comes with the hidden columns it multiplies. Weights run two units ahead, hidden
 // columns one.
 template <bool MX, int MOST> struct DownStream {
+    static constexpr int kStages = 3;
     static constexpr uint32_t kUnit = w4_unit_bytes(MX), kHidden = MOST * kHiddenBytes;
     static constexpr int kRingBytes = 8 * (kStages * (int)kUnit + 2 * (int)kHidden);
     const MoeArgs & a;
@@ -1316,16 +1339,18 @@ __global__ void __launch_bounds__(256, MOST > 1 ? 2 : 3) w4_moe_down_kernel(MoeA
     pdl_trigger();
     pdl_wait();
     {
-        // the lists as long as they can be, in 16-byte words; what lies behind the last set is not used
+        // the lists as long as they can be, in 16-byte words, every one by a thread of its own; what lies behind the last set is not used
         const int sets = min(kMaxSets, (a.T * a.k + 15) / 16 * 16);
-        auto fetch = [&](void * to, const void * from, int bytes) {
-            for (int i = threadIdx.x; i < bytes / 16; i += kWarps * 32) static_cast<int4 *>(to)[i] = static_cast<const int4 *>(from)[i];
-        };
-        fetch(&meta.n, &a.meta->n, 16);
-        fetch(meta.expert, a.meta->expert, 2 * sets);
-        fetch(meta.first, a.meta->first, 2 * sets);
-        fetch(meta.count, a.meta->count, sets);
-        fetch(meta.token, a.meta->token, 4 * sets);
+        const int n_expert = 1 + sets / 8, n_first = n_expert + sets / 8, n_count = n_first + sets / 16, n_token = n_count + sets / 4;
+        const int4 * from = reinterpret_cast<const int4 *>(a.meta);
+        int4 * to = reinterpret_cast<int4 *>(&meta);
+        for (int i = threadIdx.x; i < n_token; i += kWarps * 32) {
+            const int at = i == 0 ? 0
+                : i < n_expert ? (int)offsetof(MoeMeta, expert) / 16 + i - 1
+                : i < n_first ? (int)offsetof(MoeMeta, first) / 16 + i - n_expert
+                : i < n_count ? (int)offsetof(MoeMeta, count) / 16 + i - n_first : (int)offsetof(MoeMeta, token) / 16 + i - n_count;
+            to[at] = from[at];
+        }
     }
     cluster_wait();
     __syncthreads();
@@ -1549,23 +1574,24 @@ struct Cut {
 // shared memory a step. The estimate is in clocks: the weight stream at the SM's share of the memory bandwidth, but no faster
 // than the busiest SM's warps get through it or than its copies in flight allow; the conversion of the CTA's share of the activations; the sums it
 // receives; and a barrier for every round its inbox allows. `step_clocks` is what else a column step costs a CTA.
-Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int most_resident, int most_c, int fixed, double step_clocks, int sms) {
+Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int stages, int most_resident, int least_c, int most_c, int fixed, double step_clocks, int sms) {
     Cut best;
-    const int warps = warps_for(n), ring = ring_bytes(mx, warps), unit = (int)w4_unit_bytes(mx);
-    for (int C = 1; C <= most_c && C <= steps; C *= 2) {
+    const int warps = warps_for(n), ring = ring_bytes(mx, n, stages), unit = (int)w4_unit_bytes(mx);
+    for (int C = least_c; C <= most_c && C <= steps; C *= 2) {
         const int s = (steps + C - 1) / C;
         const int64_t smem = (int64_t)s * each + ring + fixed + 2 * inbox_bytes(n, C, 1, per) + 4096;
         if (smem > kMaxSmem) continue;
         Cut c;
         c.C = C;
         c.resident = (int)std::min<int64_t>(most_resident, kSmShare / smem);
+        // as few clusters as keep their size: the places they leave free are where the next kernel of the stream begins
         const int most = resident_clusters(log2_of(C), c.resident, warps * 32), blocks_each = (blocks + most - 1) / most;
         c.clusters = (blocks + blocks_each - 1) / blocks_each;
         const int busy = (c.clusters * C + sms - 1) / sms;
         const int ks = split_columns(blocks_each * per, steps / C, warps, warps);
         const int runs = (blocks_each * per * ks + warps - 1) / warps;           // of the busiest warp
         const double unit_clocks = n > 8 ? 150 : n > 4 ? 120 : 80;
-        const double in_flight = (double)c.clusters * C * warps * (kStages - 1) * unit;
+        const double in_flight = (double)c.clusters * C * warps * (stages - 1) * unit;
         const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms) * std::max(1.0, 13e6 / in_flight),     // two microseconds of latency under load
                                         (double)busy * runs * warps * ((s + ks - 1) / ks + (n > 8 ? 0.6 : 0.3)) * unit_clocks});
         const double convert = busy * s * (n * 128 * 0.1 + step_clocks) + 800, sums = busy * (double)blocks_each * per * n * (6 + 2 * C * ks);
@@ -1612,11 +1638,11 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
         Cut cut;
         for (;; n = (n + 1) / 2) {
-            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), mx, resident_for(product_room(n, parts)), kMaxCluster, 0, 0, device_sms());
+            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), mx, stages_for(n, parts), resident_for(product_room(n, parts)), 1, kMaxCluster, 0, 0, device_sms());
             if (cut.C || n == 1) break;
         }
         if (!cut.C) return cudaErrorInvalidValue;       // rows this long are refused when the handle is made
-        const int C = cut.C, nt = product_room(n, parts), warps = warps_for(nt), s = (steps + C - 1) / C;
+        const int C = cut.C, nt = product_room(n, parts), warps = warps_for(n), s = (steps + C - 1) / C;
         ProductArgs a{};
         a.w = p.w.units;
         a.u = glu ? p.up->units : nullptr;
@@ -1638,14 +1664,17 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
         a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
         // two inboxes in what is left of the CTA's share of the shared memory; one, if everything fits into it
-        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx, warps);
+        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx, nt, stages_for(nt, parts));
         const int blocks_each = a.each + (a.more > 0);
         const int64_t room = std::min(kSmShare / cut.resident - 4096, kMaxSmem) - fixed;
         a.ks = split_columns(blocks_each * per, steps / C, warps, (int)std::max<int64_t>(1, room / 2 / inbox_bytes(n, C, 1, per)));
         const int64_t whole = inbox_bytes((int64_t)blocks_each * n, C, a.ks, per);
         a.inbox = (int)(whole <= room ? whole : std::max<int64_t>(room / 2 / 128 * 128, inbox_bytes(n, C, a.ks, per)));
         a.per_round = whole <= room ? blocks_each : blocks_per_round(a.inbox, n, C, a.ks, per, warps);
-        const size_t smem = (size_t)fixed + (whole <= room ? 1 : 2) * (size_t)a.inbox;
+        size_t smem = (size_t)fixed + (whole <= room ? 1 : 2) * (size_t)a.inbox;
+        // no more CTAs on an SM than an even spread needs: clusters are packed densely otherwise, and leave SMs idle
+        const int spread = (cut.clusters * C + device_sms() - 1) / device_sms();
+        if (spread < cut.resident) smem = std::max(smem, (size_t)(kSmShare / (spread + 1)));
         cudaError_t e;
         if (mx) e = glu ? launch_product_of<true, true>(a, parts, cut.clusters, C, smem, stream) : launch_product_of<true, false>(a, parts, cut.clusters, C, smem, stream);
         else e = glu ? launch_product_of<false, true>(a, parts, cut.clusters, C, smem, stream) : launch_product_of<false, false>(a, parts, cut.clusters, C, smem, stream);
@@ -1668,12 +1697,14 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
     constexpr int kStatic = 16 * 1024;          // the routing tables
     for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
-        // first kernel: n tokens that choose independently choose about `reach` experts. Up to four tokens it runs in clusters of at most four
-        // (one token, 32 experts of 2880 x 2880: 33 us the layer, 39 us with eight), unless rows are so long that four cannot hold them.
+        // first kernel: n tokens that choose independently choose about `reach` experts. It runs in clusters of four (one token, 32 experts of
+        // 2880 x 2880: 33 us the layer, 39 us with eight; sixteen tokens: 147 us, 181 us with two), of eight where rows are so long
+        // that four cannot hold them.
         Cut cut;
         for (;; n = (n + 1) / 2) {
             const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n))));
-            cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), mx, product_room(n, parts) > 4 ? 1 : 2, n > 4 || steps_d > 256 ? kMaxCluster : 4,
+            const int least_c = std::min(4, steps_d < 2 ? 1 : steps_d < 4 ? 2 : 4);
+            for (int C = least_c; !cut.C && C <= kMaxCluster; C *= 2) cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), mx, kMoeStages, product_room(n, parts) > 4 ? 1 : 2, C, C,
                              2 * up_to(n * E * 4, 128) + kStatic, n * E * 0.4 + E * 4.0, sms);
             if (cut.C || n == 1) break;
         }
@@ -1716,7 +1747,7 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
         a.logit_bytes = up_to(n * E * 4, 128);
         a.clusters = cut.clusters;
-        const int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx, warps_for(nt));
+        const int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx, nt, kMoeStages);
         a.inbox = (int)std::max<int64_t>((std::min(kSmShare / cut.resident - kStatic - 4096, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, cut.C, 1, 2));
         cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream)
                            : launch_gate_up_of<false>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream);
