@@ -1488,20 +1488,20 @@ template <bool MX, int PARTS, bool GLU, int NT> cudaError_t launch_product(const
 }
 
 // Room the kernels that take whole calls of n tokens stage them with: those sizes they are built for.
-int product_room(int n, int parts) { return n == 1 ? 1 : n <= 4 && parts == 2 ? 4 : n <= 8 ? 8 : 16; }
+int product_room(int n) { return n == 1 ? 1 : n <= 4 ? 4 : n <= 8 ? 8 : 16; }
 
 // Calls f with the room as a constant.
-template <int PARTS, class F> cudaError_t with_room(int nt, F f) {
+template <class F> cudaError_t with_room(int nt, F f) {
     if (nt == 1) return f(std::integral_constant<int, 1>{});
-    if constexpr (PARTS == 2) if (nt == 4) return f(std::integral_constant<int, 4>{});
+    if (nt == 4) return f(std::integral_constant<int, 4>{});
     if (nt == 8) return f(std::integral_constant<int, 8>{});
     return f(std::integral_constant<int, 16>{});
 }
 
 template <bool MX, bool GLU> cudaError_t launch_product_of(const ProductArgs & a, int parts, int clusters, int C, size_t smem, cudaStream_t stream) {
-    const int nt = product_room(a.T, parts);
-    if (parts == 2) return with_room<2>(nt, [&](auto n) { return launch_product<MX, 2, GLU, decltype(n)::value>(a, clusters, C, smem, stream); });
-    return with_room<1>(nt, [&](auto n) { return launch_product<MX, 1, GLU, decltype(n)::value>(a, clusters, C, smem, stream); });
+    const int nt = product_room(a.T);
+    if (parts == 2) return with_room(nt, [&](auto n) { return launch_product<MX, 2, GLU, decltype(n)::value>(a, clusters, C, smem, stream); });
+    return with_room(nt, [&](auto n) { return launch_product<MX, 1, GLU, decltype(n)::value>(a, clusters, C, smem, stream); });
 }
 
 template <bool MX, int PARTS, int NT> cudaError_t launch_gate_up(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
@@ -1511,9 +1511,9 @@ template <bool MX, int PARTS, int NT> cudaError_t launch_gate_up(const MoeArgs &
 }
 
 template <bool MX> cudaError_t launch_gate_up_of(const MoeArgs & a, int parts, int C, size_t smem, cudaStream_t stream) {
-    const int nt = product_room(a.T, parts);
-    if (parts == 2) return with_room<2>(nt, [&](auto n) { return launch_gate_up<MX, 2, decltype(n)::value>(a, C, smem, stream); });
-    return with_room<1>(nt, [&](auto n) { return launch_gate_up<MX, 1, decltype(n)::value>(a, C, smem, stream); });
+    const int nt = product_room(a.T);
+    if (parts == 2) return with_room(nt, [&](auto n) { return launch_gate_up<MX, 2, decltype(n)::value>(a, C, smem, stream); });
+    return with_room(nt, [&](auto n) { return launch_gate_up<MX, 1, decltype(n)::value>(a, C, smem, stream); });
 }
 
 template <bool MX, int MOST> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
@@ -1603,6 +1603,30 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int sta
     return best;
 }
 
+// choose_cut for a product of n tokens (in passes of fewer, where rows are too long for them): remembered by the sizes it depends on.
+Cut product_cut(int blocks, int per, int steps, bool mx, int parts, int & n) {
+    struct Known {
+        int key[7] = {};
+        int n = 0;
+        Cut cut;
+    };
+    thread_local Known known[16];
+    int device = 0;
+    cudaGetDevice(&device);
+    const int key[7] = {blocks, per, steps, mx, parts, n, device + 1};
+    Known & k = known[((unsigned)blocks * 31 + (unsigned)steps * 7 + (unsigned)n * 3 + (unsigned)per) % 16];
+    if (!std::equal(key, key + 7, k.key)) {
+        for (k.n = n;; k.n = (k.n + 1) / 2) {
+            const int room = product_room(k.n);
+            k.cut = choose_cut(blocks, per, steps, k.n, step_bytes(mx, parts, room), mx, stages_for(k.n, parts), resident_for(room), 1, kMaxCluster, 0, 0, device_sms());
+            if (k.cut.C || k.n == 1) break;
+        }
+        std::copy(key, key + 7, k.key);
+    }
+    n = k.n;
+    return k.cut;
+}
+
 } // namespace
 
 size_t w4_bytes(uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert) {
@@ -1636,13 +1660,9 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
     const int blocks = (int)p.w.blocks, per = glu ? 2 : 1, steps = (int)p.w.steps;
     for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
-        Cut cut;
-        for (;; n = (n + 1) / 2) {
-            cut = choose_cut(blocks, per, steps, n, step_bytes(mx, parts, product_room(n, parts)), mx, stages_for(n, parts), resident_for(product_room(n, parts)), 1, kMaxCluster, 0, 0, device_sms());
-            if (cut.C || n == 1) break;
-        }
+        const Cut cut = product_cut(blocks, per, steps, mx, parts, n);
         if (!cut.C) return cudaErrorInvalidValue;       // rows this long are refused when the handle is made
-        const int C = cut.C, nt = product_room(n, parts), warps = warps_for(n), s = (steps + C - 1) / C;
+        const int C = cut.C, nt = product_room(n), warps = warps_for(n), s = (steps + C - 1) / C;
         ProductArgs a{};
         a.w = p.w.units;
         a.u = glu ? p.up->units : nullptr;
@@ -1704,7 +1724,7 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         for (;; n = (n + 1) / 2) {
             const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n))));
             const int least_c = std::min(4, steps_d < 2 ? 1 : steps_d < 4 ? 2 : 4);
-            for (int C = least_c; !cut.C && C <= kMaxCluster; C *= 2) cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n, parts)), mx, kMoeStages, product_room(n, parts) > 4 ? 1 : 2, C, C,
+            for (int C = least_c; !cut.C && C <= kMaxCluster; C *= 2) cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n)), mx, kMoeStages, product_room(n) > 4 ? 1 : 2, C, C,
                              2 * up_to(n * E * 4, 128) + kStatic, n * E * 0.4 + E * 4.0, sms);
             if (cut.C || n == 1) break;
         }
@@ -1742,7 +1762,7 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.meta = static_cast<MoeMeta *>(p.workspace);
         a.hidden = static_cast<uint8_t *>(p.workspace) + (sizeof(MoeMeta) + 255) / 256 * 256;
 
-        const int nt = product_room(n, parts), s = (steps_d + cut.C - 1) / cut.C;
+        const int nt = product_room(n), s = (steps_d + cut.C - 1) / cut.C;
         a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
         a.logit_bytes = up_to(n * E * 4, 128);
