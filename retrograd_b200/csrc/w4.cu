@@ -228,10 +228,10 @@ template <int WARPS> struct Scratch {
     uint64_t zero;                              // start values of PACK's lo columns
 };
 
-// 2^shift brings the magnitude with these bits into [2^13, 2^14), as far as it and the factor that takes it back are f32 (below 2^-113 the
-// values only come near; above 2^113 they count as infinite). Rows with an infinity or a NaN are left as they are: their own
+// 2^shift brings the magnitude with these bits into [2^13, 2^14), as far as it and the factor that takes it back (2^-8 - shift for MXFP4) are
+// normal f32: below 2^-104 the values only come near, and are off by 2^-143 at most; above 2^113 they count as infinite. Rows with an infinity or a NaN are left as they are: their own
 // sums become NaN, those of the other tokens stay what they are.
-__device__ __forceinline__ int shift_for(uint32_t top) { return top > 0 && top < 0x7f800000u ? max(-100, min(126, 140 - (int)(top >> 23))) : 0; }
+__device__ __forceinline__ int shift_for(uint32_t top) { return top > 0 && top < 0x7f800000u ? max(-100, min(118, 140 - (int)(top >> 23))) : 0; }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // The power of two a sum is short of: of the weights' f16 form, and of MXFP4's scale bytes (kept plus 8).
 __host__ __device__ constexpr int weight_shift(bool mx) { return mx ? -8 : 18; }

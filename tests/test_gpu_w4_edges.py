@@ -86,6 +86,30 @@ def test_result_types(rb):
 
 
 @pytest.mark.parametrize("kind", [Q4_0, MXFP4])
+@pytest.mark.parametrize("tokens", [1, 2, 4, 7, 16])
+def test_small_and_large_magnitudes(rb, kind, tokens):
+    """Rows of zeros, rows down to the smallest f32 and up to 2^100. Below 2^-104 an activation is a multiple of 2^-142 (the scale that takes
+    sums back has to be an f32 too) and off by half of that."""
+    import torch
+
+    rng = np.random.default_rng(tokens + kind)
+    n_in = 224
+    m, w, mag = matrix(rb, rng, kind, 90, n_in, spread=1)
+    for exponent in (-140, -130, -120, -112, -108, -104, -100, -60, 60, 100):
+        base = rng.normal(0, 1, (tokens, n_in)).clip(-3, 3)
+        x = torch.tensor((base * 2.0 ** exponent).astype(np.float32)).cuda()
+        if tokens > 1:
+            x[tokens // 2] = 0
+        x64 = x.double().cpu().numpy()
+        y = rb.w4_matvec(m, x).double().cpu().numpy()
+        # 2^-149: the result's own half step below the normal numbers, in each of the cluster's partial sums and the factor's product
+        bound = f32_bound(n_in) * (np.abs(x64) @ mag.T) + 2.0 ** -143 * mag.sum(1) + 8 * 2.0 ** -149
+        assert (np.abs(y - x64 @ w.T) <= bound).all(), exponent
+        if tokens > 1:
+            assert (y[tokens // 2] == 0).all()
+
+
+@pytest.mark.parametrize("kind", [Q4_0, MXFP4])
 @pytest.mark.parametrize("tokens", [2, 4, 6, 16])
 def test_tokens_do_not_reach_one_another(rb, kind, tokens):
     """A token with an infinity or a NaN: its own results are not finite, the others are what they were. In the expert layer the other token's
