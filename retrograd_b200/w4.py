@@ -13,13 +13,16 @@ from . import _ffi
 from .engine import EngineError, InvalidArgument, _check, _last_error
 
 _TYPES: dict = {}       # torch dtype -> GGML type code
+_raw_stream = None      # current stream handle of a device
 
 
 def _torch():
     import torch
 
+    global _raw_stream
     if not _TYPES:
         _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
     return torch
 
 
@@ -63,6 +66,7 @@ class W4Matrix:
         _check(lib.retro_b200_w4_info(h, None, None, C.byref(nbytes), C.byref(where)))
         self.ggml_type, self.n_out, self.n_in, self.n_expert = ggml_type, n_out, n_in, n_expert
         self.nbytes, self.device = nbytes.value, where.value
+        self._workspace: dict = {}      # bytes of w4_moe's workspace by (tokens of a pass, experts per token)
 
     def close(self) -> None:
         """Frees the device memory; no call that uses the matrix may be pending."""
@@ -96,8 +100,7 @@ def _rows(op: str, name: str, t, width: int, device: int, tokens: int = -1):
 def _vector(op: str, name: str, t, n: int, device: int):
     if t is None:
         return None
-    torch = _torch()
-    if t.dtype != torch.float32 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
+    if _TYPES.get(t.dtype) != 0 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
         raise InvalidArgument(f"{op}: {name} must be {n} consecutive float32 on the weights' device")
     return t.data_ptr()
 
@@ -111,48 +114,66 @@ def _open(op: str, *matrices) -> int:
     return matrices[0].device
 
 
-def _result(torch, op, x, out, tokens, width, device):
+def _new(x, shape, dtype, stream, device: int):
+    """A tensor on x's device, made on the stream the call runs on: the allocator hands its memory to no other stream before."""
+    on = _raw_stream(device)
+    if stream is None or getattr(stream, "cuda_stream", stream) == on:
+        return x.new_empty(shape, dtype=dtype)
+    torch = _torch()
+    with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=device)):
+        return x.new_empty(shape, dtype=dtype)
+
+
+def _result(op: str, x, out, tokens: int, width: int, device: int, stream):
+    """The result tensor (a new one of x's type unless `out` is given), its pointer, type code and row stride."""
     if out is None:
-        return torch.empty(tokens, width, dtype=x.dtype, device=x.device)
-    return out
+        y = _new(x, (tokens, width), x.dtype, stream, device)
+        return y, y.data_ptr(), _TYPES[x.dtype], width
+    return (out, *_rows(op, "out", out, width, device, tokens))
 
 
-def _stream(torch, stream, device):
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else getattr(stream, "cuda_stream", stream)
+def _residual(op: str, residual, code: int, width: int, device: int, tokens: int):
+    if residual is None:
+        return None, 0
+    pointer, own, ld = _rows(op, "residual", residual, width, device, tokens)
+    if own != code:
+        raise InvalidArgument(f"{op}: residual must have the result's element type")
+    return pointer, ld
+
+
+def _stream(stream, device: int):
+    return _raw_stream(device) if stream is None else getattr(stream, "cuda_stream", stream)
 
 
 def w4_matvec(w: W4Matrix, x, *, norm=None, eps: float = 1e-5, bias=None, residual=None, out=None, stream=None):
     """y = xn W^T + bias + residual for x [tokens, n_in]; xn is x, or its RMSNorm with the weights `norm`. `out` (any of the three
     element types, may be `residual`) or a new tensor of x's type is returned; a residual has the result's type."""
-    torch = _torch()
+    _TYPES or _torch()
     device = _open("w4_matvec", w)
-    n_in, n_out = w.n_in, w.n_out
-    px, tx, ldx = _rows("w4_matvec", "x", x, n_in, device)
+    px, tx, ldx = _rows("w4_matvec", "x", x, w.n_in, device)
     tokens = x.shape[0]
-    y = _result(torch, "w4_matvec", x, out, tokens, n_out, device)
-    py, ty, ldy = _rows("w4_matvec", "out", y, n_out, device, tokens)
-    pr, ldr = None, 0
-    if residual is not None:
-        pr, tr, ldr = _rows("w4_matvec", "residual", residual, n_out, device, tokens)
-        if tr != ty:
-            raise InvalidArgument("w4_matvec: residual must have the result's element type")
+    y, py, ty, ldy = _result("w4_matvec", x, out, tokens, w.n_out, device, stream)
+    pr, ldr = _residual("w4_matvec", residual, ty, w.n_out, device, tokens)
     if tokens:
-        _check(w._lib.retro_b200_w4_matvec(w._h, px, tx, ldx, tokens, _vector("w4_matvec", "norm", norm, n_in, device), eps,
-                                           _vector("w4_matvec", "bias", bias, n_out, device), pr, ldr, py, ty, ldy, _stream(torch, stream, device)))
+        status = w._lib.retro_b200_w4_matvec(w._h, px, tx, ldx, tokens, _vector("w4_matvec", "norm", norm, w.n_in, device), eps,
+                                             _vector("w4_matvec", "bias", bias, w.n_out, device), pr, ldr, py, ty, ldy, _stream(stream, device))
+        if status:
+            _check(status)
     return y
 
 
 def w4_glu(gate: W4Matrix, up: W4Matrix, x, *, norm=None, eps: float = 1e-5, out=None, stream=None):
     """y = silu(xn Wgate^T) * (xn Wup^T) for x [tokens, n_in]: the first half of a gated FFN."""
-    torch = _torch()
+    _TYPES or _torch()
     device = _open("w4_glu", gate, up)
     px, tx, ldx = _rows("w4_glu", "x", x, gate.n_in, device)
     tokens = x.shape[0]
-    y = _result(torch, "w4_glu", x, out, tokens, gate.n_out, device)
-    py, ty, ldy = _rows("w4_glu", "out", y, gate.n_out, device, tokens)
+    y, py, ty, ldy = _result("w4_glu", x, out, tokens, gate.n_out, device, stream)
     if tokens:
-        _check(gate._lib.retro_b200_w4_glu(gate._h, up._h, px, tx, ldx, tokens, _vector("w4_glu", "norm", norm, gate.n_in, device), eps, py, ty, ldy,
-                                           _stream(torch, stream, device)))
+        status = gate._lib.retro_b200_w4_glu(gate._h, up._h, px, tx, ldx, tokens, _vector("w4_glu", "norm", norm, gate.n_in, device), eps, py, ty, ldy,
+                                             _stream(stream, device))
+        if status:
+            _check(status)
     return y
 
 
@@ -167,13 +188,8 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
     n_in = gate.n_in
     px, tx, ldx = _rows("w4_moe", "x", x, n_in, device)
     tokens = x.shape[0]
-    y = _result(torch, "w4_moe", x, out, tokens, n_in, device)
-    py, ty, ldy = _rows("w4_moe", "out", y, n_in, device, tokens)
-    pr, ldr = None, 0
-    if residual is not None:
-        pr, tr, ldr = _rows("w4_moe", "residual", residual, n_in, device, tokens)
-        if tr != ty:
-            raise InvalidArgument("w4_moe: residual must have the result's element type")
+    y, py, ty, ldy = _result("w4_moe", x, out, tokens, n_in, device, stream)
+    pr, ldr = _residual("w4_moe", residual, ty, n_in, device, tokens)
     if not 1 <= n_used <= min(gate.n_expert, 32):
         raise InvalidArgument("w4_moe: n_used must be 1 to n_expert, at most 32")
     for name, t, dtype in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
@@ -181,12 +197,9 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
             raise InvalidArgument(f"w4_moe: {name} must be contiguous {dtype} [{tokens}, {n_used}] on the weights' device")
     if not tokens:
         return y
-    on = _stream(torch, stream, device)
+    on = _stream(stream, device)
     if workspace is None:
-        workspace = torch.empty(w4_moe_workspace(gate, tokens, n_used), dtype=torch.uint8, device=x.device)
-        if stream is not None and on != torch.cuda.current_stream(device).cuda_stream:
-            # freed to the allocator when this call returns: it must not be handed out before the given stream is done with it
-            workspace.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(on, device=device))
+        workspace = _new(x, (w4_moe_workspace(gate, tokens, n_used),), torch.uint8, stream, device)
     elif workspace.get_device() != device or not workspace.is_contiguous():
         raise InvalidArgument("w4_moe: the workspace must be contiguous on the weights' device")
     _check(gate._lib.retro_b200_w4_moe(_vector("w4_moe", "router", router, gate.n_expert * n_in, device), gate._h, up._h, down._h, px, tx, ldx, tokens, n_used,
@@ -198,7 +211,11 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
 
 def w4_moe_workspace(gate: W4Matrix, tokens: int, n_used: int) -> int:
     """Bytes of workspace a `w4_moe` call of `tokens` tokens needs."""
-    _open("w4_moe_workspace", gate)
-    n = C.c_size_t()
-    _check(gate._lib.retro_b200_w4_moe_workspace(gate._h, tokens, n_used, C.byref(n)))
-    return n.value
+    key = min(tokens, 16), n_used
+    known = gate._workspace.get(key)
+    if known is None:
+        _open("w4_moe_workspace", gate)
+        n = C.c_size_t()
+        _check(gate._lib.retro_b200_w4_moe_workspace(gate._h, key[0], n_used, C.byref(n)))
+        known = gate._workspace[key] = n.value
+    return known
