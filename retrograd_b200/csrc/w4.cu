@@ -39,8 +39,8 @@ constexpr int kMaxCluster = 8;
 __host__ __device__ constexpr int warps_for(int n) { return n > 4 ? 16 : 8; }
 __host__ __device__ constexpr int resident_for(int n) { return n > 4 ? 1 : 3; }
 // Units in the ring of each of its warps. For products of more than eight f32 tokens the activations and the sums need the room more (14336 x
-// 4096 gated pair, sixteen tokens: 50 us with three, whose sums took seven rounds, 35 us with two); where the activations are
-// halves two is slower (4096 x 14336, eleven f16 tokens: 25 us and 20 us), and so it is for the expert layer (163 us and 149 us).
+// 4096 gated pair, sixteen tokens: 50 us with three, whose sums took seven rounds, 36 us with two); where the activations are
+// halves two is slower (4096 x 14336, eleven f16 tokens: 25 us and 20 us), and so it is for the expert layer (163 us and 147 us).
 __host__ __device__ constexpr int stages_for(int n, int parts) { return n > 8 && parts == 2 ? 2 : 3; }
 constexpr int kMoeStages = 3;
 
@@ -48,7 +48,7 @@ struct Act {
     const void * p;
     int64_t ld;
     uint32_t type;
-    bool vec;       // four elements may be read at once
+    bool vec;       // rows may be read sixteen bytes at a time
 };
 
 __device__ __forceinline__ float load1(const Act & a, int64_t row, int k) {
@@ -56,42 +56,6 @@ __device__ __forceinline__ float load1(const Act & a, int64_t row, int k) {
     if (a.type == GGML_F32) return static_cast<const float *>(a.p)[i];
     const uint16_t h = static_cast<const uint16_t *>(a.p)[i];
     return a.type == GGML_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
-}
-
-// Elements k .. k + 3 of a row.
-__device__ __forceinline__ void load4(const Act & a, int64_t row, int k, float (&v)[4]) {
-    if (!a.vec) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = load1(a, row, k + i);
-        return;
-    }
-    const int64_t at = row * a.ld + k;
-    if (a.type == GGML_F32) {
-        const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.p) + at);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else {
-        const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.p) + at);
-        if (a.type == GGML_F16) {
-            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-            v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
-        } else {
-            v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-            v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
-        }
-    }
-}
-
-__device__ __forceinline__ void scale4(float (&v)[4], const float * by, bool vec) {
-    float w[4];
-    if (vec) {
-        const float4 f = *reinterpret_cast<const float4 *>(by);
-        w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = by[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= w[e];
 }
 
 __device__ __forceinline__ void store1(void * p, uint32_t type, int64_t i, float v) {
@@ -154,6 +118,9 @@ __device__ __forceinline__ uint2 shared_u2(uint32_t at) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
     return v;
+}
+__device__ __forceinline__ void store_u4(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 __device__ __forceinline__ float shared_f1(uint32_t at) {
     float v;
@@ -249,58 +216,69 @@ template <int PARTS> __device__ __forceinline__ void put_split(uint8_t * dst, in
     }
 }
 
-// Converts columns [k0, k0 + 128 steps) of n rows into the layout of nt tokens; columns at and behind n_in are zero. A row is one warp's
-// work, or with few rows that of several warps. NORM: rows are multiplied by `norm`, and put_squares(row, sum) gets the row's sum of
-// squares. Every thread takes part; a barrier follows at the caller's.
-template <bool MX, int PARTS, int WARPS, bool NORM, class PutSquares>
-__device__ void stage_rows(const Act & act, int n, int nt, int k0, int steps, int n_in, const float * norm, const Staged & out, Scratch<WARPS> & sc,
-                           PutSquares put_squares) {
-    constexpr int kHeld = 4;            // loads of that many chunks of four columns are in flight together
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int shared = 1;                     // warps that share a row
-    while (2 * shared * n <= WARPS) shared *= 2;
-    const int part = warp & (shared - 1), row = warp / shared;
-    const int count = min(steps * 32, (n_in - k0) / 4), padded = steps * 32;
-    const int trips = (padded + shared * 32 - 1) / (shared * 32), first = part * 32 + lane;
-    const bool live = row < n;          // there are as many warps as tokens, or more
-    const bool norm_vec = (reinterpret_cast<uintptr_t>(norm) & 15) == 0;
-    float held[kHeld][4];
-    auto load = [&](int it0) {
-#pragma unroll
-        for (int it = 0; it < kHeld; ++it) {
-            const int i = first + (it0 + it) * shared * 32;
-            held[it][0] = held[it][1] = held[it][2] = held[it][3] = 0.f;
-            if (it0 + it < trips && i < count) load4(act, row, k0 + 4 * i, held[it]);
-        }
-    };
-    auto weigh = [&](int it0) {
-        if constexpr (NORM) {
-#pragma unroll
-            for (int it = 0; it < kHeld; ++it) {
-                const int i = first + (it0 + it) * shared * 32;
-                if (it0 + it < trips && i < count) scale4(held[it], norm + k0 + 4 * i, norm_vec);
-            }
-        }
-    };
-    // the largest magnitude as bits: a NaN is above infinity, infinity above every number
-    uint32_t top = 0;
-    float squares = 0.f;
-    for (int it0 = 0; live && it0 < trips; it0 += kHeld) {
-        load(it0);
-        if constexpr (NORM) {
-#pragma unroll
-            for (int it = 0; it < kHeld; ++it)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) squares += held[it][e] * held[it][e];
-        }
-        weigh(it0);
-#pragma unroll
-        for (int it = 0; it < kHeld; ++it)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(held[it][e]) & 0x7fffffffu);
+// Where a call's norm weights wait for its rows: 512 bytes for every step, four steps in each of `count` places `stride` bytes apart.
+struct NormRoom {
+    uint32_t base;
+    int stride, count;
+    __device__ __forceinline__ uint32_t at(int step) const { return base + (step >> 2) * stride + (step & 3) * 512; }
+};
+
+// Sixteen bytes of `from` (element size ES) to shared memory, asynchronously where their alignment allows it. Through the L2 cache only.
+template <int ES> __device__ __forceinline__ void fetch16(uint32_t dst, const void * from, bool vec) {
+    if (vec) {
+        copy16(dst, static_cast<const uint8_t *>(from));
+        return;
     }
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (ES == 4) w[j] = __ldcg(static_cast<const unsigned *>(from) + j);
+        else w[j] = __ldcg(static_cast<const unsigned short *>(from) + 2 * j) | (uint32_t)__ldcg(static_cast<const unsigned short *>(from) + 2 * j + 1) << 16;
+    }
+    store_u4(dst, w[0], w[1], w[2], w[3]);
+}
+
+// Four columns of a row as they are stored: f32 in .x to .w, halves in .x and .y.
+__device__ __forceinline__ void widen4(const uint4 & u, uint32_t type, float (&v)[4]) {
+    if (type == GGML_F32) {
+        v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
+    } else if (type == GGML_F16) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    } else {
+        v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
+        v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+}
+template <int PARTS> __device__ __forceinline__ uint32_t type_of(const Act & act) { return PARTS == 2 ? act.type : act.type == GGML_F16 ? GGML_F16 : GGML_BF16; }
+
+// Columns k .. k + 3 of a row, through the L2 cache only.
+__device__ __forceinline__ uint4 load4(const Act & act, uint32_t type, int64_t row, int k) {
+    uint4 u = {};
+    if (type == GGML_F32) {
+        const unsigned * from = static_cast<const unsigned *>(act.p) + row * act.ld + k;
+        if (act.vec) u = __ldcg(reinterpret_cast<const uint4 *>(from));
+        else u = make_uint4(__ldcg(from), __ldcg(from + 1), __ldcg(from + 2), __ldcg(from + 3));
+    } else {
+        const unsigned short * from = static_cast<const unsigned short *>(act.p) + row * act.ld + k;
+        if (act.vec) {
+            const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(from));
+            u.x = w.x;
+            u.y = w.y;
+        } else {
+            u.x = __ldcg(from) | (uint32_t)__ldcg(from + 1) << 16;
+            u.y = __ldcg(from + 2) | (uint32_t)__ldcg(from + 3) << 16;
+        }
+    }
+    return u;
+}
+
+// The largest magnitude (as bits: a NaN is above infinity, infinity above every number) and the sum of squares of a row that
+// `shared` warps share. Every thread takes part.
+template <int WARPS> __device__ __forceinline__ void row_totals(Scratch<WARPS> & sc, int shared, int part, uint32_t & top, float & squares) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     top = __reduce_max_sync(0xffffffffu, top);
-    if constexpr (NORM) {
+    {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
     }
@@ -311,49 +289,177 @@ __device__ void stage_rows(const Act & act, int n, int nt, int k0, int steps, in
         squares = 0.f;
         for (int i = 0; i < shared; ++i) { top = max(top, sc.top[warp - part + i]); squares += sc.squares[warp - part + i]; }
     }
-    if (!live) return;
-    const int shift = shift_for(top);
-    const float up = power(shift);
-    if (part == 0 && lane == 0) {
-        sc.factor[row] = power(weight_shift(MX) - shift);
-        if constexpr (NORM) put_squares(row, squares);
-    }
-    for (int it0 = 0; it0 < trips; it0 += kHeld) {
-        if (trips > kHeld) {            // a longer row is read again
-            load(it0);
-            weigh(it0);
+}
+
+// Converts columns [k0, k0 + 128 steps) of n rows into the layout of nt tokens; columns at and behind n_in are zero. A row is one warp's
+// work, or with few rows that of several warps, a step at a time. Up to kHeld steps a warp are held in registers. For more, all rows
+// are first copied as they are, every 32 columns to where their converted form belongs (f32 fill the places of hi and lo, halves that of hi), so
+// that the copies are in flight together; the largest magnitude and the conversion are two passes over shared memory. (Sixteen f32 tokens,
+// 14336 x 4096 gated pair: 36 us; 38.6 us with registers in two batches and a second reading. One token, 4096 x 14336: 11.4 us in registers,
+// 12.0 us through shared memory.) A function of its own, so that the product loops' registers do not depend on it. With `norm`, rows are multiplied by it,
+// and put_squares(row, sum) gets the row's sum of squares. Every thread takes part; a barrier follows at the caller's.
+template <bool MX, int PARTS, int WARPS, class PutSquares>
+__device__ __noinline__ void stage_rows(const Act act, int n, int nt, int k0, int steps, int n_in, const float * norm, const NormRoom room, const Staged out,
+                           Scratch<WARPS> & sc, PutSquares put_squares) {
+    constexpr int kHeld = 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int shared = 1, log_shared = 0;     // warps that share a row
+    while (2 * shared * n <= WARPS) { shared *= 2; ++log_shared; }
+    const int part = warp & (shared - 1), row = warp >> log_shared;
+    const int columns = min(steps * 128, n_in - k0);
+    const bool live = row < n;          // there are as many warps as tokens, or more
+    const uint32_t type = type_of<PARTS>(act);
+    const int group_bytes = PARTS * nt * 64, lo = nt * 64;
+    const bool norm_vec = norm && (reinterpret_cast<uintptr_t>(norm) & 15) == 0;
+    uint32_t top = 0;
+    float squares = 0.f, up = 1.f;
+    auto count = [&](const float (&v)[4]) {
+        if (norm) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) squares += v[e] * v[e];
         }
+    };
+    auto compare = [&](const float (&v)[4]) {
 #pragma unroll
-        for (int it = 0; it < kHeld; ++it) {
-            if (it0 + it >= trips) break;
-            const int i = first + (it0 + it) * shared * 32;
-            const int step = i >> 5, group = (i >> 3) & 3, at = (i & 7) * 4;
+        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    };
+    auto totals = [&] {
+        row_totals<WARPS>(sc, shared, part, top, squares);
+        const int shift = shift_for(top);
+        up = power(shift);
+        if (live && part == 0 && lane == 0) {
+            sc.factor[row] = power(weight_shift(MX) - shift);
+            if (norm) put_squares(row, squares);
+        }
+    };
+    // the lane's columns of a step in their final form; every lane has read what it needs of the place they go to
+    auto put = [&](int step, float (&v)[4]) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) held[it][e] *= up;
-            if constexpr (!MX) {
-                float sum = (held[it][0] + held[it][1]) + (held[it][2] + held[it][3]);
+        for (int e = 0; e < 4; ++e) v[e] *= up;
+        if constexpr (!MX) {
+            float sum = (v[0] + v[1]) + (v[2] + v[3]);
 #pragma unroll
-                for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (i < padded && (lane & 7) == 0) out.c[(step * 4 + group) * nt + row] = sum * kStart;
+            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if ((lane & 7) == 0) out.c[(step * 4 + (lane >> 3)) * nt + row] = sum * kStart;
+        }
+        put_split<PARTS>(out.x + (step * 4 + (lane >> 3)) * group_bytes + row * 64 + (lane & 7) * 8, lo, v);
+    };
+
+    if (steps <= kHeld << log_shared) {
+        uint4 raw[kHeld], by[kHeld];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int c = (part + (i << log_shared)) * 128 + lane * 4;
+            raw[i] = by[i] = make_uint4(0, 0, 0, 0);
+            if (live && c < columns) {
+                raw[i] = load4(act, type, row, k0 + c);
+                if (norm) by[i] = load4(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
             }
-            if (i < padded) put_split<PARTS>(out.x + ((step * 4 + group) * PARTS * nt + row) * 64 + at * 2, nt * 64, held[it]);
         }
+        float v[kHeld][4];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            widen4(raw[i], type, v[i]);
+            count(v[i]);
+            if (norm) {
+                v[i][0] *= __uint_as_float(by[i].x); v[i][1] *= __uint_as_float(by[i].y); v[i][2] *= __uint_as_float(by[i].z); v[i][3] *= __uint_as_float(by[i].w);
+            }
+            compare(v[i]);
+        }
+        totals();
+        if (!live) return;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int step = part + (i << log_shared);
+            if (step >= steps) break;
+            put(step, v[i]);
+        }
+        return;
+    }
+
+    const uint32_t slot = smem_address(out.x) + row * 64;
+    const bool norm_staged = norm && steps <= 4 * room.count;
+    if (norm_staged) {
+        for (int i = threadIdx.x; i < steps * 32; i += WARPS * 32) {
+            const uint32_t dst = room.at(i >> 5) + (i & 31) * 16;
+            if (4 * i < columns) fetch16<4>(dst, norm + k0 + 4 * i, norm_vec);
+            else store_u4(dst, 0, 0, 0, 0);
+        }
+    }
+    if (live) {
+        if (type == GGML_F32) {
+            const float * from = static_cast<const float *>(act.p) + row * act.ld + k0;
+            for (int step = part; step < steps; step += shared) {
+                const uint32_t dst = slot + (step * 4 + (lane >> 3)) * group_bytes + (lane & 4 ? lo : 0) + (lane & 3) * 16;
+                const int c = step * 128 + lane * 4;
+                if (c < columns) fetch16<4>(dst, from + c, act.vec);
+                else store_u4(dst, 0, 0, 0, 0);
+            }
+        } else {                        // two of the warp's steps at a time
+            const uint16_t * from = static_cast<const uint16_t *>(act.p) + row * act.ld + k0;
+            for (int step = part + ((lane >> 4) << log_shared); step < steps; step += 2 * shared) {
+                const uint32_t dst = slot + (step * 4 + ((lane & 15) >> 2)) * group_bytes + (lane & 3) * 16;
+                const int c = step * 128 + (lane & 15) * 8;
+                if (c < columns) fetch16<2>(dst, from + c, act.vec);
+                else store_u4(dst, 0, 0, 0, 0);
+            }
+        }
+    }
+    copies_commit();
+    copies_wait<0>();
+    __syncthreads();
+
+    auto read = [&](int step, float (&v)[4]) {
+        const uint32_t at = slot + (step * 4 + (lane >> 3)) * group_bytes;
+        uint4 u = {};
+        if (type == GGML_F32) {
+            u = shared_u4(at + (lane & 4 ? lo : 0) + (lane & 3) * 16);
+        } else {
+            const uint2 w = shared_u2(at + (lane & 7) * 8);
+            u.x = w.x;
+            u.y = w.y;
+        }
+        widen4(u, type, v);
+    };
+    auto weigh = [&](int step, float (&v)[4]) {
+        if (norm) {
+            uint4 by = {};
+            const int c = step * 128 + lane * 4;
+            if (norm_staged) by = shared_u4(room.at(step) + lane * 16);
+            else if (c < columns) by = load4(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
+            v[0] *= __uint_as_float(by.x); v[1] *= __uint_as_float(by.y); v[2] *= __uint_as_float(by.z); v[3] *= __uint_as_float(by.w);
+        }
+    };
+    if (live) {
+#pragma unroll 2
+        for (int step = part; step < steps; step += shared) {
+            float v[4];
+            read(step, v);
+            count(v);
+            weigh(step, v);
+            compare(v);
+        }
+    }
+    totals();
+    if (!live) return;
+#pragma unroll 2
+    for (int step = part; step < steps; step += shared) {
+        float v[4];
+        read(step, v);
+        weigh(step, v);
+        __syncwarp();
+        put(step, v);
     }
 }
 
 // The rows of a call's tokens, normalised by its weights when it has any. A row's squares go to every CTA of the cluster.
 template <bool MX, int PARTS, int WARPS>
-__device__ __forceinline__ void stage_tokens(const Act & act, int n, int nt, int k0, int steps, int n_in, const float * norm, const Staged & out,
-                                             Scratch<WARPS> & sc, int rank, int C) {
-    if (norm) {
-        cluster_wait();
-        stage_rows<MX, PARTS, WARPS, true>(act, n, nt, k0, steps, n_in, norm, out, sc, [&](int t, float squares) {
-            for (int c = 0; c < C; ++c) remote_store(remote_address(smem_address(&sc.ss[rank][t]), c), squares);
-        });
-    } else {
-        stage_rows<MX, PARTS, WARPS, false>(act, n, nt, k0, steps, n_in, nullptr, out, sc, [](int, float) {});
-        cluster_wait();
-    }
+__device__ __forceinline__ void stage_tokens(const Act & act, int n, int nt, int k0, int steps, int n_in, const float * norm, const NormRoom & room,
+                                             const Staged & out, Scratch<WARPS> & sc, int rank, int C) {
+    cluster_wait();
+    stage_rows<MX, PARTS, WARPS>(act, n, nt, k0, steps, n_in, norm, room, out, sc, [&](int t, float squares) {
+        for (int c = 0; c < C; ++c) remote_store(remote_address(smem_address(&sc.ss[rank][t]), c), squares);
+    });
 }
 
 // 1 / sqrt(mean of squares + eps) of token t, once the cluster has met after stage_tokens.
@@ -738,7 +844,10 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, resident_for(NT)) w4_produ
     // the weights above are the library's own; everything below is the caller's
     pdl_trigger();
     pdl_wait();
-    stage_tokens<MX, PARTS>(a.x, a.T, NT, s0 * 128, n_steps, a.n_in, a.norm, x, sc, rank, C);
+    // the norm's weights wait in the last stage of every warp's ring, which the first units leave free
+    using Ring = Stream<MX, stages_for(NT, PARTS), ProductSource<MX, PARTS, GLU, NT>>;
+    const NormRoom room{smem_address(rings) + (Ring::kStages - 1) * Ring::kUnit, (int)(Ring::kStages * Ring::kUnit), kWarps};
+    stage_tokens<MX, PARTS>(a.x, a.T, NT, s0 * 128, n_steps, a.n_in, a.norm, room, x, sc, rank, C);
     __syncthreads();
     for (int b0 = 0; b0 < blocks; b0 += a.per_round, ++src.round) {
         const int now = min(a.per_round, blocks - b0);
@@ -1123,7 +1232,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
     const int idle = ring_bytes(MX, NT, kMoeStages) + a.inbox;
     fetch_router(a, k0, min(k1 - k0, router_columns(a.E, idle)), rings);
     copies_commit();
-    stage_tokens<MX, PARTS>(a.x, a.T, NT, k0, n_steps, a.d, a.norm, x, sc, rank, C);
+    stage_tokens<MX, PARTS>(a.x, a.T, NT, k0, n_steps, a.d, a.norm, NormRoom{0, 0, 0}, x, sc, rank, C);
     __syncthreads();
     partial_logits<MX, PARTS, NT, kWarps>(a, k0, k1, x, rings, idle, mine);
     // Out of the activations' scale (a token's factor without the weights' constant) and to every CTA of the cluster: into its second
@@ -1528,7 +1637,7 @@ const void * row_at(const void * p, uint32_t type, int64_t ld, int64_t row) {
 
 Act make_act(const void * p, int64_t ld, uint32_t type) {
     const size_t es = type == GGML_F32 ? 4 : 2;
-    return {p, ld, type, (uintptr_t)p % (4 * es) == 0 && (ld * (int64_t)es) % (int64_t)(4 * es) == 0};
+    return {p, ld, type, (uintptr_t)p % 16 == 0 && ld * (int64_t)es % 16 == 0};
 }
 
 // Clusters of 2^log_c CTAs that are on the GPU together, with `resident` CTAs on an SM: a cluster lies within one of the GPU's processing
