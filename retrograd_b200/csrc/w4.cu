@@ -32,7 +32,7 @@ namespace rb200 {
 
 namespace {
 
-constexpr int kSlotCol = 36;        // floats per (partial slot, token) of the second expert kernel: 32 rows, padded against bank conflicts
+constexpr int kSlotCol = 36;        // floats per (partial slot, token) of the third expert kernel: 32 rows, padded against bank conflicts
 constexpr int kRowList = kW4PassTokens;
 constexpr int kMaxCluster = 8;
 // Warps of a CTA that serves up to n tokens, and its CTAs on an SM.
@@ -74,11 +74,6 @@ __device__ __forceinline__ uint32_t remote_address(uint32_t at, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
     return a;
-}
-__device__ __forceinline__ float remote_load(uint32_t address) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
-    return v;
 }
 __device__ __forceinline__ void remote_store(uint32_t address, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
@@ -252,22 +247,26 @@ __device__ __forceinline__ void widen4(const uint4 & u, uint32_t type, float (&v
 }
 template <int PARTS> __device__ __forceinline__ uint32_t type_of(const Act & act) { return PARTS == 2 ? act.type : act.type == GGML_F16 ? GGML_F16 : GGML_BF16; }
 
-// Columns k .. k + 3 of a row, through the L2 cache only.
-__device__ __forceinline__ uint4 load4(const Act & act, uint32_t type, int64_t row, int k) {
+// Columns k .. k + 3 of a row; L2: through the L2 cache only.
+template <bool L2, class T> __device__ __forceinline__ T load(const T * from) {
+    if constexpr (L2) return __ldcg(from);
+    else return *from;
+}
+template <bool L2> __device__ __forceinline__ uint4 load4(const Act & act, uint32_t type, int64_t row, int k) {
     uint4 u = {};
     if (type == GGML_F32) {
         const unsigned * from = static_cast<const unsigned *>(act.p) + row * act.ld + k;
-        if (act.vec) u = __ldcg(reinterpret_cast<const uint4 *>(from));
-        else u = make_uint4(__ldcg(from), __ldcg(from + 1), __ldcg(from + 2), __ldcg(from + 3));
+        if (act.vec) u = load<L2>(reinterpret_cast<const uint4 *>(from));
+        else u = make_uint4(load<L2>(from), load<L2>(from + 1), load<L2>(from + 2), load<L2>(from + 3));
     } else {
         const unsigned short * from = static_cast<const unsigned short *>(act.p) + row * act.ld + k;
         if (act.vec) {
-            const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(from));
+            const uint2 w = load<L2>(reinterpret_cast<const uint2 *>(from));
             u.x = w.x;
             u.y = w.y;
         } else {
-            u.x = __ldcg(from) | (uint32_t)__ldcg(from + 1) << 16;
-            u.y = __ldcg(from + 2) | (uint32_t)__ldcg(from + 3) << 16;
+            u.x = load<L2>(from) | (uint32_t)load<L2>(from + 1) << 16;
+            u.y = load<L2>(from + 2) | (uint32_t)load<L2>(from + 3) << 16;
         }
     }
     return u;
@@ -352,8 +351,8 @@ __device__ __noinline__ void stage_rows(const Act act, int n, int nt, int k0, in
             const int c = (part + (i << log_shared)) * 128 + lane * 4;
             raw[i] = by[i] = make_uint4(0, 0, 0, 0);
             if (live && c < columns) {
-                raw[i] = load4(act, type, row, k0 + c);
-                if (norm) by[i] = load4(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
+                raw[i] = load4<true>(act, type, row, k0 + c);
+                if (norm) by[i] = load4<true>(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
             }
         }
         float v[kHeld][4];
@@ -426,7 +425,7 @@ __device__ __noinline__ void stage_rows(const Act act, int n, int nt, int k0, in
             uint4 by = {};
             const int c = step * 128 + lane * 4;
             if (norm_staged) by = shared_u4(room.at(step) + lane * 16);
-            else if (c < columns) by = load4(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
+            else if (c < columns) by = load4<true>(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
             v[0] *= __uint_as_float(by.x); v[1] *= __uint_as_float(by.y); v[2] *= __uint_as_float(by.z); v[3] *= __uint_as_float(by.w);
         }
     };
@@ -723,6 +722,18 @@ __host__ __device__ inline int split_columns(int jobs, int steps, int warps, int
     return best;
 }
 
+// The same with any number of parts, where warps / ks jobs run side by side; and its cost.
+inline int divide_columns(int jobs, int steps, int warps, int most, int & cost) {
+    int best = 1;
+    cost = 0x7fffffff;
+    for (int ks = 1; ks <= warps && ks <= most && (ks == 1 || ks <= steps); ++ks) {
+        const int abreast = warps / ks, rounds = (jobs + abreast - 1) / abreast;
+        const int c = rounds * (2 * ((steps + ks - 1) / ks) + 3);
+        if (c < cost) { cost = c; best = ks; }
+    }
+    return best;
+}
+
 // Range `part` of `parts` nearly equal ranges of [0, n).
 __host__ __device__ inline int part_begin(int n, int part, int parts) {
     const unsigned each = (unsigned)n / (unsigned)parts, more = (unsigned)n - each * parts;
@@ -873,26 +884,74 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, resident_for(NT)) w4_produ
 
 // ---- a mixture-of-experts layer
 //
-// Two kernels. The first: every cluster normalises and routes all tokens for itself (the router is a few hundred
-// kilobytes that the L2 cache holds; a CTA reads its columns of it) instead of waiting for one place to do it, then multiplies its share of the chosen
-// experts' gate and up blocks and writes h = w_e silu(a) b for each (token, expert) pair, split into hi + lo f16 with a power of two for every
-// 32 columns: what the second kernel's products take. That one treats the chosen experts' down matrices as one long reduction: a cluster
+// Three kernels. The first, one cluster, routes: its CTAs take ranges of the columns of all logits, a token's parts meet in the CTA
+// that picks its experts, and the first CTA lists the chosen experts with their tokens. The second has started
+// meanwhile and staged its activations; it multiplies the chosen experts' gate and up blocks and writes h = w_e silu(a) b for each (token,
+// expert) pair, split into hi + lo f16 with a power of two for every 32 columns: what the third kernel's products take. That one treats the chosen
+// experts' down matrices as one long reduction: a cluster
 // owns a range of y's rows, its CTAs and their warps divide the experts' concatenated columns, every unit of weights arrives
 // in a warp's ring together with the hidden columns it multiplies, and the sum over experts is part of the sum over the cluster. An
 // expert of more than three tokens is visited once per three of them (its weights then come from the L2 cache).
+// (Routing in every cluster of the second kernel, which saves the launch, had them all read the router: 11 us until the weights' first
+// bytes at one token and 19 us at sixteen, 32 experts of 2880 x 2880.)
 
-constexpr int kSet = 3;                 // tokens of an expert the second kernel takes at once
-constexpr int kMaxSets = kRowList * kW4MaxUsed;
+constexpr int kSet = 3;                 // tokens of an expert the third kernel takes at once
+constexpr int kMaxPairs = kRowList * kW4MaxUsed;
 
-struct alignas(16) MoeMeta {            // in the workspace, in front of the hidden columns
-    int32_t n;                          // sets: up to kSet tokens of a chosen expert, experts ascending
-    int32_t pad[3];
-    uint16_t expert[kMaxSets];
-    uint16_t first[kMaxSets];           // tokens of the sets before
-    uint8_t count[kMaxSets];
-    uint8_t token[kMaxSets][4];
+// What the routing writes for the other kernels, in the workspace in front of the hidden columns: a header {chosen experts, sets, -, -}, then arrays
+// at these bytes, each long enough for `experts` chosen experts and `pairs` (token, expert) pairs.
+struct RouteAt {
+    int expert, before, cost;               // of the chosen experts, ascending: u16 id; u16 pairs before it; i32 cost of the blocks before it (one more of the latter two)
+    int weight, token;                      // of the pairs, by expert: f32, u8
+    int set_expert, set_first, set_count;   // up to kSet tokens of an expert: u16 id, u16 first pair, u8 count
+    int bytes;
 };
-static_assert(sizeof(MoeMeta) % 16 == 0 && kSet <= 4, "read as 16-byte words");
+__host__ __device__ constexpr RouteAt route_at(int experts, int pairs) {
+    RouteAt r{};
+    const auto up16 = [](int n) { return (n + 15) / 16 * 16; };
+    r.expert = 16;
+    r.before = r.expert + up16(2 * experts);
+    r.cost = r.before + up16(2 * (experts + 1));
+    r.weight = r.cost + up16(4 * (experts + 1));
+    r.token = r.weight + up16(4 * pairs);
+    r.set_expert = r.token + up16(pairs);
+    r.set_first = r.set_expert + up16(2 * pairs);
+    r.set_count = r.set_first + up16(2 * pairs);
+    r.bytes = r.set_count + up16(pairs);
+    return r;
+}
+constexpr int kRouteBytes = route_at(kW4MaxExperts, kMaxPairs).bytes;
+
+// A copy of it in shared memory.
+struct Route {
+    const uint8_t * p;
+    RouteAt at;
+    __device__ __forceinline__ int experts() const { return reinterpret_cast<const int *>(p)[0]; }
+    __device__ __forceinline__ int sets() const { return reinterpret_cast<const int *>(p)[1]; }
+    __device__ __forceinline__ int expert(int u) const { return reinterpret_cast<const uint16_t *>(p + at.expert)[u]; }
+    __device__ __forceinline__ int before(int u) const { return reinterpret_cast<const uint16_t *>(p + at.before)[u]; }
+    __device__ __forceinline__ int count(int u) const { return before(u + 1) - before(u); }
+    __device__ __forceinline__ int cost(int u) const { return reinterpret_cast<const int *>(p + at.cost)[u]; }
+    __device__ __forceinline__ float weight(int pair) const { return reinterpret_cast<const float *>(p + at.weight)[pair]; }
+    __device__ __forceinline__ const uint8_t * tokens(int pair) const { return p + at.token + pair; }
+    __device__ __forceinline__ int set_expert(int i) const { return reinterpret_cast<const uint16_t *>(p + at.set_expert)[i]; }
+    __device__ __forceinline__ int set_first(int i) const { return reinterpret_cast<const uint16_t *>(p + at.set_first)[i]; }
+    __device__ __forceinline__ int set_count(int i) const { return p[at.set_count + i]; }
+    // Units are the (block, token) results of the chosen experts' blocks, one behind the other: the first of a block.
+    __device__ __forceinline__ int unit(int u, int block, int blocks) const { return before(u) * blocks + block * count(u); }
+};
+
+// Copies the header and bytes [from, to) of a route, through the L2 cache only. A barrier follows at the caller's.
+__device__ __forceinline__ void copy_route(const uint8_t * route, uint8_t * copy, int from, int to) {
+    for (int i = threadIdx.x; i < 1 + (to - from) / 16; i += blockDim.x) {
+        const int at = i == 0 ? 0 : from + 16 * (i - 1);
+        *reinterpret_cast<uint4 *>(copy + at) = __ldcg(reinterpret_cast<const uint4 *>(route + at));
+    }
+}
+
+// What a block of an expert with n tokens costs, in parts of the time its weights take: 0.63 us for the two matrices' blocks of 32 x 2880 in a cluster
+// of four, 0.045 us more for each token's sums, 0.2 us more where the tokens' hi and lo are products of their own.
+__device__ __forceinline__ int block_cost(int n, int parts) { return 14 + n + (n > 8 ? 5 * parts : n > 4 && parts == 2 ? 5 : 0); }
 
 // Hidden columns: by set, by 128-column step, [group][part][token][32] f16, then [group][token] (factor, start value).
 constexpr int kHiddenBytes = 544;       // of one token and step
@@ -904,6 +963,7 @@ struct MoeArgs {
     const float * router;
     bool router_vec;            // sixteen bytes of it may be read at once
     bool down_mx;
+    int parts;
     Act x;
     int T, E, k, d, ff;
     int blocks_ff, steps_d, blocks_d, steps_ff;
@@ -917,27 +977,11 @@ struct MoeArgs {
     int64_t ld_y;
     int32_t * ids;
     float * weights;
-    MoeMeta * meta;
+    uint8_t * route;
+    RouteAt at;
     uint8_t * hidden;
-    int clusters, x_bytes, c_bytes, logit_bytes, inbox, partial;        // shared memory, in bytes
-    int ks, per_round;          // of the second kernel: parts of the columns, blocks of a round
-};
-
-struct Picks {
-    uint16_t expert[kRowList * kW4MaxUsed];
-    float weight[kRowList * kW4MaxUsed];
-    float rstd[kRowList];
-    uint16_t unique[kW4MaxExperts];
-    uint16_t before[kW4MaxExperts];                 // tokens of the experts before unique[i]
-    uint8_t count[kW4MaxExperts];                   // of unique[i]
-    uint8_t token[kW4MaxExperts][kRowList];
-    uint32_t mask[kW4MaxExperts];                   // by expert: the tokens that chose it
-    uint8_t rank[kW4MaxExperts][kRowList];          // of the expert among the token's
-    int sums[3][8];
-    int n;                                          // unique experts
-
-    // Units are the (block, token) results of the chosen experts' blocks, one behind the other: the first of a block.
-    __device__ __forceinline__ int unit(int u, int block, int blocks) const { return before[u] * blocks + block * count[u]; }
+    int clusters, x_bytes, c_bytes, inbox, partial;        // shared memory, in bytes
+    int ks, per_round;          // of the third kernel: parts of the columns, blocks of a round
 };
 
 // Sums each of the 16 values of a lane over the warp; lane i ends up with value i >> 1 (lanes 2 i and 2 i + 1 alike).
@@ -955,201 +999,271 @@ __device__ __forceinline__ float warp_sums16(float (&v)[16]) {
     return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
 }
 
-// Columns of the router that fit into `room` bytes for all experts: whole groups of 32.
-__device__ __forceinline__ int router_columns(int E, int room) { return room / (E * 128) * 32; }
-
-// Copies columns [k, k + n) of all router rows to shared memory, row e at e * n. The caller commits, waits and synchronises.
-__device__ __forceinline__ void fetch_router(const MoeArgs & a, int k, int n, uint8_t * to) {
-    const uint32_t dst = smem_address(to);
-    if (a.router_vec) {
-        const int chunks = n / 4;
-        for (int i = threadIdx.x; i < a.E * chunks; i += blockDim.x) {
-            const int e = i / chunks, c = i - e * chunks;
-            copy16(dst + i * 16, reinterpret_cast<const uint8_t *>(a.router + (size_t)e * a.d + k + c * 4));
-        }
-    } else {
-        for (int i = threadIdx.x; i < a.E * n; i += blockDim.x) {
-            const int e = i / n, c = i - e * n;
-            reinterpret_cast<float *>(to)[i] = a.router[(size_t)e * a.d + k + c];
-        }
-    }
-}
-
-// The CTA's columns' part of every (token, expert) logit, from the staged activations and, piece by piece, the router in
-// `room` (the first piece is already on its way). The sums are in the staged activations' scale.
-template <bool MX, int PARTS, int NT, int WARPS>
-__device__ void partial_logits(const MoeArgs & a, int k0, int k1, const Staged & x, uint8_t * room, int room_bytes, float * out) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int EB = 4, TB = NT == 1 ? 1 : 4;         // experts and tokens a warp takes at once
-    const int width = router_columns(a.E, room_bytes);
-    const int groups_t = (a.T + TB - 1) / TB, items = (a.E + EB - 1) / EB * groups_t;
-    for (int k = k0; k < k1; k += width) {
-        const int n = min(width, k1 - k);
-        if (k > k0) {
-            __syncthreads();
-            fetch_router(a, k, n, room);
-            copies_commit();
-        }
-        copies_wait<0>();
-        __syncthreads();
-        const float * r = reinterpret_cast<const float *>(room);
-        for (int item = warp; item < items; item += WARPS) {
-            const int e0 = item / groups_t * EB, t0 = (item - item / groups_t * groups_t) * TB;
-            float acc[16] = {};
-            for (int c = lane * 4; c < n; c += 128) {
-                const int at = k - k0 + c, step = at >> 7, group = (at >> 5) & 3;
-                float4 w[EB];
-#pragma unroll
-                for (int e = 0; e < EB; ++e) w[e] = *reinterpret_cast<const float4 *>(r + min(e0 + e, a.E - 1) * n + c);
-#pragma unroll
-                for (int t = 0; t < TB; ++t) {
-                    const uint8_t * p = x.x + ((step * 4 + group) * PARTS * NT + min(t0 + t, a.T - 1)) * 64 + (at & 31) * 2;
-                    const uint2 h = *reinterpret_cast<const uint2 *>(p);
-                    float2 v0 = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), v1 = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
-                    if constexpr (PARTS == 2) {
-                        const uint2 l = *reinterpret_cast<const uint2 *>(p + NT * 64);
-                        const float2 l0 = __half22float2(*reinterpret_cast<const __half2 *>(&l.x)), l1 = __half22float2(*reinterpret_cast<const __half2 *>(&l.y));
-                        v0.x += l0.x; v0.y += l0.y; v1.x += l1.x; v1.y += l1.y;
-                    }
-#pragma unroll
-                    for (int e = 0; e < EB; ++e)
-                        acc[e * TB + t] += w[e].x * v0.x + w[e].y * v0.y + w[e].z * v1.x + w[e].w * v1.y;
-                }
-            }
-            const float sum = warp_sums16(acc);
-            const int i = lane >> 1, e = e0 + i / TB, t = t0 + i % TB;
-            if (!(lane & 1) && i < EB * TB && e < a.E && t < a.T) {
-                if (k == k0) out[t * a.E + e] = sum;
-                else out[t * a.E + e] += sum;
-            }
-        }
-    }
-}
-
-// Softmax over the experts and the n_used likeliest of one token, by one warp. Ties go to the lowest index; whatever the
-// logits hold, n_used different experts are chosen (a NaN makes the weights NaN).
-__device__ void pick_experts(const float * logits, int E, int k, bool normalise, uint16_t * expert, float * weight) {
+// Softmax over the experts and the n_used likeliest of one token, by one warp: pick i is lane i's. Ties go to the lowest index; whatever the
+// logits hold, k different experts are chosen (a NaN makes the weights NaN). PER: experts of a lane.
+template <int PER, class Logit> __device__ __forceinline__ void pick_experts(Logit logit, int E, int k, bool normalise, int & expert, float & weight) {
     const int lane = threadIdx.x & 31;
-    constexpr int PER = kW4MaxExperts / 32;
     float p[PER];
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int e = lane + 32 * j;
-        p[j] = e < E ? logits[e] : -INFINITY;
-        if (32 * j < E) mx = fmaxf(mx, p[j]);
+        p[j] = e < E ? logit(e) : -INFINITY;
+        mx = fmaxf(mx, p[j]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        if (32 * j >= E) break;
         p[j] = lane + 32 * j < E ? expf(p[j] - mx) : 0.f;
         sum += p[j];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    // key: the probability's bits, which order like the probabilities, plus one; a NaN behind every number, taken ones at zero
+    // key: the probability's bits, which order like the probabilities, plus two; a NaN behind every number, taken ones at zero
     uint32_t key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        key[j] = 0;
-        if (32 * j >= E) continue;
         p[j] /= sum;
         key[j] = lane + 32 * j < E ? (p[j] >= 0.f ? __float_as_uint(p[j]) + 2u : 1u) : 0u;
     }
     float chosen = 0.f;
+    expert = 0;
+    weight = 0.f;
     for (int pick = 0; pick < k; ++pick) {
         uint32_t best = 0;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) if (32 * j < E) best = max(best, key[j]);
+        for (int j = 0; j < PER; ++j) best = max(best, key[j]);
         best = __reduce_max_sync(0xffffffffu, best);
         uint32_t at = 0xffffffffu;
 #pragma unroll
-        for (int j = PER - 1; j >= 0; --j) if (32 * j < E && key[j] == best) at = lane + 32 * j;
+        for (int j = PER - 1; j >= 0; --j) if (key[j] == best) at = lane + 32 * j;
         at = __reduce_min_sync(0xffffffffu, at);
         float value = 0.f;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            if (32 * j < E && at == (uint32_t)(lane + 32 * j)) {
+            if (at == (uint32_t)(lane + 32 * j)) {
                 value = p[j];
                 key[j] = 0;
             }
         }
         value = __shfl_sync(0xffffffffu, value, at & 31);
-        if (lane == 0) { expert[pick] = (uint16_t)at; weight[pick] = value; }
+        if (lane == pick) { expert = (int)at; weight = value; }
         chosen += value;
     }
-    if (normalise) {
-        __syncwarp();
-        for (int i = lane; i < k; i += 32) weight[i] /= chosen;
-    }
+    if (normalise) weight /= chosen;
 }
 
-// The chosen experts in ascending order with their tokens, from the picks of all tokens. Picks::mask is zero before. `meta`,
-// when not null, gets the sets of the second kernel.
-__device__ void group_picks(const MoeArgs & a, Picks & p, MoeMeta * meta) {
+// The routing tables of one CTA of the routing kernel.
+struct RouteScratch {
+    float sums[kRowList * kW4MaxExperts];       // parts of the CTA's logits [part][token][expert]; at most max(experts, 64) * 16
+    float mail[kRowList * kW4MaxExperts];       // [CTA][token of this CTA][expert]: the cluster's parts of the logits
+    float squares[kMaxCluster][kRowList];       // [CTA][token of this CTA]
+    uint32_t expert[kMaxPairs];                 // the first CTA's: picks of all tokens, likeliest first
+    float weight[kMaxPairs];
+    uint32_t mask[kW4MaxExperts];               // by expert: the tokens that chose it
+    uint16_t before[kW4MaxExperts];             // pairs of the experts before
+    int totals[4][8];
+};
+
+// Writes the lists of the chosen experts, ascending, from the picks of all tokens. RouteScratch::mask is zero before.
+__device__ void write_route(const MoeArgs & a, RouteScratch & p) {
     const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
-    for (int i = e; i < a.T * a.k; i += blockDim.x) {
-        const int t = i / a.k, expert = p.expert[i];
-        atomicOr(&p.mask[expert], 1u << t);
-        p.rank[expert][t] = (uint8_t)(i - t * a.k);
-    }
+    static_assert(kMaxPairs <= 512, "a thread of the routing kernel for every pair");
+    const bool pair = e < a.T * a.k;
+    const int t = e / a.k, own_expert = pair ? p.expert[e] : 0;
+    if (pair) atomicOr(&p.mask[own_expert], 1u << t);
     __syncthreads();
     const uint32_t mask = e < (int)kW4MaxExperts ? p.mask[e] : 0;      // tokens that chose expert e
-    // experts, tokens and sets of the experts before this one: inside the warp, then over the eight warps that hold experts
     const int n = __popc(mask), sets = (n + kSet - 1) / kSet;
-    int sum[3] = {n > 0 ? 1 : 0, n, sets};
+    // chosen experts, pairs, sets and cost before this one: inside the warp, then over the eight warps that hold experts
+    const int own[4] = {n > 0 ? 1 : 0, n, sets, n > 0 ? a.blocks_ff * block_cost(n, a.parts) : 0};
+    int sum[4] = {own[0], own[1], own[2], own[3]};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const int v = __shfl_up_sync(0xffffffffu, sum[i], o);
             if (lane >= o) sum[i] += v;
         }
     }
     if (warp < 8 && lane == 31) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) p.sums[i][warp] = sum[i];
+        for (int i = 0; i < 4; ++i) p.totals[i][warp] = sum[i];
     }
     __syncthreads();
-    int before[3] = {sum[0] - (n > 0), sum[1] - n, sum[2] - sets}, all = 0, all_sets = 0;
-    for (int w = 0; w < 8; ++w) {
-        if (w < warp) { before[0] += p.sums[0][w]; before[1] += p.sums[1][w]; before[2] += p.sums[2][w]; }
-        all += p.sums[0][w];
-        all_sets += p.sums[2][w];
+    int before[4], all[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        before[i] = sum[i] - own[i];
+        all[i] = 0;
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp) before[i] += p.totals[i][w];
+            all[i] += p.totals[i][w];
+        }
     }
     if (mask) {
         const int u = before[0];
-        p.unique[u] = (uint16_t)e;
-        p.count[u] = (uint8_t)n;
-        p.before[u] = (uint16_t)before[1];
-        int i = 0;
-        for (uint32_t m = mask; m; m &= m - 1, ++i) {
-            const uint8_t t = (uint8_t)(__ffs(m) - 1);
-            p.token[u][i] = t;
-            if (meta) meta->token[before[2] + i / kSet][i % kSet] = t;
-        }
-        if (meta) {
-            for (int j = 0; j < sets; ++j) {
-                meta->expert[before[2] + j] = (uint16_t)e;
-                meta->first[before[2] + j] = (uint16_t)(before[1] + kSet * j);
-                meta->count[before[2] + j] = (uint8_t)min(kSet, n - kSet * j);
-            }
+        reinterpret_cast<uint16_t *>(a.route + a.at.expert)[u] = (uint16_t)e;
+        reinterpret_cast<uint16_t *>(a.route + a.at.before)[u] = (uint16_t)before[1];
+        reinterpret_cast<int *>(a.route + a.at.cost)[u] = before[3];
+        p.before[e] = (uint16_t)before[1];
+        for (int j = 0; j < sets; ++j) {
+            reinterpret_cast<uint16_t *>(a.route + a.at.set_expert)[before[2] + j] = (uint16_t)e;
+            reinterpret_cast<uint16_t *>(a.route + a.at.set_first)[before[2] + j] = (uint16_t)(before[1] + kSet * j);
+            a.route[a.at.set_count + before[2] + j] = (uint8_t)min(kSet, n - kSet * j);
         }
     }
     if (e == 0) {
-        p.n = all;
-        if (meta) meta->n = all_sets;
+        reinterpret_cast<uint16_t *>(a.route + a.at.before)[all[0]] = (uint16_t)all[1];
+        reinterpret_cast<int *>(a.route + a.at.cost)[all[0]] = all[3];
+        *reinterpret_cast<int4 *>(a.route) = make_int4(all[0], all[2], 0, 0);
     }
     __syncthreads();
+    if (pair) {                 // an expert's tokens ascend
+        const int i = p.before[own_expert] + __popc(p.mask[own_expert] & ((1u << t) - 1));
+        a.route[a.at.token + i] = (uint8_t)t;
+        reinterpret_cast<float *>(a.route + a.at.weight)[i] = p.weight[e];
+    }
+}
+
+constexpr int kRouteRoom = 64 * 1024;       // the routing kernel's shared memory for tokens
+
+// The routing, by one cluster. A CTA's columns of the tokens are staged as f32; a warp takes four experts and a part of the columns for all
+// tokens, so the router is read once, from memory into registers, the first of it before the tokens are there. What bounds it is latency: a read of the
+// tokens and the router, two meetings of the cluster.
+template <int NT>
+__global__ void __launch_bounds__(512, 1) w4_route_kernel(MoeArgs a) {
+    constexpr int kWarps = 16, EB = 4, kWide = kRouteRoom / (4 * NT) / 128 * 128;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ RouteScratch sc;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), C = (int)cluster_size(), log_c = __ffs(C) - 1;
+    cluster_arrive();
+    float * const xs = reinterpret_cast<float *>(smem);
+    if (threadIdx.x < kW4MaxExperts) sc.mask[threadIdx.x] = 0;
+    pdl_wait();
+    pdl_trigger();          // behind the wait: the next kernel may read what was complete before this one
+    const int k0 = part_begin2(a.d / 32, rank, log_c) * 32, columns = part_begin2(a.d / 32, rank + 1, log_c) * 32 - k0;
+    const int groups = (a.E + EB - 1) / EB;
+    int log_parts = 0;                      // parts of the columns: as many as there are warps for
+    while ((groups << (log_parts + 1)) <= kWarps) ++log_parts;
+    const Act norm{a.norm, 0, GGML_F32, (reinterpret_cast<uintptr_t>(a.norm) & 15) == 0};
+    // columns [from, from + wide) of all tokens at a time
+    for (int from = 0; from < columns; from += kWide) {
+        const int wide = min(kWide, columns - from), chunks = wide / 4;
+        float4 w[EB];
+        auto load_router = [&](int group, int c) {
+#pragma unroll
+            for (int e = 0; e < EB; ++e) {
+                const float * r = a.router + (size_t)min(group * EB + e, a.E - 1) * a.d + k0 + from + c;
+                if (a.router_vec) w[e] = *reinterpret_cast<const float4 *>(r);
+                else w[e] = make_float4(r[0], r[1], r[2], r[3]);
+            }
+        };
+        auto begin = [&](int job) { return part_begin2(chunks, job & ((1 << log_parts) - 1), log_parts) * 4; };
+        auto end = [&](int job) { return part_begin2(chunks, (job & ((1 << log_parts) - 1)) + 1, log_parts) * 4; };
+        const int jobs = groups << log_parts;
+        if (warp < jobs && begin(warp) + lane * 4 < end(warp)) load_router(warp >> log_parts, begin(warp) + lane * 4);
+        if (from > 0) __syncthreads();
+        for (int i = threadIdx.x; i < a.T * chunks; i += kWarps * 32) {
+            const int t = i / chunks, c = (i - t * chunks) * 4;
+            float v[4];
+            widen4(load4<false>(a.x, a.x.type, t, k0 + from + c), a.x.type, v);
+            if (a.norm) {
+                float by[4];
+                widen4(load4<false>(norm, GGML_F32, 0, k0 + from + c), GGML_F32, by);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= by[e];
+            }
+            *reinterpret_cast<float4 *>(xs + t * wide + c) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        __syncthreads();
+        for (int job = warp; job < jobs; job += kWarps) {
+            const int group = job >> log_parts;
+            float acc[EB * NT] = {};
+            for (int c = begin(job) + lane * 4, c_end = end(job), first = job == warp; c < c_end; c += 128, first = 0) {
+                if (!first) load_router(group, c);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float4 v = *reinterpret_cast<const float4 *>(xs + min(t, a.T - 1) * wide + c);
+#pragma unroll
+                    for (int e = 0; e < EB; ++e) acc[e * NT + t] += w[e].x * v.x + w[e].y * v.y + w[e].z * v.z + w[e].w * v.w;
+                }
+            }
+            constexpr int kChunk = EB * NT < 16 ? EB * NT : 16;
+#pragma unroll
+            for (int at = 0; at < EB * NT; at += kChunk) {
+                float v[16] = {};
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) v[i] = acc[at + i];
+                const float sum = warp_sums16(v);
+                const int i = at + (lane >> 1), e = group * EB + i / NT, t = i % NT;
+                float * to = &sc.sums[((job & ((1 << log_parts) - 1)) * a.T + t) * a.E + e];
+                if (!(lane & 1) && (lane >> 1) < kChunk && e < a.E && t < a.T) *to = from > 0 ? *to + sum : sum;
+            }
+        }
+    }
+    if (columns == 0) {
+        for (int i = threadIdx.x; i < (a.T * a.E) << log_parts; i += kWarps * 32) sc.sums[i] = 0.f;
+    }
+    float squares = 0.f;
+    if (a.norm && warp < a.T) {
+        for (int c = lane * 4; c < columns; c += 128) {
+            float v[4];
+            widen4(load4<false>(a.x, a.x.type, warp, k0 + c), a.x.type, v);
+            squares += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    }
+    cluster_wait();
+    __syncthreads();
+    // token t's go to CTA t % C
+    const int of_cta = kRowList >> log_c;
+    if (a.norm && warp < a.T && lane == 0) remote_store(remote_address(smem_address(&sc.squares[rank][warp >> log_c]), warp & (C - 1)), squares);
+    for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) {
+        const int t = i / a.E, e = i - t * a.E;
+        float v = 0.f;
+        for (int part = 0; part < 1 << log_parts; ++part) v += sc.sums[part * a.T * a.E + i];
+        remote_store(remote_address(smem_address(&sc.mail[(rank * of_cta + (t >> log_c)) * a.E + e]), t & (C - 1)), v);
+    }
+    cluster_sync();
+    const int t = warp * C + rank;
+    if (t < a.T) {
+        float rstd = 1.f;
+        if (a.norm) {
+            float ss = 0.f;
+            for (int c = 0; c < C; ++c) ss += sc.squares[c][warp];
+            rstd = rsqrtf(ss / (float)a.d + a.eps);
+        }
+        auto logit = [&](int e) {
+            float v = 0.f;
+            for (int c = 0; c < C; ++c) v += sc.mail[(c * of_cta + warp) * a.E + e];
+            return v * rstd;
+        };
+        int expert;
+        float weight;
+        if (a.E <= 32) pick_experts<1>(logit, a.E, a.k, a.normalise, expert, weight);
+        else if (a.E <= 128) pick_experts<4>(logit, a.E, a.k, a.normalise, expert, weight);
+        else pick_experts<kW4MaxExperts / 32>(logit, a.E, a.k, a.normalise, expert, weight);
+        if (lane < a.k) {
+            const int i = t * a.k + lane;
+            remote_store(remote_address(smem_address(&sc.expert[i]), 0), __uint_as_float((uint32_t)expert));
+            remote_store(remote_address(smem_address(&sc.weight[i]), 0), weight);
+            if (a.ids) a.ids[i] = expert;
+            if (a.weights) a.weights[i] = weight;
+        }
+    }
+    cluster_sync();
+    if (rank == 0) write_route(a, sc);
 }
 
 // Jobs: block j of an expert's gate and of its up matrix are jobs 2 j and 2 j + 1, experts one behind the other.
 template <bool MX, int PARTS, int NT> struct GateUpSource {
     const MoeArgs & a;
-    const Picks & p;
+    const Route & r;
     Staged x;
     Inbox inbox;
     int job0, jobs;
@@ -1163,7 +1277,7 @@ template <bool MX, int PARTS, int NT> struct GateUpSource {
         if (!c.live) return;
         const int job = job0 + c.job, block = job >> 1;
         c.group = block / a.blocks_ff;
-        const int e = p.unique[c.group];
+        const int e = r.expert(c.group);
         c.p = (job & 1 ? a.up + e * a.up_expert : a.gate + e * a.gate_expert) +
               ((size_t)(block - c.group * a.blocks_ff) * a.steps_d + step) * w4_unit_bytes(MX) + (threadIdx.x & 31) * 16;
         c.rem = len;
@@ -1176,18 +1290,18 @@ template <bool MX, int PARTS, int NT> struct GateUpSource {
         c.job += stride;
         point(c);
     }
-    __device__ __forceinline__ Group group(const Cursor & c) const { return {x, p.token[c.group], p.count[c.group]}; }
+    __device__ __forceinline__ Group group(const Cursor & c) const { return {x, r.tokens(r.before(c.group)), r.count(c.group)}; }
     __device__ __forceinline__ uint32_t column(const Cursor & c, int col) const {
         const int job = job0 + c.job;
-        return inbox.slot(round, p.unit(c.group, (job >> 1) - c.group * a.blocks_ff, a.blocks_ff) - unit0 + col, job & 1, sub);
+        return inbox.slot(round, r.unit(c.group, (job >> 1) - c.group * a.blocks_ff, a.blocks_ff) - unit0 + col, job & 1, sub);
     }
 };
 
 // Writes one token's hidden value of column block * 32 + lane (and, behind the last block, zeros up to a whole step).
-__device__ __forceinline__ void put_hidden(const MoeArgs & a, const Picks & p, int u, int col, int block, float v) {
+__device__ __forceinline__ void put_hidden(const MoeArgs & a, const Route & r, int u, int col, int block, float v) {
     const int lane = threadIdx.x & 31;
-    const int set = col / kSet, place = col - set * kSet, nt = min(kSet, p.count[u] - set * kSet);
-    uint8_t * at = a.hidden + ((size_t)(p.before[u] + set * kSet) * a.steps_ff + (size_t)(block >> 2) * nt) * kHiddenBytes;
+    const int set = col / kSet, place = col - set * kSet, nt = min(kSet, r.count(u) - set * kSet);
+    uint8_t * at = a.hidden + ((size_t)(r.before(u) + set * kSet) * a.steps_ff + (size_t)(block >> 2) * nt) * kHiddenBytes;
     const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
     const int shift = shift_for(top);
     const int last = block == a.blocks_ff - 1 ? 3 : block & 3;
@@ -1212,71 +1326,49 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
     constexpr int kWarps = warps_for(NT);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Scratch<kWarps> sc;
-    __shared__ Picks picks;
+    __shared__ __align__(16) uint8_t route_copy[kRouteBytes];
+    __shared__ int range[2];
     const int warp = threadIdx.x >> 5;
     const int rank = (int)cluster_rank(), C = (int)cluster_size(), log_c = __ffs(C) - 1;
     const int cluster = blockIdx.x >> log_c;
     cluster_arrive();
     const int s0 = part_begin2(a.steps_d, rank, log_c), n_steps = part_begin2(a.steps_d, rank + 1, log_c) - s0;
     const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
-    float * mine = reinterpret_cast<float *>(smem + a.x_bytes + a.c_bytes);         // this CTA's part of the logits
-    float * logits = mine + a.logit_bytes / 4;
-    uint8_t * const rings = smem + a.x_bytes + a.c_bytes + 2 * a.logit_bytes;
+    uint8_t * const rings = smem + a.x_bytes + a.c_bytes;
     if (threadIdx.x == 0) sc.zero = 0;
-    if (threadIdx.x < kW4MaxExperts) picks.mask[threadIdx.x] = 0;
 
-    pdl_trigger();
+    // The activations were complete before the routing kernel, which lets this one start behind its own wait; they are read
+    // through the L2 cache only. The norm's weights wait in the rings' first stage.
+    stage_tokens<MX, PARTS>(a.x, a.T, NT, s0 * 128, n_steps, a.d, a.norm, NormRoom{smem_address(rings), (int)(kMoeStages * w4_unit_bytes(MX)), kWarps}, x, sc, rank, C);
     pdl_wait();
-    const int k0 = s0 * 128, k1 = min(a.d, (s0 + n_steps) * 128);
-    // the rings and the first inbox are idle until the experts are known
-    const int idle = ring_bytes(MX, NT, kMoeStages) + a.inbox;
-    fetch_router(a, k0, min(k1 - k0, router_columns(a.E, idle)), rings);
-    copies_commit();
-    stage_tokens<MX, PARTS>(a.x, a.T, NT, k0, n_steps, a.d, a.norm, NormRoom{0, 0, 0}, x, sc, rank, C);
+    pdl_trigger();          // behind the wait: the next kernel may read the route
+    const Route route{route_copy, a.at};
+    copy_route(a.route, route_copy, a.at.expert, a.at.set_expert);
     __syncthreads();
-    partial_logits<MX, PARTS, NT, kWarps>(a, k0, k1, x, rings, idle, mine);
-    // Out of the activations' scale (a token's factor without the weights' constant) and to every CTA of the cluster: into its second
-    // inbox, which nobody else writes before the cluster has met after the first round, where that has room.
+    // The cluster's blocks: those whose cost begins in its share of the whole cost.
+    if (threadIdx.x < 2) range[threadIdx.x] = 0;
     __syncthreads();
-    const int n_logits = a.T * a.E;
-    const uint32_t mail = smem_address(rings) + ring_bytes(MX, NT, kMoeStages) + a.inbox;
-    const bool posted = C * n_logits * 4 <= a.inbox;
-    for (int i = threadIdx.x; i < n_logits; i += kWarps * 32) {
-        const float v = mine[i] * (sc.factor[i / a.E] * power(-weight_shift(MX)));
-        if (posted) {
-            for (int c = 0; c < C; ++c) remote_store(remote_address(mail + (rank * n_logits + i) * 4, c), v);
-        } else {
-            mine[i] = v;
+    {
+        const int u = threadIdx.x, n = route.experts();
+        if (u < n) {
+            const int64_t all = route.cost(n);
+            const int from = route.cost(u), to = route.cost(u + 1), each = (to - from) / a.blocks_ff;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int point = (int)(all * (cluster + i) / a.clusters);
+                if (from < point && point <= to) range[i] = u * a.blocks_ff + (point - from + each - 1) / each;
+            }
         }
     }
-    cluster_sync();
-    for (int i = threadIdx.x; i < n_logits; i += kWarps * 32) {
-        float v = 0.f;
-        for (int c = 0; c < C; ++c) v += posted ? shared_f1(mail + (c * n_logits + i) * 4) : remote_load(remote_address(smem_address(mine + i), c));
-        logits[i] = a.norm ? v * rms_factor(sc, i / a.E, C, a.d, a.eps) : v;
-    }
-    if (threadIdx.x < a.T) picks.rstd[threadIdx.x] = a.norm ? rms_factor(sc, threadIdx.x, C, a.d, a.eps) : 1.f;
     __syncthreads();
-    for (int t = warp; t < a.T; t += kWarps) pick_experts(logits + t * a.E, a.E, a.k, a.normalise, picks.expert + t * a.k, picks.weight + t * a.k);
-    __syncthreads();
-    const bool first = blockIdx.x == 0;
-    group_picks(a, picks, first ? a.meta : nullptr);
-    if (first) {
-        for (int i = threadIdx.x; i < a.T * a.k; i += kWarps * 32) {
-            if (a.ids) a.ids[i] = picks.expert[i];
-            if (a.weights) a.weights[i] = picks.weight[i];
-        }
-    }
-
-    const int total = picks.n * a.blocks_ff;
-    const int b_begin = part_begin(total, cluster, a.clusters), blocks = part_begin(total, cluster + 1, a.clusters) - b_begin;
+    const int b_begin = range[0], blocks = range[1] - b_begin;
     // parts of the columns: no more than the inbox has room for with every token at one expert
     const int ks = split_columns(blocks * 2, a.steps_d >> log_c, kWarps, (int)(a.inbox / inbox_bytes(a.T, C, 1, 2))), log_ks = __ffs(ks) - 1;
     const int room = (a.inbox >> (log_c + log_ks + 8)) << log_c;        // units of a round
     const int sub = warp & (ks - 1), step = part_begin2(n_steps, sub, log_ks), len = part_begin2(n_steps, sub + 1, log_ks) - step;
     const Staged x_warp{x.x + step * step_x_bytes(PARTS, NT), x.c + step * step_c_bytes(MX, NT) / 4};
     const Inbox inbox{smem_address(rings + ring_bytes(MX, NT, kMoeStages)), a.inbox, rank, log_c, ks, 2};
-    GateUpSource<MX, PARTS, NT> src{a, picks, x_warp, inbox, 2 * b_begin, 2 * blocks, warp >> log_ks, kWarps >> log_ks, sub, s0 + step, len, 0, 0};
+    GateUpSource<MX, PARTS, NT> src{a, route, x_warp, inbox, 2 * b_begin, 2 * blocks, warp >> log_ks, kWarps >> log_ks, sub, s0 + step, len, 0, 0};
     Stream<MX, kMoeStages, GateUpSource<MX, PARTS, NT>> stream(src, rings);
     stream.prefetch();
     int u = b_begin / a.blocks_ff, block = b_begin - u * a.blocks_ff;       // where the round begins
@@ -1285,7 +1377,7 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
         const int u0 = u, block0 = block;
         int now = 0, units = 0;
         while (b0 + now < blocks) {
-            const int n = picks.count[u], more = min(min(a.blocks_ff - block, blocks - b0 - now), (room - units) / n);
+            const int n = route.count(u), more = min(min(a.blocks_ff - block, blocks - b0 - now), (room - units) / n);
             now += more;
             units += more * n;
             block += more;
@@ -1293,31 +1385,31 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
             ++u;
             block = 0;
         }
-        src.unit0 = picks.unit(u0, block0, a.blocks_ff);
+        src.unit0 = route.unit(u0, block0, a.blocks_ff);
         stream.template work<PARTS, NT, (NT > 1)>(sc, 2 * (b0 + now));
         cluster_sync();
         int v_u = u0;
         for (int i = warp; i * C + rank < units; i += kWarps) {
             const int unit = src.unit0 + i * C + rank;
-            while (v_u + 1 < picks.n && unit >= picks.unit(v_u + 1, 0, a.blocks_ff)) ++v_u;
-            const int n = picks.count[v_u], at = unit - picks.unit(v_u, 0, a.blocks_ff), b = at / n, col = at - b * n;
-            const int t = picks.token[v_u][col];
-            const float v = inbox.sum(src.round, i, 0) * picks.rstd[t], up = inbox.sum(src.round, i, 1) * picks.rstd[t];
-            put_hidden(a, picks, v_u, col, b, picks.weight[t * a.k + picks.rank[picks.unique[v_u]][t]] * (v / (1.f + expf(-v)) * up));
+            while (v_u + 1 < route.experts() && unit >= route.unit(v_u + 1, 0, a.blocks_ff)) ++v_u;
+            const int n = route.count(v_u), at = unit - route.unit(v_u, 0, a.blocks_ff), b = at / n, col = at - b * n, pair = route.before(v_u) + col;
+            const float rstd = a.norm ? rms_factor(sc, *route.tokens(pair), C, a.d, a.eps) : 1.f;
+            const float v = inbox.sum(src.round, i, 0) * rstd, up = inbox.sum(src.round, i, 1) * rstd;
+            put_hidden(a, route, v_u, col, b, route.weight(pair) * (v / (1.f + expf(-v)) * up));
         }
         b0 += now;
     }
-    if (blocks == 0) cluster_sync();        // nobody leaves while its logits are read
+    if (blocks == 0) cluster_sync();        // nobody leaves while the squares of its rows are on their way
 }
 
-// The second kernel's stream: as Stream, but a unit comes with the hidden columns it multiplies. Weights run two units ahead, hidden
+// The third kernel's stream: as Stream, but a unit comes with the hidden columns it multiplies. Weights run two units ahead, hidden
 // columns one.
 template <bool MX, int MOST> struct DownStream {
-    static constexpr int kStages = 3;
+    static constexpr int kWarps = MOST > 1 ? 16 : 8, kStages = 3;
     static constexpr uint32_t kUnit = w4_unit_bytes(MX), kHidden = MOST * kHiddenBytes;
-    static constexpr int kRingBytes = 8 * (kStages * (int)kUnit + 2 * (int)kHidden);
+    static constexpr int kRingBytes = kWarps * (kStages * (int)kUnit + 2 * (int)kHidden);
     const MoeArgs & a;
-    const MoeMeta & meta;
+    const Route & r;
     const int lane;
     const uint32_t weights;             // the warp's rings
     uint8_t * const hidden;
@@ -1330,9 +1422,9 @@ template <bool MX, int MOST> struct DownStream {
     } w, h, c;
     uint32_t fill, h_fill, at, h_at;
 
-    __device__ __forceinline__ DownStream(const MoeArgs & args, const MoeMeta & m, uint8_t * rings, int f, int t, int j0, int j, int first, int step)
-        : a(args), meta(m), lane(threadIdx.x & 31), weights(smem_address(rings) + (threadIdx.x >> 5) * (kStages * kUnit)),
-          hidden(rings + 8 * kStages * kUnit + (threadIdx.x >> 5) * (2 * kHidden)), from(f), to(t), job0(j0), jobs(j), stride(step),
+    __device__ __forceinline__ DownStream(const MoeArgs & args, const Route & route, uint8_t * rings, int f, int t, int j0, int j, int first, int step)
+        : a(args), r(route), lane(threadIdx.x & 31), weights(smem_address(rings) + (threadIdx.x >> 5) * (kStages * kUnit)),
+          hidden(rings + kWarps * kStages * kUnit + (threadIdx.x >> 5) * (2 * kHidden)), from(f), to(t), job0(j0), jobs(j), stride(step),
           fill(0), h_fill(0), at(0), h_at(0) {
         w.live = from < to && first < jobs;
         w.job = first;
@@ -1348,11 +1440,11 @@ template <bool MX, int MOST> struct DownStream {
     }
     __device__ __forceinline__ int left(const Place & p) const { return min(to, (p.set + 1) * a.steps_ff) - p.at; }
     __device__ __forceinline__ void point_weights() {
-        w.p = a.down + meta.expert[w.set] * a.down_expert + ((size_t)(job0 + w.job) * a.steps_ff + (w.at - w.set * a.steps_ff)) * kUnit + lane * 16;
+        w.p = a.down + r.set_expert(w.set) * a.down_expert + ((size_t)(job0 + w.job) * a.steps_ff + (w.at - w.set * a.steps_ff)) * kUnit + lane * 16;
         w.left = left(w);
     }
     __device__ __forceinline__ void point_hidden() {
-        h.p = a.hidden + ((size_t)meta.first[h.set] * a.steps_ff + (size_t)(h.at - h.set * a.steps_ff) * meta.count[h.set]) * kHiddenBytes + lane * 16;
+        h.p = a.hidden + ((size_t)r.set_first(h.set) * a.steps_ff + (size_t)(h.at - h.set * a.steps_ff) * r.set_count(h.set)) * kHiddenBytes + lane * 16;
         h.left = left(h);
     }
     // To the next run: the next set of the job, or the next job from the beginning.
@@ -1384,7 +1476,7 @@ template <bool MX, int MOST> struct DownStream {
     __device__ __forceinline__ void fetch_hidden() {
         if (h.live) {
             const uint32_t dst = smem_address(hidden) + h_fill + lane * 16;
-            const int chunks = meta.count[h.set] * (kHiddenBytes / 16);
+            const int chunks = r.set_count(h.set) * (kHiddenBytes / 16);
 #pragma unroll
             for (int i = 0; i < (MOST * (kHiddenBytes / 16) + 31) / 32; ++i) if (lane + 32 * i < chunks) copy16(dst + i * 512, h.p + i * 512);
             h.p += chunks * 16;
@@ -1396,10 +1488,14 @@ template <bool MX, int MOST> struct DownStream {
         h_fill ^= kHidden;              // one stage or the other
         copies_commit();
     }
+    // The first two units' weights, and with `begin` the first one's hidden columns: the loop finds all of them older than one group of copies.
     __device__ __forceinline__ void prefetch() {
         fetch_weights();
-        fetch_hidden();
         fetch_weights();
+    }
+    __device__ __forceinline__ void begin() {
+        fetch_hidden();
+        copies_commit();
     }
     template <int NT, class Column> __device__ __forceinline__ void work_run(Column column) {
         float acc[2][2][4] = {};
@@ -1422,8 +1518,8 @@ template <bool MX, int MOST> struct DownStream {
     // slot(job, token): where 32 rows' sums are added up
     template <class Slot> __device__ __forceinline__ void work(Slot slot) {
         while (c.live) {
-            const int n = meta.count[c.set];
-            auto column = [&](int col) { return slot(c.job, meta.token[c.set][col]); };
+            const int n = r.set_count(c.set);
+            auto column = [&](int col) { return slot(c.job, *r.tokens(r.set_first(c.set) + col)); };
             if (n == 1) work_run<1>(column);
             if constexpr (MOST > 1) if (n == 2) work_run<2>(column);
             if constexpr (MOST > 2) if (n == 3) work_run<3>(column);
@@ -1434,10 +1530,10 @@ template <bool MX, int MOST> struct DownStream {
 };
 
 template <bool MX, int MOST>
-__global__ void __launch_bounds__(256, MOST > 1 ? 2 : 3) w4_moe_down_kernel(MoeArgs a) {
-    constexpr int kWarps = 8;
+__global__ void __launch_bounds__(DownStream<MX, MOST>::kWarps * 32, MOST > 1 ? 1 : 3) w4_moe_down_kernel(MoeArgs a) {
+    constexpr int kWarps = DownStream<MX, MOST>::kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ MoeMeta meta;
+    __shared__ __align__(16) uint8_t route_copy[kRouteBytes];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), C = (int)cluster_size(), log_c = __ffs(C) - 1;
     const int cluster = blockIdx.x >> log_c;
@@ -1446,34 +1542,25 @@ __global__ void __launch_bounds__(256, MOST > 1 ? 2 : 3) w4_moe_down_kernel(MoeA
     const Inbox inbox{smem_address(partial) + a.partial, a.inbox, rank, log_c, 1, 1};
     const int j_begin = part_begin(a.blocks_d, cluster, a.clusters), j_end = part_begin(a.blocks_d, cluster + 1, a.clusters);
     pdl_trigger();
-    pdl_wait();
-    {
-        // the lists as long as they can be, in 16-byte words, every one by a thread of its own; what lies behind the last set is not used
-        const int sets = min(kMaxSets, (a.T * a.k + 15) / 16 * 16);
-        const int n_expert = 1 + sets / 8, n_first = n_expert + sets / 8, n_count = n_first + sets / 16, n_token = n_count + sets / 4;
-        const int4 * from = reinterpret_cast<const int4 *>(a.meta);
-        int4 * to = reinterpret_cast<int4 *>(&meta);
-        for (int i = threadIdx.x; i < n_token; i += kWarps * 32) {
-            const int at = i == 0 ? 0
-                : i < n_expert ? (int)offsetof(MoeMeta, expert) / 16 + i - 1
-                : i < n_first ? (int)offsetof(MoeMeta, first) / 16 + i - n_expert
-                : i < n_count ? (int)offsetof(MoeMeta, count) / 16 + i - n_first : (int)offsetof(MoeMeta, token) / 16 + i - n_count;
-            to[at] = from[at];
-        }
-    }
-    cluster_wait();
+    // the kernel before this one lets it start when the route is there
+    const Route route{route_copy, a.at};
+    copy_route(a.route, route_copy, a.at.token, a.at.bytes);
     __syncthreads();
-    const int total = meta.n * a.steps_ff;          // the sets' columns, one behind the other
+    const int total = route.sets() * a.steps_ff;    // the sets' columns, one behind the other
     const int begin = part_begin2(total, rank, log_c), n = part_begin2(total, rank + 1, log_c) - begin;
-    const int ks = a.ks, log_ks = __ffs(ks) - 1;
-    const int sub = warp & (ks - 1);
+    const int ks = a.ks, first = warp / ks, sub = warp - first * ks, stride = kWarps / ks;
     int round = 0;
     for (int j0 = j_begin; j0 < j_end; j0 += a.per_round, ++round) {
         const int jobs = min(a.per_round, j_end - j0);
-        DownStream<MX, MOST> stream(a, meta, smem, begin + part_begin2(n, sub, log_ks), begin + part_begin2(n, sub + 1, log_ks), j0, jobs, warp >> log_ks,
-                                    kWarps >> log_ks);
+        DownStream<MX, MOST> stream(a, route, smem, begin + part_begin(n, sub, ks), begin + part_begin(n, sub + 1, ks), j0,
+                                    first < stride ? jobs : 0, first, stride);
         stream.prefetch();
         for (int i = threadIdx.x; i < jobs * ks * a.T * kSlotCol; i += kWarps * 32) partial[i] = 0.f;
+        if (round == 0) {
+            pdl_wait();         // the hidden columns
+            cluster_wait();
+        }
+        stream.begin();
         __syncthreads();
         stream.work([&](int job, int token) { return partial + ((job * ks + sub) * a.T + token) * kSlotCol; });
         __syncthreads();
@@ -1625,10 +1712,20 @@ template <bool MX> cudaError_t launch_gate_up_of(const MoeArgs & a, int parts, i
     return with_room(nt, [&](auto n) { return launch_gate_up<MX, 1, decltype(n)::value>(a, C, smem, stream); });
 }
 
+cudaError_t launch_route(const MoeArgs & a, cudaStream_t stream) {
+    return with_room(product_room(a.T), [&](auto n) {
+        constexpr int nt = decltype(n)::value;
+        static PerDeviceOnce once;
+        const cudaError_t e = once.first() ? cudaFuncSetAttribute(w4_route_kernel<nt>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteRoom) : cudaSuccess;
+        const int columns = (a.d / 32 + kMaxCluster - 1) / kMaxCluster * 32;        // of a CTA, at most
+        return e != cudaSuccess ? e : launch_cluster(w4_route_kernel<nt>, kMaxCluster, 512, kMaxCluster, (size_t)std::min(kRouteRoom, columns * 4 * a.T), stream, a);
+    });
+}
+
 template <bool MX, int MOST> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
     static PerDeviceOnce once;
     const cudaError_t e = allow_smem(once, w4_moe_down_kernel<MX, MOST>);
-    return e != cudaSuccess ? e : launch_cluster(w4_moe_down_kernel<MX, MOST>, a.clusters * C, 256, C, smem, stream, a);
+    return e != cudaSuccess ? e : launch_cluster(w4_moe_down_kernel<MX, MOST>, a.clusters * C, DownStream<MX, MOST>::kWarps * 32, C, smem, stream, a);
 }
 
 const void * row_at(const void * p, uint32_t type, int64_t ld, int64_t row) {
@@ -1682,8 +1779,8 @@ struct Cut {
 // Chooses the cluster size for `blocks` row blocks of `per` matrices and `steps` column steps whose activations take `each` bytes of
 // shared memory a step. The estimate is in clocks: the weight stream at the SM's share of the memory bandwidth, but no faster
 // than the busiest SM's warps get through it or than its copies in flight allow; the conversion of the CTA's share of the activations; the sums it
-// receives; and a barrier for every round its inbox allows. `step_clocks` is what else a column step costs a CTA.
-Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int stages, int most_resident, int least_c, int most_c, int fixed, double step_clocks, int sms) {
+// receives; and a barrier for every round its inbox allows.
+Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int stages, int most_resident, int least_c, int most_c, int fixed, int sms) {
     Cut best;
     const int warps = warps_for(n), ring = ring_bytes(mx, n, stages), unit = (int)w4_unit_bytes(mx);
     for (int C = least_c; C <= most_c && C <= steps; C *= 2) {
@@ -1703,7 +1800,7 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int sta
         const double in_flight = (double)c.clusters * C * warps * (stages - 1) * unit;
         const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms) * std::max(1.0, 13e6 / in_flight),     // two microseconds of latency under load
                                         (double)busy * runs * warps * ((s + ks - 1) / ks + (n > 8 ? 0.6 : 0.3)) * unit_clocks});
-        const double convert = busy * s * (n * 128 * 0.1 + step_clocks) + 800, sums = busy * (double)blocks_each * per * n * (6 + 2 * C * ks);
+        const double convert = busy * s * n * 128 * 0.1 + 800, sums = busy * (double)blocks_each * per * n * (6 + 2 * C * ks);
         const int64_t room = std::min(kSmShare / c.resident - 4096, kMaxSmem) - fixed - ring - (int64_t)s * each;
         const double rounds = std::ceil((double)inbox_bytes((int64_t)blocks_each * n, C, ks, per) / std::max<int64_t>(room, 1024));
         c.cost = stream + convert + sums / 4 + (rounds > 1 ? 2 * rounds : 1) * 1500;
@@ -1727,7 +1824,7 @@ Cut product_cut(int blocks, int per, int steps, bool mx, int parts, int & n) {
     if (!std::equal(key, key + 7, k.key)) {
         for (k.n = n;; k.n = (k.n + 1) / 2) {
             const int room = product_room(k.n);
-            k.cut = choose_cut(blocks, per, steps, k.n, step_bytes(mx, parts, room), mx, stages_for(k.n, parts), resident_for(room), 1, kMaxCluster, 0, 0, device_sms());
+            k.cut = choose_cut(blocks, per, steps, k.n, step_bytes(mx, parts, room), mx, stages_for(k.n, parts), resident_for(room), 1, kMaxCluster, 0, device_sms());
             if (k.cut.C || k.n == 1) break;
         }
         std::copy(key, key + 7, k.key);
@@ -1812,32 +1909,104 @@ cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {
     return cudaSuccess;
 }
 
+// Workspace in front of the hidden columns.
+static size_t route_room(size_t pairs) { return (route_at((int)std::min<size_t>(pairs, kW4MaxExperts), (int)pairs).bytes + 255) / 256 * 256; }
+
 size_t w4_moe_workspace_bytes(uint32_t ff, uint32_t n_tokens, uint32_t n_used) {
     const size_t pairs = (size_t)std::min<uint32_t>(n_tokens, kW4PassTokens) * n_used;
-    return (sizeof(MoeMeta) + 255) / 256 * 256 + pairs * ((ff + 127) / 128) * kHiddenBytes;
+    return route_room(pairs) + pairs * ((ff + 127) / 128) * kHiddenBytes;
 }
+
+namespace {
+
+constexpr int kMoeStatic = 9 * 1024;        // static shared memory of the second kernel, rounded up: the route and what stage_tokens needs
+
+// How the second and third kernel of a pass over n tokens are cut.
+struct MoePlan {
+    int n = 0;
+    Cut cut;
+    int C = 0, clusters = 0, ks = 0, per_round = 0, inbox = 0, partial = 0;
+    size_t smem = 0;
+};
+
+MoePlan make_moe_plan(int E, int used, int blocks_ff, int steps_d, int blocks_d, int steps_ff, bool mx, bool mx_down, int parts, int n) {
+    MoePlan m;
+    // Second kernel: n tokens that choose independently choose about `reach` experts. It runs in clusters of four (one token, 32 experts of
+    // 2880 x 2880: 32 us the layer, 38 us with eight; sixteen tokens: 147 us, 150 us), of eight where rows are so long that four cannot hold them.
+    for (;; n = (n + 1) / 2) {
+        const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)used / E, n)))), room = product_room(n);
+        const int least_c = std::min(4, steps_d < 2 ? 1 : steps_d < 4 ? 2 : 4);
+        for (int C = least_c; !m.cut.C && C <= kMaxCluster; C *= 2)
+            m.cut = choose_cut(reach * blocks_ff, 2, steps_d, n, step_bytes(mx, parts, room), mx, kMoeStages, room > 4 ? 1 : 2, C, C, kMoeStatic, device_sms());
+        if (m.cut.C || n == 1) break;
+    }
+    m.n = n;
+    if (!m.cut.C) return m;
+    // Third kernel, in clusters of four: eight would leave a warp two units of a run at one token. One token: three CTAs of eight warps on an SM;
+    // several: one of sixteen, whose partial sums share the room better (sixteen tokens: 124 us the layer, 135 us with two of eight).
+    m.C = 4;
+    while (m.C > steps_ff * used) m.C /= 2;
+    const int resident = n > 1 ? 1 : 3, warps = n > 1 ? 16 : 8;
+    const int most = resident_clusters(log2_of(m.C), resident, warps * 32), per = (blocks_d + most - 1) / most;
+    m.clusters = (blocks_d + per - 1) / per;
+    const int slot = n * kSlotCol * 4;
+    const int rings = mx_down ? (n > 1 ? DownStream<true, kSet>::kRingBytes : DownStream<true, 1>::kRingBytes)
+                              : (n > 1 ? DownStream<false, kSet>::kRingBytes : DownStream<false, 1>::kRingBytes);
+    // A slot for every (block, part of the columns) of a round, and an inbox for its blocks, two where there are several rounds. A
+    // round's end costs about as much as five steps.
+    const int left = std::min(kSmShare / resident - 8 * 1024, kMaxSmem) - rings, steps = std::max(1, n * used * steps_ff / m.C);
+    int64_t least = INT64_MAX;
+    for (int rounds = 1, found = 0; found < 4 && rounds <= per; ++rounds) {
+        const int blocks = (per + rounds - 1) / rounds, many = rounds > 1 ? 2 : 1;
+        const int64_t inbox = inbox_bytes((int64_t)blocks * n, m.C, 1, 1), fit = (left - many * inbox) / ((int64_t)blocks * slot);
+        if (fit < 1) continue;
+        int cost;
+        const int ks = divide_columns(blocks, steps, warps, (int)std::min<int64_t>(fit, warps), cost);
+        ++found;
+        if ((int64_t)rounds * (cost + 10) < least) {
+            least = (int64_t)rounds * (cost + 10);
+            m.per_round = blocks;
+            m.ks = ks;
+            m.inbox = (int)inbox;
+            m.partial = blocks * ks * slot;
+            m.smem = (size_t)rings + m.partial + many * (size_t)inbox;
+        }
+    }
+    if (!m.smem) m.cut.C = 0;
+    return m;
+}
+
+// The same, remembered by the sizes it depends on.
+MoePlan moe_plan(const W4Moe & p, bool mx, bool mx_down, int parts, int n) {
+    struct Known {
+        int key[11] = {};
+        MoePlan plan;
+    };
+    thread_local Known known[16];
+    int device = 0;
+    cudaGetDevice(&device);
+    const int key[11] = {(int)p.gate.n_expert, p.n_used, (int)p.gate.blocks, (int)p.gate.steps, (int)p.down.blocks, (int)p.down.steps, mx, mx_down, parts, n, device + 1};
+    Known & k = known[((unsigned)key[0] + (unsigned)key[2] * 31 + (unsigned)key[3] * 7 + (unsigned)n * 3) % 16];
+    if (!std::equal(key, key + 11, k.key)) {
+        k.plan = make_moe_plan(key[0], key[1], key[2], key[3], key[4], key[5], mx, mx_down, parts, n);
+        std::copy(key, key + 11, k.key);
+    }
+    return k.plan;
+}
+
+} // namespace
 
 cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
     const bool mx = p.gate.type == GGML_MXFP4, mx_down = p.down.type == GGML_MXFP4;
     const int parts = p.x_type == GGML_F32 || p.norm ? 2 : 1;
-    const int sms = device_sms();
     const int E = (int)p.gate.n_expert, d = (int)p.gate.n_in, ff = (int)p.gate.n_out;
     const int steps_d = (int)p.gate.steps, steps_ff = (int)p.down.steps;
-    constexpr int kStatic = 16 * 1024;          // the routing tables
     for (int t0 = 0, n = 0; t0 < p.n_tokens; t0 += n) {
         n = std::min(kW4PassTokens, p.n_tokens - t0);
-        // first kernel: n tokens that choose independently choose about `reach` experts. It runs in clusters of four (one token, 32 experts of
-        // 2880 x 2880: 33 us the layer, 39 us with eight; sixteen tokens: 147 us, 181 us with two), of eight where rows are so long
-        // that four cannot hold them.
-        Cut cut;
-        for (;; n = (n + 1) / 2) {
-            const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)p.n_used / E, n))));
-            const int least_c = std::min(4, steps_d < 2 ? 1 : steps_d < 4 ? 2 : 4);
-            for (int C = least_c; !cut.C && C <= kMaxCluster; C *= 2) cut = choose_cut(reach * (int)p.gate.blocks, 2, steps_d, n, step_bytes(mx, parts, product_room(n)), mx, kMoeStages, product_room(n) > 4 ? 1 : 2, C, C,
-                             2 * up_to(n * E * 4, 128) + kStatic, n * E * 0.4 + E * 4.0, sms);
-            if (cut.C || n == 1) break;
-        }
-        if (!cut.C) return cudaErrorInvalidValue;
+        const MoePlan plan = moe_plan(p, mx, mx_down, parts, n);
+        if (!plan.cut.C) return cudaErrorInvalidValue;      // rows this long are refused when the handle is made
+        n = plan.n;
+        const Cut & cut = plan.cut;
         MoeArgs a{};
         a.gate = p.gate.units;
         a.up = p.up.units;
@@ -1868,46 +2037,30 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         a.ld_y = p.ld_y;
         a.ids = p.ids ? p.ids + (size_t)t0 * p.n_used : nullptr;
         a.weights = p.weights ? p.weights + (size_t)t0 * p.n_used : nullptr;
-        a.meta = static_cast<MoeMeta *>(p.workspace);
-        a.hidden = static_cast<uint8_t *>(p.workspace) + (sizeof(MoeMeta) + 255) / 256 * 256;
+        a.parts = parts;
+        a.at = route_at(std::min(E, n * p.n_used), n * p.n_used);
+        a.route = static_cast<uint8_t *>(p.workspace);
+        a.hidden = a.route + route_room((size_t)n * p.n_used);
 
         const int nt = product_room(n), s = (steps_d + cut.C - 1) / cut.C;
         a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
-        a.logit_bytes = up_to(n * E * 4, 128);
         a.clusters = cut.clusters;
-        const int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx, nt, kMoeStages);
-        a.inbox = (int)std::max<int64_t>((std::min(kSmShare / cut.resident - kStatic - 4096, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, cut.C, 1, 2));
-        cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream)
+        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx, nt, kMoeStages);
+        a.inbox = (int)std::max<int64_t>((std::min(kSmShare / cut.resident - kMoeStatic - 4096, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, cut.C, 1, 2));
+        cudaError_t e = launch_route(a, stream);
+        if (e != cudaSuccess) return e;
+        e = mx ? launch_gate_up_of<true>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream)
                            : launch_gate_up_of<false>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream);
         if (e != cudaSuccess) return e;
 
-        // second kernel
-        int C = 4;                      // eight would leave a warp two units of a run at one token
-        while (C > steps_ff * p.n_used) C /= 2;
-        const int resident = n > 1 ? 2 : 3;
-        const int most = resident_clusters(log2_of(C), resident, 256), per = (a.blocks_d + most - 1) / most;
-        a.clusters = (a.blocks_d + per - 1) / per;
-        const int slot = n * kSlotCol * 4;
-        const int rings = mx_down ? (n > 1 ? DownStream<true, kSet>::kRingBytes : DownStream<true, 1>::kRingBytes)
-                                  : (n > 1 ? DownStream<false, kSet>::kRingBytes : DownStream<false, 1>::kRingBytes);
-        // a slot for every (block, part of the columns), in one round if all blocks have room, with an inbox for each of two rounds else
-        const int left = kSmShare / resident - 8 * 1024 - rings;
-        const int whole = (int)inbox_bytes((int64_t)std::min(per, 64) * n, C, 1, 1);
-        const int slots = std::min(8 * per, std::max(8, (left - whole) / slot));
-        int rounds_inboxes = 1;
-        if (per <= slots && per <= 64) {
-            a.per_round = per;
-            a.ks = split_columns(per, std::max(1, n * p.n_used * steps_ff / C), 8, slots / per);
-            a.inbox = whole;
-        } else {
-            a.per_round = std::min(slots, 64);
-            a.ks = 1;
-            a.inbox = (int)inbox_bytes((int64_t)a.per_round * n, C, 1, 1);
-            rounds_inboxes = 2;
-        }
-        a.partial = a.per_round * a.ks * slot;
-        const size_t smem = (size_t)rings + a.partial + rounds_inboxes * (size_t)a.inbox;
+        a.clusters = plan.clusters;
+        a.ks = plan.ks;
+        a.per_round = plan.per_round;
+        a.inbox = plan.inbox;
+        a.partial = plan.partial;
+        const int C = plan.C;
+        const size_t smem = plan.smem;
         if (mx_down) e = n > 1 ? launch_down<true, kSet>(a, C, smem, stream) : launch_down<true, 1>(a, C, smem, stream);
         else e = n > 1 ? launch_down<false, kSet>(a, C, smem, stream) : launch_down<false, 1>(a, C, smem, stream);
         if (e != cudaSuccess) return e;
