@@ -1931,11 +1931,13 @@ struct MoePlan {
 
 MoePlan make_moe_plan(int E, int used, int blocks_ff, int steps_d, int blocks_d, int steps_ff, bool mx, bool mx_down, int parts, int n) {
     MoePlan m;
-    // Second kernel: n tokens that choose independently choose about `reach` experts. It runs in clusters of four (one token, 32 experts of
-    // 2880 x 2880: 32 us the layer, 38 us with eight; sixteen tokens: 147 us, 150 us), of eight where rows are so long that four cannot hold them.
+    // Second kernel: n tokens that choose independently choose about `reach` experts. Up to four tokens it runs in clusters of four (one token, 32 experts of
+    // 2880 x 2880: 29.4 us the layer, 30.1 us with two and 29.5 with eight), more in clusters of two, which fill the SMs better (64 experts of
+    // 1024 x 2048, six tokens: 47.6 us, 50.0 us with four; the former layer, sixteen tokens: 119.5 us with either), of more where rows are so long that
+    // these cannot hold them.
     for (;; n = (n + 1) / 2) {
         const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)used / E, n)))), room = product_room(n);
-        const int least_c = std::min(4, steps_d < 2 ? 1 : steps_d < 4 ? 2 : 4);
+        const int least_c = steps_d < 2 ? 1 : steps_d < 4 || n > 4 ? 2 : 4;
         for (int C = least_c; !m.cut.C && C <= kMaxCluster; C *= 2)
             m.cut = choose_cut(reach * blocks_ff, 2, steps_d, n, step_bytes(mx, parts, room), mx, kMoeStages, room > 4 ? 1 : 2, C, C, kMoeStatic, device_sms());
         if (m.cut.C || n == 1) break;
