@@ -1786,7 +1786,7 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int sta
     for (int C = least_c; C <= most_c && C <= steps; C *= 2) {
         const int s = (steps + C - 1) / C;
         const int64_t smem = (int64_t)s * each + ring + fixed + 2 * inbox_bytes(n, C, 1, per) + 4096;
-        if (smem > kMaxSmem) continue;
+        if (smem - fixed - 4096 + 256 > kMaxSmem || smem > kSmShare) continue;      // `fixed` is static, and the parts are rounded up
         Cut c;
         c.C = C;
         c.resident = (int)std::min<int64_t>(most_resident, kSmShare / smem);

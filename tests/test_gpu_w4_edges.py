@@ -325,6 +325,29 @@ def test_in_place_expert_layer(rb, weights):
             assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("kind,d,ff,tokens", [(Q4_0, 65536, 64, 16), (MXFP4, 65536, 64, 3), (MXFP4, 262144, 32, 16), (Q4_0, 262144, 32, 1), (Q4_0, 64, 65536, 16), (MXFP4, 4096, 8192, 5)])
+def test_expert_layer_of_long_rows(rb, kind, d, ff, tokens):
+    """Columns that the routing takes in pieces, and passes of fewer tokens where sixteen rows do not fit. Bounds as in test_moe_against_float64."""
+    import torch
+
+    rng = np.random.default_rng(d + ff)
+    E, k = 3, 2
+    raws, x, router = moe_inputs(rng, torch, kind, kind, E, d, ff, tokens, "f32")
+    gate, up, down = bank(rb, raws, (kind, kind), E, d, ff)
+    norm = rng.normal(1, 0.2, d).astype(np.float32)
+    ids = torch.zeros(tokens, k, dtype=torch.int32, device="cuda")
+    y = rb.w4_moe(torch.tensor(router).cuda(), gate, up, down, x, k, norm=torch.tensor(norm).cuda(), ids=ids).double().cpu().numpy()
+    xn = normed(x.double().cpu().numpy(), norm.astype(np.float64), 1e-5)
+    order, p, gap = route64(xn, router.astype(np.float64), k, False)
+    chosen = ids.cpu().numpy().astype(np.int64)
+    clear = gap > 4e-5
+    assert clear.any() and np.array_equal(chosen[clear], order[clear, :k])
+    banks = [[decode(kind, r) for r in b] for b in raws]
+    want, bound = moe64(xn, p, chosen, *banks, False)
+    bound = bound + 4e-5 * expert_parts(xn, p, chosen, *banks, False) + 2.0 ** -22 * np.abs(want)
+    assert (np.abs(y - want) <= bound).all()
+
+
 def test_no_tokens(rb, weights):
     import torch
 
