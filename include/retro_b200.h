@@ -436,11 +436,11 @@ int retro_b200_trainer_weights_updated(retro_trainer * trainer, const char * ada
 
 /* Writes a seeded random model as GGUF. `spec` is whitespace-separated key=value pairs:
  * arch(llama|qwen2|olmoe) layers d heads kv_heads head_dim ff vocab experts experts_used
- * dtype expert_dtype embd_dtype (f32|f16|q8_0|q4_k|mxfp4) std seed bias rope_base eps dist eot turn_end
+ * dtype expert_dtype embd_dtype (f32|f16|q4_0|q8_0|q4_k|mxfp4) std seed bias rope_base eps dist eot turn_end
  * (eot: a token id named by tokenizer.ggml.eot_token_id; turn_end: a token id only spelled as an end-of-turn piece). */
 int retro_b200_synth_gguf(const char * path, const char * spec, uint64_t * out_bytes);
 
-/* Encodes `n` floats as one stored row of `ggml_type` (0 f32, 1 f16, 8 q8_0, 12 q4_K, 39 mxfp4)
+/* Encodes `n` floats as one stored row of `ggml_type` (0 f32, 1 f16, 2 q4_0, 8 q8_0, 12 q4_K, 39 mxfp4)
  * with the same encoders the synthesiser uses. */
 int retro_b200_quantize_row(uint32_t ggml_type, const float * values, size_t n, uint8_t * out, size_t n_out, size_t * out_bytes);
 
@@ -549,7 +549,9 @@ int retro_b200_nccl_unique_id(void * out_id_128);
 /* GGML type codes the layer's gate / up / down expert banks are held in on the device. MXFP4 banks (type 39)
  * stay MXFP4: the grouped tcgen05 GEMM decodes the 17-byte blocks itself when every block's E8M0 byte is in
  * 104..128 (every weight then is an f16); banks outside that range whose scales an f16 still holds are re-coded,
- * exactly, as Q8_0 (type 8) for the mma.sync grouped GEMM; RB200_MOE=rows keeps the CUDA-core row kernel. */
+ * exactly, as Q8_0 (type 8) for the mma.sync grouped GEMM; RB200_MOE=rows keeps the CUDA-core row kernel.
+ * Q4_0 banks are held as Q8_0 blocks of the same values (type 8) for longer steps, and once more for the few-token kernels; RB200_MOE=few holds
+ * MXFP4 banks for those too. */
 int retro_b200_engine_expert_storage(retro_engine * engine, int layer, uint32_t * out_types_3);
 /* The load-time re-coding itself (host only, no GPU): n_blocks MXFP4 blocks (17 B each) -> Q8_0 blocks
  * (34 B each) holding the same values; *out_recoded = 0 and nothing written when a block's scale is not

@@ -32,7 +32,7 @@ namespace rb200 {
 
 namespace {
 
-constexpr int kSlotCol = 36;        // floats per (partial slot, token) of the third expert kernel: 32 rows, padded against bank conflicts
+constexpr int kSlotCol = 36;        // floats per (partial slot, token) of the second expert kernel: 32 rows, padded against bank conflicts
 constexpr int kRowList = kW4PassTokens;
 constexpr int kMaxCluster = 8;
 // Warps of a CTA that serves up to n tokens, and its CTAs on an SM.
@@ -74,6 +74,11 @@ __device__ __forceinline__ uint32_t remote_address(uint32_t at, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
     return a;
+}
+__device__ __forceinline__ float remote_load(uint32_t address) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
+    return v;
 }
 __device__ __forceinline__ void remote_store(uint32_t address, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
@@ -884,21 +889,18 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, resident_for(NT)) w4_produ
 
 // ---- a mixture-of-experts layer
 //
-// Three kernels. The first, one cluster, routes: its CTAs take ranges of the columns of all logits, a token's parts meet in the CTA
-// that picks its experts, and the first CTA lists the chosen experts with their tokens. The second has started
-// meanwhile and staged its activations; it multiplies the chosen experts' gate and up blocks and writes h = w_e silu(a) b for each (token,
-// expert) pair, split into hi + lo f16 with a power of two for every 32 columns: what the third kernel's products take. That one treats the chosen
-// experts' down matrices as one long reduction: a cluster
+// Two kernels. The first: every cluster normalises and routes all tokens for itself (the router is a few hundred
+// kilobytes that the L2 cache holds; a CTA reads its columns of it), then multiplies its share of the chosen
+// experts' gate and up blocks and writes h = w_e silu(a) b for each (token, expert) pair, split into hi + lo f16 with a power of two for every
+// 32 columns: what the second kernel's products take. That one treats the chosen experts' down matrices as one long reduction: a cluster
 // owns a range of y's rows, its CTAs and their warps divide the experts' concatenated columns, every unit of weights arrives
 // in a warp's ring together with the hidden columns it multiplies, and the sum over experts is part of the sum over the cluster. An
 // expert of more than three tokens is visited once per three of them (its weights then come from the L2 cache).
-// (Routing in every cluster of the second kernel, which saves the launch, had them all read the router: 11 us until the weights' first
-// bytes at one token and 19 us at sixteen, 32 experts of 2880 x 2880.)
 
-constexpr int kSet = 3;                 // tokens of an expert the third kernel takes at once
+constexpr int kSet = 3;                 // tokens of an expert the second kernel takes at once
 constexpr int kMaxPairs = kRowList * kW4MaxUsed;
 
-// What the routing writes for the other kernels, in the workspace in front of the hidden columns: a header {chosen experts, sets, -, -}, then arrays
+// The routing's result, in shared memory and for the second kernel in the workspace in front of the hidden columns: a header {chosen experts, sets, -, -}, then arrays
 // at these bytes, each long enough for `experts` chosen experts and `pairs` (token, expert) pairs.
 struct RouteAt {
     int expert, before, cost;               // of the chosen experts, ascending: u16 id; u16 pairs before it; i32 cost of the blocks before it (one more of the latter two)
@@ -980,8 +982,8 @@ struct MoeArgs {
     uint8_t * route;
     RouteAt at;
     uint8_t * hidden;
-    int clusters, x_bytes, c_bytes, inbox, partial;        // shared memory, in bytes
-    int ks, per_round;          // of the third kernel: parts of the columns, blocks of a round
+    int clusters, x_bytes, c_bytes, logit_bytes, inbox, partial;        // shared memory, in bytes
+    int ks, per_round;          // of the second kernel: parts of the columns, blocks of a round
 };
 
 // Sums each of the 16 values of a lane over the warp; lane i ends up with value i >> 1 (lanes 2 i and 2 i + 1 alike).
@@ -997,6 +999,77 @@ __device__ __forceinline__ float warp_sums16(float (&v)[16]) {
         }
     }
     return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+}
+
+// Columns of the router that fit into `room` bytes for all experts: whole groups of 32.
+__device__ __forceinline__ int router_columns(int E, int room) { return room / (E * 128) * 32; }
+
+// Copies columns [k, k + n) of all router rows to shared memory, row e at e * n. The caller commits, waits and synchronises.
+__device__ __forceinline__ void fetch_router(const MoeArgs & a, int k, int n, uint8_t * to) {
+    const uint32_t dst = smem_address(to);
+    if (a.router_vec) {
+        const int chunks = n / 4;
+        for (int i = threadIdx.x; i < a.E * chunks; i += blockDim.x) {
+            const int e = i / chunks, c = i - e * chunks;
+            copy16(dst + i * 16, reinterpret_cast<const uint8_t *>(a.router + (size_t)e * a.d + k + c * 4));
+        }
+    } else {
+        for (int i = threadIdx.x; i < a.E * n; i += blockDim.x) {
+            const int e = i / n, c = i - e * n;
+            reinterpret_cast<float *>(to)[i] = a.router[(size_t)e * a.d + k + c];
+        }
+    }
+}
+
+// The CTA's columns' part of every (token, expert) logit, from the staged activations and, piece by piece, the router in
+// `room` (the first piece is already on its way). The sums are in the staged activations' scale.
+template <bool MX, int PARTS, int NT, int WARPS>
+__device__ void partial_logits(const MoeArgs & a, int k0, int k1, const Staged & x, uint8_t * room, int room_bytes, float * out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int EB = 4, TB = NT == 1 ? 1 : 4;         // experts and tokens a warp takes at once
+    const int width = router_columns(a.E, room_bytes);
+    const int groups_t = (a.T + TB - 1) / TB, items = (a.E + EB - 1) / EB * groups_t;
+    for (int k = k0; k < k1; k += width) {
+        const int n = min(width, k1 - k);
+        if (k > k0) {
+            __syncthreads();
+            fetch_router(a, k, n, room);
+            copies_commit();
+        }
+        copies_wait<0>();
+        __syncthreads();
+        const float * r = reinterpret_cast<const float *>(room);
+        for (int item = warp; item < items; item += WARPS) {
+            const int e0 = item / groups_t * EB, t0 = (item - item / groups_t * groups_t) * TB;
+            float acc[16] = {};
+            for (int c = lane * 4; c < n; c += 128) {
+                const int at = k - k0 + c, step = at >> 7, group = (at >> 5) & 3;
+                float4 w[EB];
+#pragma unroll
+                for (int e = 0; e < EB; ++e) w[e] = *reinterpret_cast<const float4 *>(r + min(e0 + e, a.E - 1) * n + c);
+#pragma unroll
+                for (int t = 0; t < TB; ++t) {
+                    const uint8_t * p = x.x + ((step * 4 + group) * PARTS * NT + min(t0 + t, a.T - 1)) * 64 + (at & 31) * 2;
+                    const uint2 h = *reinterpret_cast<const uint2 *>(p);
+                    float2 v0 = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), v1 = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+                    if constexpr (PARTS == 2) {
+                        const uint2 l = *reinterpret_cast<const uint2 *>(p + NT * 64);
+                        const float2 l0 = __half22float2(*reinterpret_cast<const __half2 *>(&l.x)), l1 = __half22float2(*reinterpret_cast<const __half2 *>(&l.y));
+                        v0.x += l0.x; v0.y += l0.y; v1.x += l1.x; v1.y += l1.y;
+                    }
+#pragma unroll
+                    for (int e = 0; e < EB; ++e)
+                        acc[e * TB + t] += w[e].x * v0.x + w[e].y * v0.y + w[e].z * v1.x + w[e].w * v1.y;
+                }
+            }
+            const float sum = warp_sums16(acc);
+            const int i = lane >> 1, e = e0 + i / TB, t = t0 + i % TB;
+            if (!(lane & 1) && i < EB * TB && e < a.E && t < a.T) {
+                if (k == k0) out[t * a.E + e] = sum;
+                else out[t * a.E + e] += sum;
+            }
+        }
+    }
 }
 
 // Softmax over the experts and the n_used likeliest of one token, by one warp: pick i is lane i's. Ties go to the lowest index; whatever the
@@ -1055,25 +1128,20 @@ template <int PER, class Logit> __device__ __forceinline__ void pick_experts(Log
     if (normalise) weight /= chosen;
 }
 
-// The routing tables of one CTA of the routing kernel.
-struct RouteScratch {
-    float sums[kRowList * kW4MaxExperts];       // parts of the CTA's logits [part][token][expert]; at most max(experts, 64) * 16
-    float mail[kRowList * kW4MaxExperts];       // [CTA][token of this CTA][expert]: the cluster's parts of the logits
-    float squares[kMaxCluster][kRowList];       // [CTA][token of this CTA]
-    uint32_t expert[kMaxPairs];                 // the first CTA's: picks of all tokens, likeliest first
+// What the lists are made from.
+struct Picks {
+    uint32_t expert[kMaxPairs];                 // of all tokens, likeliest first
     float weight[kMaxPairs];
     uint32_t mask[kW4MaxExperts];               // by expert: the tokens that chose it
     uint16_t before[kW4MaxExperts];             // pairs of the experts before
     int totals[4][8];
 };
 
-// Writes the lists of the chosen experts, ascending, from the picks of all tokens. RouteScratch::mask is zero before.
-__device__ void write_route(const MoeArgs & a, RouteScratch & p) {
+// Writes the lists of the chosen experts, ascending, from the picks of all tokens. Picks::mask is zero before; a barrier follows at the caller's.
+__device__ void write_route(const MoeArgs & a, Picks & p, uint8_t * route) {
     const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
-    static_assert(kMaxPairs <= 512, "a thread of the routing kernel for every pair");
-    const bool pair = e < a.T * a.k;
-    const int t = e / a.k, own_expert = pair ? p.expert[e] : 0;
-    if (pair) atomicOr(&p.mask[own_expert], 1u << t);
+    const int pairs = a.T * a.k;
+    for (int i = e; i < pairs; i += blockDim.x) atomicOr(&p.mask[p.expert[i]], 1u << (i / a.k));
     __syncthreads();
     const uint32_t mask = e < (int)kW4MaxExperts ? p.mask[e] : 0;      // tokens that chose expert e
     const int n = __popc(mask), sets = (n + kSet - 1) / kSet;
@@ -1105,159 +1173,27 @@ __device__ void write_route(const MoeArgs & a, RouteScratch & p) {
     }
     if (mask) {
         const int u = before[0];
-        reinterpret_cast<uint16_t *>(a.route + a.at.expert)[u] = (uint16_t)e;
-        reinterpret_cast<uint16_t *>(a.route + a.at.before)[u] = (uint16_t)before[1];
-        reinterpret_cast<int *>(a.route + a.at.cost)[u] = before[3];
+        reinterpret_cast<uint16_t *>(route + a.at.expert)[u] = (uint16_t)e;
+        reinterpret_cast<uint16_t *>(route + a.at.before)[u] = (uint16_t)before[1];
+        reinterpret_cast<int *>(route + a.at.cost)[u] = before[3];
         p.before[e] = (uint16_t)before[1];
         for (int j = 0; j < sets; ++j) {
-            reinterpret_cast<uint16_t *>(a.route + a.at.set_expert)[before[2] + j] = (uint16_t)e;
-            reinterpret_cast<uint16_t *>(a.route + a.at.set_first)[before[2] + j] = (uint16_t)(before[1] + kSet * j);
-            a.route[a.at.set_count + before[2] + j] = (uint8_t)min(kSet, n - kSet * j);
+            reinterpret_cast<uint16_t *>(route + a.at.set_expert)[before[2] + j] = (uint16_t)e;
+            reinterpret_cast<uint16_t *>(route + a.at.set_first)[before[2] + j] = (uint16_t)(before[1] + kSet * j);
+            route[a.at.set_count + before[2] + j] = (uint8_t)min(kSet, n - kSet * j);
         }
     }
     if (e == 0) {
-        reinterpret_cast<uint16_t *>(a.route + a.at.before)[all[0]] = (uint16_t)all[1];
-        reinterpret_cast<int *>(a.route + a.at.cost)[all[0]] = all[3];
-        *reinterpret_cast<int4 *>(a.route) = make_int4(all[0], all[2], 0, 0);
+        reinterpret_cast<uint16_t *>(route + a.at.before)[all[0]] = (uint16_t)all[1];
+        reinterpret_cast<int *>(route + a.at.cost)[all[0]] = all[3];
+        *reinterpret_cast<int4 *>(route) = make_int4(all[0], all[2], 0, 0);
     }
     __syncthreads();
-    if (pair) {                 // an expert's tokens ascend
-        const int i = p.before[own_expert] + __popc(p.mask[own_expert] & ((1u << t) - 1));
-        a.route[a.at.token + i] = (uint8_t)t;
-        reinterpret_cast<float *>(a.route + a.at.weight)[i] = p.weight[e];
+    for (int i = e; i < pairs; i += blockDim.x) {               // an expert's tokens ascend
+        const int t = i / a.k, at = p.before[p.expert[i]] + __popc(p.mask[p.expert[i]] & ((1u << t) - 1));
+        route[a.at.token + at] = (uint8_t)t;
+        reinterpret_cast<float *>(route + a.at.weight)[at] = p.weight[i];
     }
-}
-
-constexpr int kRouteRoom = 64 * 1024;       // the routing kernel's shared memory for tokens
-
-// The routing, by one cluster. A CTA's columns of the tokens are staged as f32; a warp takes four experts and a part of the columns for all
-// tokens, so the router is read once, from memory into registers, the first of it before the tokens are there. What bounds it is latency: a read of the
-// tokens and the router, two meetings of the cluster.
-template <int NT>
-__global__ void __launch_bounds__(512, 1) w4_route_kernel(MoeArgs a) {
-    constexpr int kWarps = 16, EB = 4, kWide = kRouteRoom / (4 * NT) / 128 * 128;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ RouteScratch sc;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)cluster_rank(), C = (int)cluster_size(), log_c = __ffs(C) - 1;
-    cluster_arrive();
-    float * const xs = reinterpret_cast<float *>(smem);
-    if (threadIdx.x < kW4MaxExperts) sc.mask[threadIdx.x] = 0;
-    pdl_wait();
-    pdl_trigger();          // behind the wait: the next kernel may read what was complete before this one
-    const int k0 = part_begin2(a.d / 32, rank, log_c) * 32, columns = part_begin2(a.d / 32, rank + 1, log_c) * 32 - k0;
-    const int groups = (a.E + EB - 1) / EB;
-    int log_parts = 0;                      // parts of the columns: as many as there are warps for
-    while ((groups << (log_parts + 1)) <= kWarps) ++log_parts;
-    const Act norm{a.norm, 0, GGML_F32, (reinterpret_cast<uintptr_t>(a.norm) & 15) == 0};
-    // columns [from, from + wide) of all tokens at a time
-    for (int from = 0; from < columns; from += kWide) {
-        const int wide = min(kWide, columns - from), chunks = wide / 4;
-        float4 w[EB];
-        auto load_router = [&](int group, int c) {
-#pragma unroll
-            for (int e = 0; e < EB; ++e) {
-                const float * r = a.router + (size_t)min(group * EB + e, a.E - 1) * a.d + k0 + from + c;
-                if (a.router_vec) w[e] = *reinterpret_cast<const float4 *>(r);
-                else w[e] = make_float4(r[0], r[1], r[2], r[3]);
-            }
-        };
-        auto begin = [&](int job) { return part_begin2(chunks, job & ((1 << log_parts) - 1), log_parts) * 4; };
-        auto end = [&](int job) { return part_begin2(chunks, (job & ((1 << log_parts) - 1)) + 1, log_parts) * 4; };
-        const int jobs = groups << log_parts;
-        if (warp < jobs && begin(warp) + lane * 4 < end(warp)) load_router(warp >> log_parts, begin(warp) + lane * 4);
-        if (from > 0) __syncthreads();
-        for (int i = threadIdx.x; i < a.T * chunks; i += kWarps * 32) {
-            const int t = i / chunks, c = (i - t * chunks) * 4;
-            float v[4];
-            widen4(load4<false>(a.x, a.x.type, t, k0 + from + c), a.x.type, v);
-            if (a.norm) {
-                float by[4];
-                widen4(load4<false>(norm, GGML_F32, 0, k0 + from + c), GGML_F32, by);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= by[e];
-            }
-            *reinterpret_cast<float4 *>(xs + t * wide + c) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-        __syncthreads();
-        for (int job = warp; job < jobs; job += kWarps) {
-            const int group = job >> log_parts;
-            float acc[EB * NT] = {};
-            for (int c = begin(job) + lane * 4, c_end = end(job), first = job == warp; c < c_end; c += 128, first = 0) {
-                if (!first) load_router(group, c);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const float4 v = *reinterpret_cast<const float4 *>(xs + min(t, a.T - 1) * wide + c);
-#pragma unroll
-                    for (int e = 0; e < EB; ++e) acc[e * NT + t] += w[e].x * v.x + w[e].y * v.y + w[e].z * v.z + w[e].w * v.w;
-                }
-            }
-            constexpr int kChunk = EB * NT < 16 ? EB * NT : 16;
-#pragma unroll
-            for (int at = 0; at < EB * NT; at += kChunk) {
-                float v[16] = {};
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) v[i] = acc[at + i];
-                const float sum = warp_sums16(v);
-                const int i = at + (lane >> 1), e = group * EB + i / NT, t = i % NT;
-                float * to = &sc.sums[((job & ((1 << log_parts) - 1)) * a.T + t) * a.E + e];
-                if (!(lane & 1) && (lane >> 1) < kChunk && e < a.E && t < a.T) *to = from > 0 ? *to + sum : sum;
-            }
-        }
-    }
-    if (columns == 0) {
-        for (int i = threadIdx.x; i < (a.T * a.E) << log_parts; i += kWarps * 32) sc.sums[i] = 0.f;
-    }
-    float squares = 0.f;
-    if (a.norm && warp < a.T) {
-        for (int c = lane * 4; c < columns; c += 128) {
-            float v[4];
-            widen4(load4<false>(a.x, a.x.type, warp, k0 + c), a.x.type, v);
-            squares += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-    }
-    cluster_wait();
-    __syncthreads();
-    // token t's go to CTA t % C
-    const int of_cta = kRowList >> log_c;
-    if (a.norm && warp < a.T && lane == 0) remote_store(remote_address(smem_address(&sc.squares[rank][warp >> log_c]), warp & (C - 1)), squares);
-    for (int i = threadIdx.x; i < a.T * a.E; i += kWarps * 32) {
-        const int t = i / a.E, e = i - t * a.E;
-        float v = 0.f;
-        for (int part = 0; part < 1 << log_parts; ++part) v += sc.sums[part * a.T * a.E + i];
-        remote_store(remote_address(smem_address(&sc.mail[(rank * of_cta + (t >> log_c)) * a.E + e]), t & (C - 1)), v);
-    }
-    cluster_sync();
-    const int t = warp * C + rank;
-    if (t < a.T) {
-        float rstd = 1.f;
-        if (a.norm) {
-            float ss = 0.f;
-            for (int c = 0; c < C; ++c) ss += sc.squares[c][warp];
-            rstd = rsqrtf(ss / (float)a.d + a.eps);
-        }
-        auto logit = [&](int e) {
-            float v = 0.f;
-            for (int c = 0; c < C; ++c) v += sc.mail[(c * of_cta + warp) * a.E + e];
-            return v * rstd;
-        };
-        int expert;
-        float weight;
-        if (a.E <= 32) pick_experts<1>(logit, a.E, a.k, a.normalise, expert, weight);
-        else if (a.E <= 128) pick_experts<4>(logit, a.E, a.k, a.normalise, expert, weight);
-        else pick_experts<kW4MaxExperts / 32>(logit, a.E, a.k, a.normalise, expert, weight);
-        if (lane < a.k) {
-            const int i = t * a.k + lane;
-            remote_store(remote_address(smem_address(&sc.expert[i]), 0), __uint_as_float((uint32_t)expert));
-            remote_store(remote_address(smem_address(&sc.weight[i]), 0), weight);
-            if (a.ids) a.ids[i] = expert;
-            if (a.weights) a.weights[i] = weight;
-        }
-    }
-    cluster_sync();
-    if (rank == 0) write_route(a, sc);
 }
 
 // Jobs: block j of an expert's gate and of its up matrix are jobs 2 j and 2 j + 1, experts one behind the other.
@@ -1326,25 +1262,75 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
     constexpr int kWarps = warps_for(NT);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Scratch<kWarps> sc;
+    __shared__ Picks picks;
     __shared__ __align__(16) uint8_t route_copy[kRouteBytes];
     __shared__ int range[2];
-    const int warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), C = (int)cluster_size(), log_c = __ffs(C) - 1;
     const int cluster = blockIdx.x >> log_c;
     cluster_arrive();
     const int s0 = part_begin2(a.steps_d, rank, log_c), n_steps = part_begin2(a.steps_d, rank + 1, log_c) - s0;
     const Staged x{smem, reinterpret_cast<float *>(smem + a.x_bytes)};
-    uint8_t * const rings = smem + a.x_bytes + a.c_bytes;
+    float * mine = reinterpret_cast<float *>(smem + a.x_bytes + a.c_bytes);         // this CTA's part of the logits
+    float * logits = mine + a.logit_bytes / 4;
+    uint8_t * const rings = smem + a.x_bytes + a.c_bytes + 2 * a.logit_bytes;
     if (threadIdx.x == 0) sc.zero = 0;
+    if (threadIdx.x < kW4MaxExperts) picks.mask[threadIdx.x] = 0;
 
-    // The activations were complete before the routing kernel, which lets this one start behind its own wait; they are read
-    // through the L2 cache only. The norm's weights wait in the rings' first stage.
-    stage_tokens<MX, PARTS>(a.x, a.T, NT, s0 * 128, n_steps, a.d, a.norm, NormRoom{smem_address(rings), (int)(kMoeStages * w4_unit_bytes(MX)), kWarps}, x, sc, rank, C);
+    pdl_trigger();
     pdl_wait();
-    pdl_trigger();          // behind the wait: the next kernel may read the route
-    const Route route{route_copy, a.at};
-    copy_route(a.route, route_copy, a.at.expert, a.at.set_expert);
+    const int k0 = s0 * 128, k1 = min(a.d, (s0 + n_steps) * 128);
+    // the rings and the first inbox are idle until the experts are known
+    const int idle = ring_bytes(MX, NT, kMoeStages) + a.inbox;
+    fetch_router(a, k0, min(k1 - k0, router_columns(a.E, idle)), rings);
+    copies_commit();
+    stage_tokens<MX, PARTS>(a.x, a.T, NT, k0, n_steps, a.d, a.norm, NormRoom{0, 0, 0}, x, sc, rank, C);
     __syncthreads();
+    partial_logits<MX, PARTS, NT, kWarps>(a, k0, k1, x, rings, idle, mine);
+    // Out of the activations' scale (a token's factor without the weights' constant) and to every CTA of the cluster: into its second
+    // inbox, which nobody else writes before the cluster has met after the first round, where that has room.
+    __syncthreads();
+    const int n_logits = a.T * a.E;
+    const uint32_t mail = smem_address(rings) + ring_bytes(MX, NT, kMoeStages) + a.inbox;
+    const bool posted = C * n_logits * 4 <= a.inbox;
+    for (int i = threadIdx.x; i < n_logits; i += kWarps * 32) {
+        const float v = mine[i] * (sc.factor[i / a.E] * power(-weight_shift(MX)));
+        if (posted) {
+            for (int c = 0; c < C; ++c) remote_store(remote_address(mail + (rank * n_logits + i) * 4, c), v);
+        } else {
+            mine[i] = v;
+        }
+    }
+    cluster_sync();
+    for (int i = threadIdx.x; i < n_logits; i += kWarps * 32) {
+        float v = 0.f;
+        for (int c = 0; c < C; ++c) v += posted ? shared_f1(mail + (c * n_logits + i) * 4) : remote_load(remote_address(smem_address(mine + i), c));
+        logits[i] = a.norm ? v * rms_factor(sc, i / a.E, C, a.d, a.eps) : v;
+    }
+    __syncthreads();
+    for (int t = warp; t < a.T; t += kWarps) {
+        auto logit = [&](int e) { return logits[t * a.E + e]; };
+        int expert;
+        float weight;
+        if (a.E <= 32) pick_experts<1>(logit, a.E, a.k, a.normalise, expert, weight);
+        else if (a.E <= 128) pick_experts<4>(logit, a.E, a.k, a.normalise, expert, weight);
+        else pick_experts<kW4MaxExperts / 32>(logit, a.E, a.k, a.normalise, expert, weight);
+        if (lane < a.k) {
+            const int i = t * a.k + lane;
+            picks.expert[i] = (uint32_t)expert;
+            picks.weight[i] = weight;
+            if (blockIdx.x == 0 && a.ids) a.ids[i] = expert;
+            if (blockIdx.x == 0 && a.weights) a.weights[i] = weight;
+        }
+    }
+    if (threadIdx.x < 2) range[threadIdx.x] = 0;
+    __syncthreads();
+    write_route(a, picks, route_copy);
+    __syncthreads();
+    const Route route{route_copy, a.at};
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < a.at.bytes / 16; i += kWarps * 32) reinterpret_cast<uint4 *>(a.route)[i] = reinterpret_cast<const uint4 *>(route_copy)[i];
+    }
     // The cluster's blocks: those whose cost begins in its share of the whole cost.
     if (threadIdx.x < 2) range[threadIdx.x] = 0;
     __syncthreads();
@@ -1399,10 +1385,10 @@ __global__ void __launch_bounds__(warps_for(NT) * 32, NT > 4 ? 1 : 2) w4_moe_gat
         }
         b0 += now;
     }
-    if (blocks == 0) cluster_sync();        // nobody leaves while the squares of its rows are on their way
+    if (blocks == 0) cluster_sync();        // nobody leaves while its logits are read
 }
 
-// The third kernel's stream: as Stream, but a unit comes with the hidden columns it multiplies. Weights run two units ahead, hidden
+// The second kernel's stream: as Stream, but a unit comes with the hidden columns it multiplies. Weights run two units ahead, hidden
 // columns one.
 template <bool MX, int MOST> struct DownStream {
     static constexpr int kWarps = MOST > 1 ? 16 : 8, kStages = 3;
@@ -1488,14 +1474,10 @@ template <bool MX, int MOST> struct DownStream {
         h_fill ^= kHidden;              // one stage or the other
         copies_commit();
     }
-    // The first two units' weights, and with `begin` the first one's hidden columns: the loop finds all of them older than one group of copies.
     __device__ __forceinline__ void prefetch() {
         fetch_weights();
-        fetch_weights();
-    }
-    __device__ __forceinline__ void begin() {
         fetch_hidden();
-        copies_commit();
+        fetch_weights();
     }
     template <int NT, class Column> __device__ __forceinline__ void work_run(Column column) {
         float acc[2][2][4] = {};
@@ -1542,9 +1524,10 @@ __global__ void __launch_bounds__(DownStream<MX, MOST>::kWarps * 32, MOST > 1 ? 
     const Inbox inbox{smem_address(partial) + a.partial, a.inbox, rank, log_c, 1, 1};
     const int j_begin = part_begin(a.blocks_d, cluster, a.clusters), j_end = part_begin(a.blocks_d, cluster + 1, a.clusters);
     pdl_trigger();
-    // the kernel before this one lets it start when the route is there
+    pdl_wait();
     const Route route{route_copy, a.at};
     copy_route(a.route, route_copy, a.at.token, a.at.bytes);
+    cluster_wait();
     __syncthreads();
     const int total = route.sets() * a.steps_ff;    // the sets' columns, one behind the other
     const int begin = part_begin2(total, rank, log_c), n = part_begin2(total, rank + 1, log_c) - begin;
@@ -1556,11 +1539,6 @@ __global__ void __launch_bounds__(DownStream<MX, MOST>::kWarps * 32, MOST > 1 ? 
                                     first < stride ? jobs : 0, first, stride);
         stream.prefetch();
         for (int i = threadIdx.x; i < jobs * ks * a.T * kSlotCol; i += kWarps * 32) partial[i] = 0.f;
-        if (round == 0) {
-            pdl_wait();         // the hidden columns
-            cluster_wait();
-        }
-        stream.begin();
         __syncthreads();
         stream.work([&](int job, int token) { return partial + ((job * ks + sub) * a.T + token) * kSlotCol; });
         __syncthreads();
@@ -1712,16 +1690,6 @@ template <bool MX> cudaError_t launch_gate_up_of(const MoeArgs & a, int parts, i
     return with_room(nt, [&](auto n) { return launch_gate_up<MX, 1, decltype(n)::value>(a, C, smem, stream); });
 }
 
-cudaError_t launch_route(const MoeArgs & a, cudaStream_t stream) {
-    return with_room(product_room(a.T), [&](auto n) {
-        constexpr int nt = decltype(n)::value;
-        static PerDeviceOnce once;
-        const cudaError_t e = once.first() ? cudaFuncSetAttribute(w4_route_kernel<nt>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteRoom) : cudaSuccess;
-        const int columns = (a.d / 32 + kMaxCluster - 1) / kMaxCluster * 32;        // of a CTA, at most
-        return e != cudaSuccess ? e : launch_cluster(w4_route_kernel<nt>, kMaxCluster, 512, kMaxCluster, (size_t)std::min(kRouteRoom, columns * 4 * a.T), stream, a);
-    });
-}
-
 template <bool MX, int MOST> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
     static PerDeviceOnce once;
     const cudaError_t e = allow_smem(once, w4_moe_down_kernel<MX, MOST>);
@@ -1779,14 +1747,14 @@ struct Cut {
 // Chooses the cluster size for `blocks` row blocks of `per` matrices and `steps` column steps whose activations take `each` bytes of
 // shared memory a step. The estimate is in clocks: the weight stream at the SM's share of the memory bandwidth, but no faster
 // than the busiest SM's warps get through it or than its copies in flight allow; the conversion of the CTA's share of the activations; the sums it
-// receives; and a barrier for every round its inbox allows.
-Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int stages, int most_resident, int least_c, int most_c, int fixed, int sms) {
+// receives; and a barrier for every round its inbox allows. `fixed` is other dynamic shared memory, `statics` the kernel's static one.
+Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int stages, int most_resident, int least_c, int most_c, int fixed, int statics, int sms) {
     Cut best;
     const int warps = warps_for(n), ring = ring_bytes(mx, n, stages), unit = (int)w4_unit_bytes(mx);
     for (int C = least_c; C <= most_c && C <= steps; C *= 2) {
         const int s = (steps + C - 1) / C;
-        const int64_t smem = (int64_t)s * each + ring + fixed + 2 * inbox_bytes(n, C, 1, per) + 4096;
-        if (smem - fixed - 4096 + 256 > kMaxSmem || smem > kSmShare) continue;      // `fixed` is static, and the parts are rounded up
+        const int64_t smem = (int64_t)s * each + ring + fixed + statics + 2 * inbox_bytes(n, C, 1, per) + 4096;
+        if (smem - statics - 4096 + 256 > kMaxSmem || smem > kSmShare) continue;    // the parts are rounded up
         Cut c;
         c.C = C;
         c.resident = (int)std::min<int64_t>(most_resident, kSmShare / smem);
@@ -1801,7 +1769,7 @@ Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int sta
         const double stream = std::max({(double)blocks * per * steps * unit / (23.5 * sms) * std::max(1.0, 13e6 / in_flight),     // two microseconds of latency under load
                                         (double)busy * runs * warps * ((s + ks - 1) / ks + (n > 8 ? 0.6 : 0.3)) * unit_clocks});
         const double convert = busy * s * n * 128 * 0.1 + 800, sums = busy * (double)blocks_each * per * n * (6 + 2 * C * ks);
-        const int64_t room = std::min(kSmShare / c.resident - 4096, kMaxSmem) - fixed - ring - (int64_t)s * each;
+        const int64_t room = std::min(kSmShare / c.resident - statics - 4096, kMaxSmem) - fixed - ring - (int64_t)s * each;
         const double rounds = std::ceil((double)inbox_bytes((int64_t)blocks_each * n, C, ks, per) / std::max<int64_t>(room, 1024));
         c.cost = stream + convert + sums / 4 + (rounds > 1 ? 2 * rounds : 1) * 1500;
         if (!best.C || c.cost < best.cost) best = c;
@@ -1824,7 +1792,7 @@ Cut product_cut(int blocks, int per, int steps, bool mx, int parts, int & n) {
     if (!std::equal(key, key + 7, k.key)) {
         for (k.n = n;; k.n = (k.n + 1) / 2) {
             const int room = product_room(k.n);
-            k.cut = choose_cut(blocks, per, steps, k.n, step_bytes(mx, parts, room), mx, stages_for(k.n, parts), resident_for(room), 1, kMaxCluster, 0, device_sms());
+            k.cut = choose_cut(blocks, per, steps, k.n, step_bytes(mx, parts, room), mx, stages_for(k.n, parts), resident_for(room), 1, kMaxCluster, 0, 0, device_sms());
             if (k.cut.C || k.n == 1) break;
         }
         std::copy(key, key + 7, k.key);
@@ -1919,9 +1887,9 @@ size_t w4_moe_workspace_bytes(uint32_t ff, uint32_t n_tokens, uint32_t n_used) {
 
 namespace {
 
-constexpr int kMoeStatic = 9 * 1024;        // static shared memory of the second kernel, rounded up: the route and what stage_tokens needs
+constexpr int kMoeStatic = 15 * 1024;       // static shared memory of the first kernel, rounded up: picks, route and what stage_tokens needs
 
-// How the second and third kernel of a pass over n tokens are cut.
+// How the two kernels of a pass over n tokens are cut.
 struct MoePlan {
     int n = 0;
     Cut cut;
@@ -1931,21 +1899,20 @@ struct MoePlan {
 
 MoePlan make_moe_plan(int E, int used, int blocks_ff, int steps_d, int blocks_d, int steps_ff, bool mx, bool mx_down, int parts, int n) {
     MoePlan m;
-    // Second kernel: n tokens that choose independently choose about `reach` experts. Up to four tokens it runs in clusters of four (one token, 32 experts of
-    // 2880 x 2880: 29.4 us the layer, 30.1 us with two and 29.5 with eight), more in clusters of two, which fill the SMs better (64 experts of
-    // 1024 x 2048, six tokens: 47.6 us, 50.0 us with four; the former layer, sixteen tokens: 119.5 us with either), of more where rows are so long that
-    // these cannot hold them.
+    // First kernel: n tokens that choose independently choose about `reach` experts. It runs in clusters of four (one token, 32 experts of
+    // 2880 x 2880: 31 us the layer, 38 us with eight; 64 experts of 1024 x 2048, six tokens: 50 us, 55 us with two), of more where rows are so long
+    // that four cannot hold them.
     for (;; n = (n + 1) / 2) {
         const int reach = std::max(1, (int)std::ceil(E * (1.0 - std::pow(1.0 - (double)used / E, n)))), room = product_room(n);
-        const int least_c = steps_d < 2 ? 1 : steps_d < 4 || n > 4 ? 2 : 4;
+        const int least_c = steps_d < 2 ? 1 : steps_d < 4 ? 2 : 4;
         for (int C = least_c; !m.cut.C && C <= kMaxCluster; C *= 2)
-            m.cut = choose_cut(reach * blocks_ff, 2, steps_d, n, step_bytes(mx, parts, room), mx, kMoeStages, room > 4 ? 1 : 2, C, C, kMoeStatic, device_sms());
+            m.cut = choose_cut(reach * blocks_ff, 2, steps_d, n, step_bytes(mx, parts, room), mx, kMoeStages, room > 4 ? 1 : 2, C, C, 2 * up_to(n * E * 4, 128), kMoeStatic, device_sms());
         if (m.cut.C || n == 1) break;
     }
     m.n = n;
     if (!m.cut.C) return m;
-    // Third kernel, in clusters of four: eight would leave a warp two units of a run at one token. One token: three CTAs of eight warps on an SM;
-    // several: one of sixteen, whose partial sums share the room better (sixteen tokens: 124 us the layer, 135 us with two of eight).
+    // Second kernel, in clusters of four: eight would leave a warp two units of a run at one token. One token: three CTAs of eight warps on an SM;
+    // several: one of sixteen, whose partial sums share the room better (sixteen tokens, 32 experts of 2880 x 2880: 11 us of 135 less).
     m.C = 4;
     while (m.C > steps_ff * used) m.C /= 2;
     const int resident = n > 1 ? 1 : 3, warps = n > 1 ? 16 : 8;
@@ -2047,12 +2014,11 @@ cudaError_t launch_w4_moe(const W4Moe & p, cudaStream_t stream) {
         const int nt = product_room(n), s = (steps_d + cut.C - 1) / cut.C;
         a.x_bytes = up_to(s * step_x_bytes(parts, nt), 128);
         a.c_bytes = up_to(s * step_c_bytes(mx, nt), 128);
+        a.logit_bytes = up_to(n * E * 4, 128);
         a.clusters = cut.clusters;
-        const int fixed = a.x_bytes + a.c_bytes + ring_bytes(mx, nt, kMoeStages);
+        const int fixed = a.x_bytes + a.c_bytes + 2 * a.logit_bytes + ring_bytes(mx, nt, kMoeStages);
         a.inbox = (int)std::max<int64_t>((std::min(kSmShare / cut.resident - kMoeStatic - 4096, kMaxSmem) - fixed) / 2 / 128 * 128, inbox_bytes(n, cut.C, 1, 2));
-        cudaError_t e = launch_route(a, stream);
-        if (e != cudaSuccess) return e;
-        e = mx ? launch_gate_up_of<true>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream)
+        cudaError_t e = mx ? launch_gate_up_of<true>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream)
                            : launch_gate_up_of<false>(a, parts, cut.C, (size_t)fixed + 2 * a.inbox, stream);
         if (e != cudaSuccess) return e;
 
