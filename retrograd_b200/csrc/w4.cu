@@ -1651,12 +1651,23 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), int grid, int threads, int 
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-template <typename... KArgs> cudaError_t allow_smem(PerDeviceOnce & once, void (*kernel)(KArgs...)) {
-    return once.first() ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) : cudaSuccess;
+// Devices on which a kernel has been given its shared memory. Set behind the call that does it: of threads that come at once, each does.
+struct Prepared {
+    std::atomic<uint64_t> done[4] = {};
+};
+template <typename... KArgs> cudaError_t allow_smem(Prepared & prepared, void (*kernel)(KArgs...)) {
+    int device = 0;
+    cudaGetDevice(&device);
+    std::atomic<uint64_t> & done = prepared.done[(device >> 6) & 3];
+    const uint64_t bit = 1ull << (device & 63);
+    if (done.load() & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
 }
 
 template <bool MX, int PARTS, bool GLU, int NT> cudaError_t launch_product(const ProductArgs & a, int clusters, int C, size_t smem, cudaStream_t stream) {
-    static PerDeviceOnce once;
+    static Prepared once;
     const cudaError_t e = allow_smem(once, w4_product_kernel<MX, PARTS, GLU, NT>);
     return e != cudaSuccess ? e : launch_cluster(w4_product_kernel<MX, PARTS, GLU, NT>, clusters * C, warps_for(NT) * 32, C, smem, stream, a);
 }
@@ -1679,7 +1690,7 @@ template <bool MX, bool GLU> cudaError_t launch_product_of(const ProductArgs & a
 }
 
 template <bool MX, int PARTS, int NT> cudaError_t launch_gate_up(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
-    static PerDeviceOnce once;
+    static Prepared once;
     const cudaError_t e = allow_smem(once, w4_moe_gate_up_kernel<MX, PARTS, NT>);
     return e != cudaSuccess ? e : launch_cluster(w4_moe_gate_up_kernel<MX, PARTS, NT>, a.clusters * C, warps_for(NT) * 32, C, smem, stream, a);
 }
@@ -1691,7 +1702,7 @@ template <bool MX> cudaError_t launch_gate_up_of(const MoeArgs & a, int parts, i
 }
 
 template <bool MX, int MOST> cudaError_t launch_down(const MoeArgs & a, int C, size_t smem, cudaStream_t stream) {
-    static PerDeviceOnce once;
+    static Prepared once;
     const cudaError_t e = allow_smem(once, w4_moe_down_kernel<MX, MOST>);
     return e != cudaSuccess ? e : launch_cluster(w4_moe_down_kernel<MX, MOST>, a.clusters * C, DownStream<MX, MOST>::kWarps * 32, C, smem, stream, a);
 }

@@ -308,6 +308,34 @@ assert (y == -8 * 64).all()
     assert run.returncode == 0, run.stderr[-2000:]
 
 
+def test_first_calls_of_several_threads(rb):
+    """A fresh process whose threads make their first calls at once, each on a stream of its own, with one weight handle."""
+    import subprocess
+    import sys
+
+    code = """
+import threading
+import numpy as np, torch, retrograd_b200 as rb
+raw = np.random.default_rng(0).integers(0, 256, (4096, 4096 // 32 * 18), dtype=np.uint8); raw[:, 1::18] = 0x2c
+m = rb.W4Matrix(2, raw, 4096, 4096)
+xs = {n: torch.randn(n, 4096, device="cuda") for n in (1, 3, 7, 16)}
+torch.cuda.synchronize()
+gate = threading.Barrier(8)
+got = [None] * 8
+def work(i):
+    stream = torch.cuda.Stream()
+    gate.wait()
+    got[i] = {n: [rb.w4_matvec(m, x, stream=stream) for _ in range(10)] for n, x in xs.items()}
+    stream.synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+[t.start() for t in threads]; [t.join() for t in threads]
+want = {n: rb.w4_matvec(m, x) for n, x in xs.items()}
+assert all(torch.equal(y, want[n]) for g in got for n, ys in g.items() for y in ys)
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
 def test_in_place_expert_layer(rb, weights):
     import torch
 
