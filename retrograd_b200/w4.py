@@ -114,21 +114,20 @@ def _open(op: str, *matrices) -> int:
     return matrices[0].device
 
 
-def _new(x, shape, dtype, stream, device: int):
-    """A tensor on x's device, made on the stream the call runs on: the allocator hands its memory to no other stream before."""
-    on = _raw_stream(device)
-    if stream is None or getattr(stream, "cuda_stream", stream) == on:
-        return x.new_empty(shape, dtype=dtype)
+def _new(make, stream, device: int):
+    """The tensor that make() makes, on the stream the call runs on: the allocator hands its memory to no other stream before."""
+    if stream is None or getattr(stream, "cuda_stream", stream) == _raw_stream(device):
+        return make()
     torch = _torch()
     with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=device)):
-        return x.new_empty(shape, dtype=dtype)
+        return make()
 
 
-def _result(op: str, x, out, tokens: int, width: int, device: int, stream):
+def _result(op: str, x, tx: int, out, tokens: int, width: int, device: int, stream):
     """The result tensor (a new one of x's type unless `out` is given), its pointer, type code and row stride."""
     if out is None:
-        y = _new(x, (tokens, width), x.dtype, stream, device)
-        return y, y.data_ptr(), _TYPES[x.dtype], width
+        y = x.new_empty(tokens, width) if stream is None else _new(lambda: x.new_empty(tokens, width), stream, device)
+        return y, y.data_ptr(), tx, width
     return (out, *_rows(op, "out", out, width, device, tokens))
 
 
@@ -149,14 +148,16 @@ def w4_matvec(w: W4Matrix, x, *, norm=None, eps: float = 1e-5, bias=None, residu
     """y = xn W^T + bias + residual for x [tokens, n_in]; xn is x, or its RMSNorm with the weights `norm`. `out` (any of the three
     element types, may be `residual`) or a new tensor of x's type is returned; a residual has the result's type."""
     _TYPES or _torch()
-    device = _open("w4_matvec", w)
+    device = w.device
+    if not w._h:
+        _open("w4_matvec", w)
     px, tx, ldx = _rows("w4_matvec", "x", x, w.n_in, device)
     tokens = x.shape[0]
-    y, py, ty, ldy = _result("w4_matvec", x, out, tokens, w.n_out, device, stream)
-    pr, ldr = _residual("w4_matvec", residual, ty, w.n_out, device, tokens)
+    y, py, ty, ldy = _result("w4_matvec", x, tx, out, tokens, w.n_out, device, stream)
+    pr, ldr = (None, 0) if residual is None else _residual("w4_matvec", residual, ty, w.n_out, device, tokens)
     if tokens:
-        status = w._lib.retro_b200_w4_matvec(w._h, px, tx, ldx, tokens, _vector("w4_matvec", "norm", norm, w.n_in, device), eps,
-                                             _vector("w4_matvec", "bias", bias, w.n_out, device), pr, ldr, py, ty, ldy, _stream(stream, device))
+        status = w._lib.retro_b200_w4_matvec(w._h, px, tx, ldx, tokens, None if norm is None else _vector("w4_matvec", "norm", norm, w.n_in, device), eps,
+                                             None if bias is None else _vector("w4_matvec", "bias", bias, w.n_out, device), pr, ldr, py, ty, ldy, _stream(stream, device))
         if status:
             _check(status)
     return y
@@ -168,7 +169,7 @@ def w4_glu(gate: W4Matrix, up: W4Matrix, x, *, norm=None, eps: float = 1e-5, out
     device = _open("w4_glu", gate, up)
     px, tx, ldx = _rows("w4_glu", "x", x, gate.n_in, device)
     tokens = x.shape[0]
-    y, py, ty, ldy = _result("w4_glu", x, out, tokens, gate.n_out, device, stream)
+    y, py, ty, ldy = _result("w4_glu", x, tx, out, tokens, gate.n_out, device, stream)
     if tokens:
         status = gate._lib.retro_b200_w4_glu(gate._h, up._h, px, tx, ldx, tokens, _vector("w4_glu", "norm", norm, gate.n_in, device), eps, py, ty, ldy,
                                              _stream(stream, device))
@@ -188,7 +189,7 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
     n_in = gate.n_in
     px, tx, ldx = _rows("w4_moe", "x", x, n_in, device)
     tokens = x.shape[0]
-    y, py, ty, ldy = _result("w4_moe", x, out, tokens, n_in, device, stream)
+    y, py, ty, ldy = _result("w4_moe", x, tx, out, tokens, n_in, device, stream)
     pr, ldr = _residual("w4_moe", residual, ty, n_in, device, tokens)
     if not 1 <= n_used <= min(gate.n_expert, 32):
         raise InvalidArgument("w4_moe: n_used must be 1 to n_expert, at most 32")
@@ -199,7 +200,8 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
         return y
     on = _stream(stream, device)
     if workspace is None:
-        workspace = _new(x, (w4_moe_workspace(gate, tokens, n_used),), torch.uint8, stream, device)
+        need = w4_moe_workspace(gate, tokens, n_used)
+        workspace = _new(lambda: torch.empty(need, dtype=torch.uint8, device=x.device), stream, device)
     elif workspace.get_device() != device or not workspace.is_contiguous():
         raise InvalidArgument("w4_moe: the workspace must be contiguous on the weights' device")
     _check(gate._lib.retro_b200_w4_moe(_vector("w4_moe", "router", router, gate.n_expert * n_in, device), gate._h, up._h, down._h, px, tx, ldx, tokens, n_used,
