@@ -4,7 +4,7 @@
 // of B. The weights enter as exact f16 values that cost little arithmetic:
 //   Q4_0   the nibble q in the top four mantissa bits of an f16 is the subnormal q 2^-18: a rotation and a mask. (In the
 //          low bits it would save the rotation, but the tensor cores align products by the operands' exponents and dropped up to ten
-//          bits of such products: 1.6e-6 of the result. As the difference q - 8 it costs an addition, 64 us instead of 55 for
+//          bits of such products: 1.6e-6 of the result. As the difference q - 8 it costs an addition, 63.5 us instead of 56 for
 //          128256 x 4096 at one token.) The offset is the product chain's start value, -8 2^-18 times the group's sum of activations.
 //   MXFP4  the conversion instruction for pairs of e2m1 values.
 // A token's activations are scaled by a power of two that brings the largest of them into [2^13, 2^14) and split into
@@ -18,6 +18,11 @@
 // activation. Every warp streams its units through a ring of its own in shared memory by asynchronous copies, one or two units
 // ahead, so that no registers are held by loads in flight. Up to four tokens run as three CTAs of eight warps on an SM; more
 // as one of sixteen, because all warps of a CTA share its activations.
+//
+// Measured (replayed in a graph, weights larger than the L2 cache), Q4_0: 128256 x 4096 at one token 56 us, 5.24 TB/s, bound by the integer pipe that
+// unpacks; 14336 x 4096 gated pair 18.7 us at one token (3.5 TB/s), 36 us at sixteen, where mma.sync with hi and lo parts is the busiest unit of the product loop
+// and staging takes 6 us; 4096 x 14336 at one token 11.4 us (2.9 TB/s), a third of it staging and the launch. MXFP4, 201088 x 2880, sixteen
+// bf16 tokens: 96 us, 3.2 TB/s. A layer of 32 experts of 2880 x 2880 (MXFP4, four used): 31 us at one token, 114 us at sixteen.
 
 #include "kernels.cuh"
 #include "blocks.hpp"
