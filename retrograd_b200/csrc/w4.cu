@@ -257,26 +257,22 @@ __device__ __forceinline__ void widen4(const uint4 & u, uint32_t type, float (&v
 }
 template <int PARTS> __device__ __forceinline__ uint32_t type_of(const Act & act) { return PARTS == 2 ? act.type : act.type == GGML_F16 ? GGML_F16 : GGML_BF16; }
 
-// Columns k .. k + 3 of a row; L2: through the L2 cache only.
-template <bool L2, class T> __device__ __forceinline__ T load(const T * from) {
-    if constexpr (L2) return __ldcg(from);
-    else return *from;
-}
-template <bool L2> __device__ __forceinline__ uint4 load4(const Act & act, uint32_t type, int64_t row, int k) {
+// Columns k .. k + 3 of a row, through the L2 cache only.
+__device__ __forceinline__ uint4 load4(const Act & act, uint32_t type, int64_t row, int k) {
     uint4 u = {};
     if (type == GGML_F32) {
         const unsigned * from = static_cast<const unsigned *>(act.p) + row * act.ld + k;
-        if (act.vec) u = load<L2>(reinterpret_cast<const uint4 *>(from));
-        else u = make_uint4(load<L2>(from), load<L2>(from + 1), load<L2>(from + 2), load<L2>(from + 3));
+        if (act.vec) u = __ldcg(reinterpret_cast<const uint4 *>(from));
+        else u = make_uint4(__ldcg(from), __ldcg(from + 1), __ldcg(from + 2), __ldcg(from + 3));
     } else {
         const unsigned short * from = static_cast<const unsigned short *>(act.p) + row * act.ld + k;
         if (act.vec) {
-            const uint2 w = load<L2>(reinterpret_cast<const uint2 *>(from));
+            const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(from));
             u.x = w.x;
             u.y = w.y;
         } else {
-            u.x = load<L2>(from) | (uint32_t)load<L2>(from + 1) << 16;
-            u.y = load<L2>(from + 2) | (uint32_t)load<L2>(from + 3) << 16;
+            u.x = __ldcg(from) | (uint32_t)__ldcg(from + 1) << 16;
+            u.y = __ldcg(from + 2) | (uint32_t)__ldcg(from + 3) << 16;
         }
     }
     return u;
@@ -361,8 +357,8 @@ __device__ __noinline__ void stage_rows(const Act act, int n, int nt, int k0, in
             const int c = (part + (i << log_shared)) * 128 + lane * 4;
             raw[i] = by[i] = make_uint4(0, 0, 0, 0);
             if (live && c < columns) {
-                raw[i] = load4<true>(act, type, row, k0 + c);
-                if (norm) by[i] = load4<true>(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
+                raw[i] = load4(act, type, row, k0 + c);
+                if (norm) by[i] = load4(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
             }
         }
         float v[kHeld][4];
@@ -435,7 +431,7 @@ __device__ __noinline__ void stage_rows(const Act act, int n, int nt, int k0, in
             uint4 by = {};
             const int c = step * 128 + lane * 4;
             if (norm_staged) by = shared_u4(room.at(step) + lane * 16);
-            else if (c < columns) by = load4<true>(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
+            else if (c < columns) by = load4(Act{norm, 0, GGML_F32, norm_vec}, GGML_F32, 0, k0 + c);
             v[0] *= __uint_as_float(by.x); v[1] *= __uint_as_float(by.y); v[2] *= __uint_as_float(by.z); v[3] *= __uint_as_float(by.w);
         }
     };
