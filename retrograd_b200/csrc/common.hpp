@@ -39,6 +39,10 @@ template <class F> int boundary(F && body) {
     try {
         clear_error();
         return body();
+    } catch (const CudaError & err) {
+        set_error(err.what());
+        cudaGetLastError();     // reported here: the thread's next call does not find it
+        return STATUS_RUNTIME;
     } catch (const std::exception & err) {
         set_error(err.what());
         return STATUS_RUNTIME;

@@ -48,9 +48,8 @@ int refuse(const char * op, const std::string & why) {
 }
 
 int launched(const char * op, cudaError_t status) {
-    if (status == cudaSuccess) status = cudaGetLastError();
-    else cudaGetLastError();
     if (status == cudaSuccess) return STATUS_OK;
+    cudaGetLastError();         // this call's own failure; one that the thread holds from elsewhere is no business of a launch that succeeded
     set_error(std::string(op) + ": launch failed: " + cudaGetErrorString(status));
     return STATUS_RUNTIME;
 }
