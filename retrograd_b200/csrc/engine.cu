@@ -160,7 +160,7 @@ void Engine::load_model(const std::string & path) {
         const uint32_t type = stored(names[0]).type;
         for (const std::string & name : names)
             if (stored(name).type != type) return;
-        if ((type != GGML_Q4_0 && type != GGML_MXFP4) || n_in > kW4MaxColumns || n_expert > kW4MaxExperts) return;
+        if (!w4::check_weights(type, n_out, n_in, n_expert).empty()) return;      // the other kernels serve every step
         size_t total = 0;
         for (const std::string & name : names) total += stored(name).n_bytes;
         struct Raw { uint8_t * p = nullptr; ~Raw() { if (p) cudaFree(p); } } raw;
@@ -178,7 +178,7 @@ void Engine::load_model(const std::string & path) {
         RB_CUDA(cudaMalloc(&units, bytes));
         m.allocations.push_back(units);
         RB_CUDA(cudaDeviceSynchronize());       // the blocking uploads have reached the device
-        launch_w4_retile(raw.p, type, (uint32_t)n_out, (uint32_t)n_in, n_expert, static_cast<uint8_t *>(units), d_max, stream);
+        RB_CUDA(launch_w4_retile(raw.p, type, (uint32_t)n_out, (uint32_t)n_in, n_expert, static_cast<uint8_t *>(units), d_max, stream));
         int h_max = 0;
         RB_CUDA(cudaMemcpyAsync(&h_max, d_max, sizeof h_max, cudaMemcpyDeviceToHost, stream));
         RB_CUDA(cudaStreamSynchronize(stream));

@@ -1832,12 +1832,13 @@ W4View w4_view(const uint8_t * units, uint32_t type, uint32_t n_out, uint32_t n_
     return v;
 }
 
-void launch_w4_retile(const uint8_t * rows, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert, uint8_t * units, int * max_scale,
-                      cudaStream_t stream) {
+cudaError_t launch_w4_retile(const uint8_t * rows, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert, uint8_t * units, int * max_scale,
+                             cudaStream_t stream) {
     const W4View v = w4_view(units, type, n_out, n_in, n_expert);
     const size_t n = (size_t)n_expert * v.blocks * v.steps;
     if (type == GGML_MXFP4) w4_retile_kernel<true><<<(unsigned)n, 256, 0, stream>>>(rows, n_out, n_in, v.blocks, v.steps, units, max_scale);
     else w4_retile_kernel<false><<<(unsigned)n, 256, 0, stream>>>(rows, n_out, n_in, v.blocks, v.steps, units, max_scale);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_w4_product(const W4Product & p, cudaStream_t stream) {

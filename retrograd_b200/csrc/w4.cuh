@@ -3,6 +3,8 @@
 // MXFP4 (w = 2^(s - 127) e2m1(q), s a byte).
 #pragma once
 
+#include "w4_checks.hpp"
+
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -10,8 +12,6 @@
 namespace rb200 {
 
 constexpr int kW4PassTokens = 16;            // tokens one launch serves; longer calls run pass by pass
-constexpr uint32_t kW4MaxColumns = 262144;   // longest row: one token's activations of an eighth of it fit in shared memory
-constexpr uint32_t kW4MaxExperts = 256;
 constexpr uint32_t kW4MaxUsed = 32;          // experts per token
 constexpr uint32_t kW4MaxScaleByte = 207;    // MXFP4: weight scales up to 2^80, so that a row's scaled sum stays inside f32
 
@@ -34,9 +34,9 @@ struct W4View {
 
 size_t w4_bytes(uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert);
 // Lays GGUF rows [expert][row][blocks] (device memory) out as units. *max_scale (device, zeroed by the caller) becomes the
-// largest MXFP4 scale byte; untouched for Q4_0.
-void launch_w4_retile(const uint8_t * rows, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert, uint8_t * units, int * max_scale,
-                      cudaStream_t stream);
+// largest MXFP4 scale byte; untouched for Q4_0. For shapes that w4::check_weights admits.
+cudaError_t launch_w4_retile(const uint8_t * rows, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert, uint8_t * units, int * max_scale,
+                             cudaStream_t stream);
 W4View w4_view(const uint8_t * units, uint32_t type, uint32_t n_out, uint32_t n_in, uint32_t n_expert);
 
 // Activations: f32, f16 or bf16 rows (GGML type codes); results: the same choice.

@@ -99,12 +99,9 @@ retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_
     retro_b200_w4 * made = nullptr;
     boundary([&]() -> int {
         const char * op = "w4_new";
-        if (ggml_type != GGML_Q4_0 && ggml_type != GGML_MXFP4) return refuse(op, "the weights must be Q4_0 (2) or MXFP4 (39)");
         if (!rows) return refuse(op, "rows are required");
-        if (n_out == 0 || n_in == 0 || n_in % 32 != 0) return refuse(op, "n_out must be at least 1 and n_in a multiple of 32");
-        if (n_in > kW4MaxColumns) return refuse(op, "n_in is larger than 262144");
-        if (n_expert == 0 || n_expert > kW4MaxExperts) return refuse(op, "n_expert must be 1 to 256");
-        if ((uint64_t)n_expert * (((uint64_t)n_out + 31) / 32) * ((n_in + 127) / 128) > 0x7fffffffull) return refuse(op, "the bank is too large");
+        const std::string why = w4::check_weights(ggml_type, n_out, n_in, n_expert);
+        if (!why.empty()) return refuse(op, why);
         auto w = std::make_unique<retro_b200_w4>();
         RB_CUDA(cudaGetDevice(&w->device));
         w->bytes = w4_bytes(ggml_type, n_out, n_in, n_expert);
@@ -120,8 +117,7 @@ retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_
         RB_CUDA(cudaMemcpy(raw.p, rows, n_raw, cudaMemcpyDefault));
         RB_CUDA(cudaDeviceSynchronize());       // the blocking copy has reached the device before another stream reads it
         RB_CUDA(cudaMemsetAsync(d_max, 0, sizeof(int), raw.s));
-        launch_w4_retile(raw.p, ggml_type, n_out, n_in, n_expert, w->units, d_max, raw.s);
-        RB_CUDA(cudaGetLastError());
+        RB_CUDA(launch_w4_retile(raw.p, ggml_type, n_out, n_in, n_expert, w->units, d_max, raw.s));
         int h_max = 0;
         RB_CUDA(cudaMemcpyAsync(&h_max, d_max, sizeof h_max, cudaMemcpyDeviceToHost, raw.s));
         RB_CUDA(cudaStreamSynchronize(raw.s));

@@ -9,7 +9,21 @@
 #include <string>
 
 namespace rb200 {
+
+constexpr uint32_t kW4MaxColumns = 262144;   // longest row: one token's activations of an eighth of it fit in shared memory
+constexpr uint32_t kW4MaxExperts = 256;
+
 namespace w4 {
+
+// What the kernels hold as weights: an empty text, or why not. (A grid counts the units of a bank, an int its rows.)
+inline std::string check_weights(uint32_t ggml_type, uint64_t n_out, uint64_t n_in, uint64_t n_expert) {
+    if (ggml_type != GGML_Q4_0 && ggml_type != GGML_MXFP4) return "the weights must be Q4_0 (2) or MXFP4 (39)";
+    if (n_out == 0 || n_in == 0 || n_in % 32 != 0) return "n_out must be at least 1 and n_in a multiple of 32";
+    if (n_in > kW4MaxColumns) return "n_in is larger than 262144";
+    if (n_expert == 0 || n_expert > kW4MaxExperts) return "n_expert must be 1 to 256";
+    if (n_out > 0x7fffffe0ull || n_expert * ((n_out + 31) / 32) * ((n_in + 127) / 128) > 0x7fffffffull) return "the bank is too large";
+    return "";
+}
 
 constexpr uint32_t kMaxTokens = 1u << 24;
 
