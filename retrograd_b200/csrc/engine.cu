@@ -90,6 +90,15 @@ void q4_0_to_q8_0(const void * src, size_t bytes, std::vector<uint8_t> & out) {
     }
 }
 
+// Frees the few-token units of an expert bank.
+static void drop_w4(Model & m, WeightView & w) {
+    if (!w.w4) return;
+    m.tiled_bytes -= w4_bytes(w.w4_type, w.n_out, w.n_in, m.hp.n_expert);
+    m.allocations.erase(std::find(m.allocations.begin(), m.allocations.end(), (void *)w.w4));
+    RB_CUDA(cudaFree(const_cast<uint8_t *>(w.w4)));
+    w.w4 = nullptr;
+}
+
 void Engine::load_model(const std::string & path) {
     if (const char * env = std::getenv("RB200_MOE")) {
         moe_tensor_cores_ = std::string(env) != "rows";
@@ -382,6 +391,9 @@ void Engine::load_model(const std::string & path) {
                 attach_w4(lw.gate_exps, {p + "ffn_gate_exps.weight"}, hp.d, hp.ff, hp.n_expert);
                 attach_w4(lw.up_exps, {p + "ffn_up_exps.weight"}, hp.d, hp.ff, hp.n_expert);
                 attach_w4(lw.down_exps, {p + "ffn_down_exps.weight"}, hp.ff, hp.d, hp.n_expert);
+                // a layer runs on all three or on none
+                if (!lw.gate_exps.w4 || !lw.up_exps.w4 || !lw.down_exps.w4)
+                    for (WeightView * w : {&lw.gate_exps, &lw.up_exps, &lw.down_exps}) drop_w4(m, *w);
             }
             // the inventory entry of each bank, as the file holds it (retro_experts.cpp:86-131: role = the
             // name's stem without "ffn_" and "_exps")
@@ -584,7 +596,8 @@ Engine::Engine(const std::string & path, const retro_engine_config & cfg) : conf
         moe_offsets_.ensure(hp.n_expert + 1);
         moe_sorted_.ensure(P);
         moe_w_.ensure(P);
-        w4_workspace_.ensure(w4_moe_workspace_bytes(hp.ff, kW4PassTokens, hp.n_expert_used));
+        if (std::any_of(model->layers.begin(), model->layers.end(), [](const LayerWeights & lw) { return lw.gate_exps.w4 != nullptr; }))
+            w4_workspace_.ensure(w4_moe_workspace_bytes(hp.ff, kW4PassTokens, hp.n_expert_used));
         pair_gu_.ensure(P * 2 * hp.ff);
         pair_h_.ensure(P * hp.ff);
         pair_y_.ensure(P * hp.d);
@@ -1042,13 +1055,7 @@ void Engine::ep_keep_local_experts() {
         ep_local_bank_bytes_ += per * per_expert;
     };
     for (LayerWeights & lw : m.layers) {
-        for (WeightView * w : {&lw.gate_exps, &lw.up_exps, &lw.down_exps}) {        // the exchanged pairs run on the other kernels
-            if (!w->w4) continue;
-            m.tiled_bytes -= w4_bytes(w->w4_type, w->n_out, w->n_in, m.hp.n_expert);
-            m.allocations.erase(std::find(m.allocations.begin(), m.allocations.end(), (void *)w->w4));
-            RB_CUDA(cudaFree(const_cast<uint8_t *>(w->w4)));
-            w->w4 = nullptr;
-        }
+        for (WeightView * w : {&lw.gate_exps, &lw.up_exps, &lw.down_exps}) drop_w4(m, *w);       // the exchanged pairs run on the other kernels
         keep(lw.gate_exps, lw.gate_stride);
         keep(lw.up_exps, lw.up_stride);
         keep(lw.down_exps, lw.down_stride);
@@ -1722,7 +1729,7 @@ int Engine::step(const EffRow * rows, size_t n_rows, OutRow * out_rows, int32_t 
         const bool ffn_normed = linear(lw.wo, att_.ptr, dq, Ti, x_.ptr, d, nullptr, x_.ptr, d, att_split_.get(), any_adapter ? nullptr : &ffn_norm_tail);
         if (any_adapter) lora(p + "attn_output.weight", att_.ptr, dq, Ti, x_.ptr, d);
         const bool ffn_glu = !any_adapter && hp.n_expert == 0 && lw.wgu.data && w4_serves(lw.wgu, Ti) && ff % 32 == 0;
-        const bool experts_w4 = hp.n_expert != 0 && !ep_comm_ && w4_serves(lw.gate_exps, Ti) && lw.up_exps.w4 && lw.down_exps.w4;
+        const bool experts_w4 = hp.n_expert != 0 && !ep_comm_ && w4_serves(lw.gate_exps, Ti);
         if (!ffn_normed && !ffn_glu && !experts_w4)
             RB_K(K_OTHER, 1, launch_rms_norm(x_.ptr, d, nullptr, lw.ffn_norm, d, hp.eps, gu_split ? nullptr : xn_.ptr, d, Ti, stream, xn_split_.get()));
         if (hp.n_expert == 0) {
@@ -2346,7 +2353,7 @@ uint64_t Engine::work_buffer_bytes() const {
     uint64_t total = 0;
     auto add = [&](const auto & buffer) { total += (uint64_t)buffer.count * sizeof(*buffer.ptr); };
     add(block_table_); add(maps_store_); add(d_stage_); add(d_result_); add(x_); add(xn_); add(qkv_); add(att_); add(gu_); add(hff_); add(hs_);
-    add(router_logits_); add(moe_w_); add(pair_gu_); add(pair_h_); add(pair_y_); add(lora_tmp_); add(logits_work_); add(logits); add(route_ids);
+    add(router_logits_); add(moe_w_); add(pair_gu_); add(pair_h_); add(pair_y_); add(w4_workspace_); add(lora_tmp_); add(logits_work_); add(logits); add(route_ids);
     add(moe_ids_); add(d_aux_); add(moe_offsets_); add(moe_sorted_); add(lora_offsets_); add(lora_sorted_); add(stream_scratch_);
     add(sample_scratch_); add(attn_scratch_); add(moe_xs_); add(moe_gu_s_); add(moe_y_s_); add(ep_all_offsets_); add(ep_offsets_l_);
     add(ep_sorted_l_); add(ep_send_); add(ep_recv_); add(ep_gu_); add(ep_h_); add(ep_y_); add(ep_back_);

@@ -23,3 +23,22 @@ def test_a_failed_allocation_is_not_the_next_calls_error(rb, c1_model):
     assert not too_large()
     engine.step([rb.StepRow(0, 0, [5, 9, 3], 0, sample=True, sampling=rb.SamplingParamsV2.greedy())], rb.StepOutput())
     engine.close()
+
+
+MOE = dict(arch="olmoe", layers=2, d=192, heads=4, kv_heads=4, vocab=600, experts=12, experts_used=3, dtype="q8_0", seed=34)
+
+
+def test_the_memory_report_counts_the_expert_layers_units_and_workspace(rb, models):
+    """Q4_0 banks are held as Q8_0 rows and, where a layer runs on the few-token kernels, as units with a workspace. A down bank whose rows are no
+    multiple of 32 is stored as F16: then nothing is held for those kernels."""
+    def report(ff, dtype):
+        engine = rb.Engine(str(models(f"moe_{dtype}_{ff}", **MOE, ff=ff, expert_dtype=dtype)), rb.EngineConfig(n_ctx=64, n_seq_max=1, n_batch=32, n_ubatch=32))
+        r = engine.memory_report()
+        engine.close()
+        return r["model_weight_bytes"], r["generation_compute_bytes"]
+
+    assert report(168, "q4_0") == report(168, "q8_0")
+    (w4, c4), (w8, c8) = report(160, "q4_0"), report(160, "q8_0")
+    gate, up, down = (rb.W4Matrix(Q4_0, np.zeros(12 * n_out * n_in // 32 * 18, np.uint8), n_out, n_in, n_expert=12) for n_out, n_in in ((160, 192), (160, 192), (192, 160)))
+    assert w4 - w8 == MOE["layers"] * (gate.nbytes + up.nbytes + down.nbytes)
+    assert c4 - c8 == rb.w4_moe_workspace(gate, 16, MOE["experts_used"])
