@@ -21,8 +21,8 @@ def _torch():
 
     global _raw_stream
     if not _TYPES:
-        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})      # last: another thread takes a filled table for all of it
     return torch
 
 
