@@ -1,7 +1,9 @@
 """Products with 4-bit weights for few tokens (`retro_b200_w4_*` in include/retro_b200.h) on torch CUDA tensors.
 
 The tensors' memory goes to the library as it is: rows may be strided, calls run on the current stream of the tensors' device
-(or the one given) and can be captured into a CUDA graph.
+(or the one given, as a torch stream or its handle) and can be captured into a CUDA graph. A call on a given stream does not order it behind
+the current one: the caller does, before the call for its operands and behind it for the result. Operands may be dropped
+at once, their memory is not handed out again before the call is done.
 """
 from __future__ import annotations
 
@@ -114,13 +116,29 @@ def _open(op: str, *matrices) -> int:
     return matrices[0].device
 
 
+def _other(stream, device: int):
+    """The stream a call is given, as torch's object, when it is not the current one."""
+    if stream is None or getattr(stream, "cuda_stream", stream) == _raw_stream(device):
+        return None
+    return stream if hasattr(stream, "cuda_stream") else _torch().cuda.ExternalStream(stream, device=device)
+
+
 def _new(make, stream, device: int):
     """The tensor that make() makes, on the stream the call runs on: the allocator hands its memory to no other stream before."""
-    if stream is None or getattr(stream, "cuda_stream", stream) == _raw_stream(device):
+    other = _other(stream, device)
+    if other is None:
         return make()
-    torch = _torch()
-    with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=device)):
+    with _torch().cuda.stream(other):
         return make()
+
+
+def _used(stream, device: int, *tensors) -> None:
+    """Tells the allocator that a call used these on `stream`: it hands their memory out again only behind that."""
+    other = _other(stream, device)
+    if other is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(other)
 
 
 def _result(op: str, x, tx: int, out, tokens: int, width: int, device: int, stream):
@@ -160,6 +178,8 @@ def w4_matvec(w: W4Matrix, x, *, norm=None, eps: float = 1e-5, bias=None, residu
                                              None if bias is None else _vector("w4_matvec", "bias", bias, w.n_out, device), pr, ldr, py, ty, ldy, _stream(stream, device))
         if status:
             _check(status)
+        if stream is not None:
+            _used(stream, device, x, norm, bias, residual, out)
     return y
 
 
@@ -175,6 +195,8 @@ def w4_glu(gate: W4Matrix, up: W4Matrix, x, *, norm=None, eps: float = 1e-5, out
                                              _stream(stream, device))
         if status:
             _check(status)
+        if stream is not None:
+            _used(stream, device, x, norm, out)
     return y
 
 
@@ -198,7 +220,7 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
             raise InvalidArgument(f"w4_moe: {name} must be contiguous {dtype} [{tokens}, {n_used}] on the weights' device")
     if not tokens:
         return y
-    on = _stream(stream, device)
+    on, given = _stream(stream, device), workspace
     if workspace is None:
         need = w4_moe_workspace(gate, tokens, n_used)
         workspace = _new(lambda: torch.empty(need, dtype=torch.uint8, device=x.device), stream, device)
@@ -208,6 +230,8 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
                                        normalise, _vector("w4_moe", "norm", norm, n_in, device), eps, pr, ldr, py, ty, ldy,
                                        None if ids is None else ids.data_ptr(), None if weights is None else weights.data_ptr(),
                                        workspace.data_ptr(), workspace.numel() * workspace.element_size(), on))
+    if stream is not None:
+        _used(stream, device, router, x, norm, residual, out, ids, weights, given)
     return y
 
 

@@ -42,3 +42,36 @@ def test_the_memory_report_counts_the_expert_layers_units_and_workspace(rb, mode
     gate, up, down = (rb.W4Matrix(Q4_0, np.zeros(12 * n_out * n_in // 32 * 18, np.uint8), n_out, n_in, n_expert=12) for n_out, n_in in ((160, 192), (160, 192), (192, 160)))
     assert w4 - w8 == MOE["layers"] * (gate.nbytes + up.nbytes + down.nbytes)
     assert c4 - c8 == rb.w4_moe_workspace(gate, 16, MOE["experts_used"])
+
+
+@pytest.mark.parametrize("handle", [False, True])
+def test_operands_of_a_call_on_another_stream_may_be_dropped_at_once(rb, handle):
+    """The call waits on its stream while its operands are dropped and tensors of their sizes are made: those get other memory."""
+    import torch
+
+    rng = np.random.default_rng(2)
+    make = lambda n_out, n_in, E=1: rb.W4Matrix(Q4_0, np.concatenate([stored_rows(rng, Q4_0, n_out, n_in) for _ in range(E)]), n_out, n_in, n_expert=E)
+    m, up, gates, ups, downs = make(512, 512), make(512, 512), make(64, 512, 4), make(64, 512, 4), make(512, 64, 4)
+    side = torch.cuda.Stream()
+    base = {"x": torch.randn(4, 512, device="cuda"), "norm": torch.randn(512, device="cuda"), "bias": torch.randn(512, device="cuda"),
+            "residual": torch.randn(4, 512, device="cuda"), "router": torch.randn(4, 512, device="cuda")}
+    calls = {
+        "matvec": (("x", "norm", "bias", "residual"), lambda o, s: rb.w4_matvec(m, o["x"], norm=o["norm"], bias=o["bias"], residual=o["residual"], stream=s)),
+        "glu": (("x", "norm"), lambda o, s: rb.w4_glu(m, up, o["x"], norm=o["norm"], stream=s)),
+        "moe": (("x", "norm", "residual", "router"), lambda o, s: rb.w4_moe(o["router"], gates, ups, downs, o["x"], 2, norm=o["norm"], residual=o["residual"], stream=s)),
+    }
+    for names, call in calls.values():
+        want = call(base, None)
+        torch.cuda.synchronize()
+        operands = {name: base[name].clone() for name in names}
+        at = {name: t.data_ptr() for name, t in operands.items()}
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)
+        y = call(operands, side.cuda_stream if handle else side)
+        shapes = [base[name].shape for name in names]
+        operands.clear()
+        fresh = [torch.zeros(shape, device="cuda") for shape in shapes for _ in range(3)]
+        assert not {t.data_ptr() for t in fresh} & set(at.values())
+        side.synchronize()
+        assert torch.equal(y, want)
