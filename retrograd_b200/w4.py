@@ -3,7 +3,8 @@
 The tensors' memory goes to the library as it is: rows may be strided, calls run on the current stream of the tensors' device
 (or the one given, as a torch stream or its handle) and can be captured into a CUDA graph. A call on a given stream does not order it behind
 the current one: the caller does, before the call for its operands and behind it for the result. Operands may be dropped
-at once, their memory is not handed out again before the call is done.
+at once, their memory is not handed out again before the call is done. There is no backward pass: where gradients are recorded, an
+operand that requires one is refused.
 """
 from __future__ import annotations
 
@@ -16,13 +17,15 @@ from .engine import EngineError, InvalidArgument, _check, _last_error
 
 _TYPES: dict = {}       # torch dtype -> GGML type code
 _raw_stream = None      # current stream handle of a device
+_recording = None       # whether gradients are recorded
 
 
 def _torch():
     import torch
 
-    global _raw_stream
+    global _raw_stream, _recording
     if not _TYPES:
+        _recording = torch.is_grad_enabled
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
         _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})      # last: another thread takes a filled table for all of it
     return torch
@@ -83,6 +86,11 @@ class W4Matrix:
             pass
 
 
+def _no_backward(op: str, name: str) -> None:
+    if _recording():
+        raise InvalidArgument(f"{op}: {name} requires a gradient, but there is no backward pass: call it under torch.no_grad()")
+
+
 def _rows(op: str, name: str, t, width: int, device: int, tokens: int = -1):
     """Pointer, type code and row stride of a [tokens, width] tensor."""
     code = _TYPES.get(t.dtype)
@@ -96,6 +104,8 @@ def _rows(op: str, name: str, t, width: int, device: int, tokens: int = -1):
     ld, inner = t.stride()
     if inner != 1 and width > 1:
         raise InvalidArgument(f"{op}: the elements of a row of {name} must be consecutive")
+    if t.requires_grad:
+        _no_backward(op, name)
     return t.data_ptr(), code, ld
 
 
@@ -104,6 +114,8 @@ def _vector(op: str, name: str, t, n: int, device: int):
         return None
     if _TYPES.get(t.dtype) != 0 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
         raise InvalidArgument(f"{op}: {name} must be {n} consecutive float32 on the weights' device")
+    if t.requires_grad:
+        _no_backward(op, name)
     return t.data_ptr()
 
 

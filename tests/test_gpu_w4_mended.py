@@ -75,3 +75,28 @@ def test_operands_of_a_call_on_another_stream_may_be_dropped_at_once(rb, handle)
         assert not {t.data_ptr() for t in fresh} & set(at.values())
         side.synchronize()
         assert torch.equal(y, want)
+
+
+def test_operands_that_require_a_gradient_are_refused_where_one_is_recorded(rb):
+    import torch
+
+    rng = np.random.default_rng(3)
+    make = lambda n_out, n_in, E=1: rb.W4Matrix(Q4_0, np.concatenate([stored_rows(rng, Q4_0, n_out, n_in) for _ in range(E)]), n_out, n_in, n_expert=E)
+    m, up, gates, ups, downs = make(64, 64), make(64, 64), make(32, 64, 2), make(32, 64, 2), make(64, 32, 2)
+    plain = {"x": torch.randn(2, 64, device="cuda"), "norm": torch.randn(64, device="cuda"), "bias": torch.randn(64, device="cuda"),
+             "residual": torch.randn(2, 64, device="cuda"), "router": torch.randn(2, 64, device="cuda"), "out": torch.empty(2, 64, device="cuda")}
+    calls = {
+        ("x", "norm", "bias", "residual", "out"): lambda o: rb.w4_matvec(m, o["x"], norm=o["norm"], bias=o["bias"], residual=o["residual"], out=o["out"]),
+        ("x", "norm", "out"): lambda o: rb.w4_glu(m, up, o["x"], norm=o["norm"], out=o["out"]),
+        ("router", "x", "norm", "residual", "out"): lambda o: rb.w4_moe(o["router"], gates, ups, downs, o["x"], 1, norm=o["norm"], residual=o["residual"], out=o["out"]),
+    }
+    for names, call in calls.items():
+        want = call(plain).clone()
+        for name in names:
+            operands = {**plain, name: plain[name].clone().requires_grad_()}
+            with pytest.raises(rb.InvalidArgument, match=f"{name} requires a gradient"):
+                call(operands)
+            for quiet in (torch.no_grad, torch.inference_mode):
+                with quiet():
+                    assert torch.equal(call(operands), want)
+            assert operands[name].grad is None
