@@ -505,7 +505,8 @@ int retro_b200_gemm_q4k_noalloc(const uint8_t * d_w, uint32_t n_out, uint32_t n_
  * or NULL) and do not wait, allocate or synchronise, so they may be captured into a CUDA graph. Element types: f32 (0), f16 (1), bf16 (30); x and y choose their own, a residual has
  * y's. Row strides are in elements and free (x's may be 0). Vectors (norm, bias) and the router are f32. Any number of tokens: sixteen per
  * pass over the weights. Sums are f32 of exact products with the activations (with norm: x times norm, in f32) at 22 bits or more of the largest in some
- * thousand columns; magnitudes above 2^113 count as infinite, and where the squares of a row overflow f32 its norm is zero, as f32 gives it. Results are the
+ * thousand columns; a magnitude of 65520 x 2^100 (just below 2^116) or more counts as infinite, of an expert's hidden columns too, and where the squares of a
+ * row overflow f32 its norm is zero, as f32 gives it. Results are the
  * same in every run and do not depend on the other tokens' values, but for w4_moe the last bits, whose sums are cut where the tokens' choices put it.
  * A token that holds an infinity or a NaN gets NaN or infinity, the other tokens do not.
  * -3 and a message, with nothing enqueued, for a missing or misaligned pointer, another type, a y row stride below a row, and a y that overlaps an input

@@ -201,7 +201,8 @@ template <int WARPS> struct Scratch {
 };
 
 // 2^shift brings the magnitude with these bits into [2^13, 2^14), as far as it and the factor that takes it back (2^-8 - shift for MXFP4) are
-// normal f32: below 2^-104 the values only come near, and are off by 2^-143 at most; above 2^113 they count as infinite. Rows with an infinity or a NaN are left as they are: their own
+// normal f32: below 2^-104 the values only come near, and are off by 2^-143 at most; above 2^113 the shift stays at -100, and from 65520 2^100 on, what an f16 rounds to
+// infinity, they count as infinite. Rows with an infinity or a NaN are left as they are: their own
 // sums become NaN, those of the other tokens stay what they are.
 __device__ __forceinline__ int shift_for(uint32_t top) { return top > 0 && top < 0x7f800000u ? max(-100, min(118, 140 - (int)(top >> 23))) : 0; }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_w4 import Q4_0, stored_rows
+from test_gpu_w4 import MXFP4, Q4_0, decode, dtype_of, f32_bound, stored_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,35 @@ def test_operands_that_require_a_gradient_are_refused_where_one_is_recorded(rb):
                 with quiet():
                     assert torch.equal(call(operands), want)
             assert operands[name].grad is None
+
+
+@pytest.mark.parametrize("kind", [Q4_0, MXFP4])
+@pytest.mark.parametrize("tokens", [1, 2, 6, 16])
+def test_the_largest_magnitudes(rb, kind, tokens):
+    """Up to the largest f32 below 65520 2^100 a token's results are the definition's, from there on none is finite; other tokens keep theirs. Under a norm
+    whose squares overflow f32 the rows are zeros up to the same limit. Bounds as in test_gpu_w4.py."""
+    import torch
+
+    rng = np.random.default_rng(tokens + kind)
+    n_in = 224
+    raw = stored_rows(rng, kind, 90, n_in, scale_spread=1)
+    w, mag = decode(kind, raw)
+    m = rb.W4Matrix(kind, raw, 90, n_in)
+    limit = np.float32(65520 * 2.0 ** 100)
+    plain = rng.normal(0, 1, (tokens, n_in)).clip(-0.9, 0.9).astype(np.float32)
+    for top in (np.float32(2.0 ** 112), np.float32(2.0 ** 113), np.float32(1.5 * 2.0 ** 114), np.nextafter(limit, np.float32(0))):
+        x = plain.copy()
+        x[tokens // 2] *= top
+        x[tokens // 2, 5] = top
+        x64 = x.astype(np.float64)
+        y = rb.w4_matvec(m, torch.tensor(x).cuda()).double().cpu().numpy()
+        assert (np.abs(y - x64 @ w.T) <= f32_bound(n_in) * (np.abs(x64) @ mag.T)).all(), top
+        assert (rb.w4_matvec(m, torch.tensor(x).cuda(), norm=torch.ones(n_in, device="cuda"))[tokens // 2] == 0).all(), top
+    want = rb.w4_matvec(m, torch.tensor(plain).cuda())
+    others = [t for t in range(tokens) if t != tokens // 2]
+    for top, act in ((limit, "f32"), (np.float32(2.0 ** 120), "f32"), (np.float32(3e38), "f32"), (np.float32(2.0 ** 116), "bf16")):
+        x = torch.tensor(plain).to(dtype_of(torch, act)).cuda()
+        base = rb.w4_matvec(m, x) if act == "bf16" else want
+        x[tokens // 2, 5] = float(top)
+        y = rb.w4_matvec(m, x)
+        assert not torch.isfinite(y[tokens // 2]).any() and torch.equal(y[others], base[others]), top
