@@ -132,3 +132,15 @@ def test_the_largest_magnitudes(rb, kind, tokens):
         x[tokens // 2, 5] = float(top)
         y = rb.w4_matvec(m, x)
         assert not torch.isfinite(y[tokens // 2]).any() and torch.equal(y[others], base[others]), top
+
+
+@pytest.mark.parametrize("n_out,n_in,tokens", [(40, 32, 1), (129, 992, 5), (64, 4096, 17)])
+def test_the_row_kernel_on_stored_q4_0_rows(rb, n_out, n_in, tokens):
+    """gemm_rows_kernel, which serves every stored type: sums of n_in f32 products in any order, each product and its weight rounded once."""
+    rng = np.random.default_rng(n_in)
+    raw = stored_rows(rng, Q4_0, n_out, n_in)
+    w, _ = decode(Q4_0, raw)
+    x = rng.normal(0, 1, (tokens, n_in)).astype(np.float32)
+    y, _ = rb.op_gemm(Q4_0, raw, n_out, n_in, x, path=1)
+    x64 = x.astype(np.float64)
+    assert (np.abs(y - x64 @ w.T) <= (n_in + 2) * 2.0 ** -24 * (np.abs(x64) @ np.abs(w).T)).all()
