@@ -105,19 +105,25 @@ retro_b200_w4 * retro_b200_w4_new(uint32_t ggml_type, const void * rows, uint32_
         auto w = std::make_unique<retro_b200_w4>();
         RB_CUDA(cudaGetDevice(&w->device));
         w->bytes = w4_bytes(ggml_type, n_out, n_in, n_expert);
-        RB_CUDA(cudaMalloc(&w->units, w->bytes));
+        RB_CUDA(cudaMalloc(&w->units, w->bytes + sizeof(int)));
         w->view = w4_view(w->units, ggml_type, n_out, n_in, n_expert);
-        // The stored rows, once, in device memory whatever kind of memory they come from.
-        const size_t n_raw = (size_t)n_expert * n_out * (n_in / 32) * (ggml_type == GGML_Q4_0 ? 18 : 17);
+        int * d_max = reinterpret_cast<int *>(w->units + w->bytes);     // the largest scale byte, behind the units
         struct Raw { uint8_t * p = nullptr; cudaStream_t s = nullptr; ~Raw() { if (p) cudaFree(p); if (s) cudaStreamDestroy(s); } } raw;
-        RB_CUDA(cudaMalloc(&raw.p, n_raw + 256));
         RB_CUDA(cudaStreamCreateWithFlags(&raw.s, cudaStreamNonBlocking));
-        int * d_max = reinterpret_cast<int *>(raw.p + (n_raw + 15) / 16 * 16);
-        RB_CUDA(cudaDeviceSynchronize());       // device rows that another stream is still writing
-        RB_CUDA(cudaMemcpy(raw.p, rows, n_raw, cudaMemcpyDefault));
-        RB_CUDA(cudaDeviceSynchronize());       // the blocking copy has reached the device before another stream reads it
+        // Rows that are in this device's memory are read where they are, others are copied there first. (128256 x 4096, Q4_0, rows on
+        // the device: 1.1 ms the call, 0.42 ms of it the layout kernel; 1.9 ms with a copy of them and a second wait. The same rows on the host: 29 ms.)
+        const size_t n_raw = (size_t)n_expert * n_out * (n_in / 32) * (ggml_type == GGML_Q4_0 ? 18 : 17);
+        cudaPointerAttributes from{};
+        RB_CUDA(cudaPointerGetAttributes(&from, rows));
+        const uint8_t * d_rows = static_cast<const uint8_t *>(rows);
+        RB_CUDA(cudaDeviceSynchronize());       // rows that some stream is still writing
+        if (from.type != cudaMemoryTypeDevice || from.device != w->device) {
+            RB_CUDA(cudaMalloc(&raw.p, n_raw));
+            RB_CUDA(cudaMemcpyAsync(raw.p, rows, n_raw, cudaMemcpyDefault, raw.s));
+            d_rows = raw.p;
+        }
         RB_CUDA(cudaMemsetAsync(d_max, 0, sizeof(int), raw.s));
-        RB_CUDA(launch_w4_retile(raw.p, ggml_type, n_out, n_in, n_expert, w->units, d_max, raw.s));
+        RB_CUDA(launch_w4_retile(d_rows, ggml_type, n_out, n_in, n_expert, w->units, d_max, raw.s));
         int h_max = 0;
         RB_CUDA(cudaMemcpyAsync(&h_max, d_max, sizeof h_max, cudaMemcpyDeviceToHost, raw.s));
         RB_CUDA(cudaStreamSynchronize(raw.s));

@@ -61,7 +61,7 @@ class W4Matrix:
         else:
             torch = _torch()
             with torch.cuda.device(device):
-                if hasattr(rows, "is_cuda") and rows.is_cuda:
+                if hasattr(rows, "is_cuda") and rows.is_cuda and rows.device.index != device:     # (the call waits for its own device)
                     torch.cuda.synchronize(rows.device)
                 h = lib.retro_b200_w4_new(ggml_type, pointer, n_out, n_in, n_expert)
         if not h:

@@ -144,3 +144,24 @@ def test_the_row_kernel_on_stored_q4_0_rows(rb, n_out, n_in, tokens):
     y, _ = rb.op_gemm(Q4_0, raw, n_out, n_in, x, path=1)
     x64 = x.astype(np.float64)
     assert (np.abs(y - x64 @ w.T) <= (n_in + 2) * 2.0 ** -24 * (np.abs(x64) @ np.abs(w).T)).all()
+
+
+@pytest.mark.parametrize("kind", [Q4_0, MXFP4])
+def test_rows_on_the_device_are_read_where_they_are(rb, kind):
+    """At any address, and behind a stream that is still writing them when the handle is made; they may be overwritten as soon as it is there."""
+    import torch
+
+    rng = np.random.default_rng(kind)
+    raw = stored_rows(rng, kind, 70, 416)
+    x = torch.randn(3, 416, device="cuda")
+    want = rb.w4_matvec(rb.W4Matrix(kind, raw, 70, 416), x)
+    source, side = torch.tensor(raw).cuda().view(-1), torch.cuda.Stream()
+    for offset in (0, 1, 2, 7, 16):
+        place = torch.zeros(source.numel() + offset, dtype=torch.uint8, device="cuda")[offset:]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            place.copy_(source)
+        m = rb.W4Matrix(kind, place, 70, 416)
+        place.zero_()
+        assert torch.equal(rb.w4_matvec(m, x), want), offset
