@@ -19,8 +19,8 @@
 // ahead, so that no registers are held by loads in flight. Up to four tokens run as three CTAs of eight warps on an SM; more
 // as one of sixteen, because all warps of a CTA share its activations.
 //
-// Measured (replayed in a graph, weights larger than the L2 cache), Q4_0: 128256 x 4096 at one token 56 us, 5.24 TB/s, bound by the integer pipe that
-// unpacks; 14336 x 4096 gated pair 18.7 us at one token (3.5 TB/s), 36 us at sixteen, where mma.sync with hi and lo parts is the busiest unit of the product loop
+// Measured (replayed in a graph, weights larger than the L2 cache; a call by itself is longer by up to 7 us), Q4_0: 128256 x 4096 at one token 56 us, 5.24 TB/s, bound by the integer pipe that
+// unpacks (63 us a call); 14336 x 4096 gated pair 18.7 us at one token (3.5 TB/s), 36 us at sixteen, where mma.sync with hi and lo parts is the busiest unit of the product loop
 // and staging takes 6 us; 4096 x 14336 at one token 11.4 us (2.9 TB/s), a third of it staging and the launch. MXFP4, 201088 x 2880, sixteen
 // bf16 tokens: 96 us, 3.2 TB/s. A layer of 32 experts of 2880 x 2880 (MXFP4, four used): 31 us at one token, 114 us at sixteen.
 
@@ -40,7 +40,8 @@ namespace {
 constexpr int kSlotCol = 36;        // floats per (partial slot, token) of the second expert kernel: 32 rows, padded against bank conflicts
 constexpr int kRowList = kW4PassTokens;
 constexpr int kMaxCluster = 8;
-// Warps of a CTA that serves up to n tokens, and its CTAs on an SM.
+// Warps of a CTA that serves up to n tokens, and its CTAs on an SM. (Two to four tokens on eight: 14336 x 4096
+// gated pair 21.8 to 22.2 us, where sixteen take 17.5 to 17.9 us; expert layer of 32 x 2880 x 2880 at three tokens 69 us, where they take 51 us.)
 __host__ __device__ constexpr int warps_for(int n) { return n > 4 ? 16 : 8; }
 __host__ __device__ constexpr int resident_for(int n) { return n > 4 ? 1 : 3; }
 // Units in the ring of each of its warps. For products of more than eight f32 tokens the activations and the sums need the room more (14336 x
@@ -1674,7 +1675,8 @@ template <bool MX, int PARTS, bool GLU, int NT> cudaError_t launch_product(const
     return e != cudaSuccess ? e : launch_cluster(w4_product_kernel<MX, PARTS, GLU, NT>, clusters * C, warps_for(NT) * 32, C, smem, stream, a);
 }
 
-// Room the kernels that take whole calls of n tokens stage them with: those sizes they are built for.
+// Room the kernels that take whole calls of n tokens stage them with: those sizes they are built for. (14336 x 4096 gated pair, one token: 18.7 us, 21.3 us with
+// room for four; six tokens: 24.8 us, 30.4 us with room for sixteen. Expert layer of 32 x 2880 x 2880: 30.1 and 32.2 us, 67.5 and 69.9 us.)
 int product_room(int n) { return n == 1 ? 1 : n <= 4 ? 4 : n <= 8 ? 8 : 16; }
 
 // Calls f with the room as a constant.
@@ -1760,7 +1762,8 @@ struct Cut {
 // Chooses the cluster size for `blocks` row blocks of `per` matrices and `steps` column steps whose activations take `each` bytes of
 // shared memory a step. The estimate is in clocks: the weight stream at the SM's share of the memory bandwidth, but no faster
 // than the busiest SM's warps get through it or than its copies in flight allow; the conversion of the CTA's share of the activations; the sums it
-// receives; and a barrier for every round its inbox allows. `fixed` is other dynamic shared memory, `statics` the kernel's static one.
+// receives; and a barrier for every round its inbox allows. 23.5 bytes a clock and SM and 13 MB in flight are 6.6 TB/s for two microseconds; the clocks of a unit, a
+// conversion, a sum and a barrier are fitted to measured times, not derived. `fixed` is other dynamic shared memory, `statics` the kernel's static one.
 Cut choose_cut(int blocks, int per, int steps, int n, int each, bool mx, int stages, int most_resident, int least_c, int most_c, int fixed, int statics, int sms) {
     Cut best;
     const int warps = warps_for(n), ring = ring_bytes(mx, n, stages), unit = (int)w4_unit_bytes(mx);
