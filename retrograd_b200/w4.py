@@ -18,14 +18,15 @@ from .engine import EngineError, InvalidArgument, _check, _last_error
 _TYPES: dict = {}       # torch dtype -> GGML type code
 _raw_stream = None      # current stream handle of a device
 _recording = None       # whether gradients are recorded
+_bump = None            # counts a tensor's version up
 
 
 def _torch():
     import torch
 
-    global _raw_stream, _recording
+    global _raw_stream, _recording, _bump
     if not _TYPES:
-        _recording = torch.is_grad_enabled
+        _recording, _bump = torch.is_grad_enabled, torch.autograd.graph.increment_version
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
         _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})      # last: another thread takes a filled table for all of it
     return torch
@@ -144,6 +145,13 @@ def _new(make, stream, device: int):
         return make()
 
 
+def _written(*tensors) -> None:
+    """Tells autograd that a call wrote these: a backward pass that has saved one refuses it, as after torch's own in-place operations."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            _bump(t)
+
+
 def _used(stream, device: int, *tensors) -> None:
     """Tells the allocator that a call used these on `stream`: it hands their memory out again only behind that."""
     other = _other(stream, device)
@@ -190,6 +198,8 @@ def w4_matvec(w: W4Matrix, x, *, norm=None, eps: float = 1e-5, bias=None, residu
                                              None if bias is None else _vector("w4_matvec", "bias", bias, w.n_out, device), pr, ldr, py, ty, ldy, _stream(stream, device))
         if status:
             _check(status)
+        if out is not None:
+            _written(out)
         if stream is not None:
             _used(stream, device, x, norm, bias, residual, out)
     return y
@@ -207,6 +217,8 @@ def w4_glu(gate: W4Matrix, up: W4Matrix, x, *, norm=None, eps: float = 1e-5, out
                                              _stream(stream, device))
         if status:
             _check(status)
+        if out is not None:
+            _written(out)
         if stream is not None:
             _used(stream, device, x, norm, out)
     return y
@@ -242,6 +254,7 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
                                        normalise, _vector("w4_moe", "norm", norm, n_in, device), eps, pr, ldr, py, ty, ldy,
                                        None if ids is None else ids.data_ptr(), None if weights is None else weights.data_ptr(),
                                        workspace.data_ptr(), workspace.numel() * workspace.element_size(), on))
+    _written(out, ids, weights)
     if stream is not None:
         _used(stream, device, router, x, norm, residual, out, ids, weights, given)
     return y

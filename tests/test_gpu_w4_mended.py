@@ -165,3 +165,22 @@ def test_rows_on_the_device_are_read_where_they_are(rb, kind):
         m = rb.W4Matrix(kind, place, 70, 416)
         place.zero_()
         assert torch.equal(rb.w4_matvec(m, x), want), offset
+
+
+def test_a_backward_pass_notices_that_a_call_wrote_what_it_saved(rb):
+    import torch
+
+    rng = np.random.default_rng(3)
+    make = lambda n_out, n_in, E=1: rb.W4Matrix(Q4_0, np.concatenate([stored_rows(rng, Q4_0, n_out, n_in) for _ in range(E)]), n_out, n_in, n_expert=E)
+    m, up, gates, ups, downs = make(64, 64), make(64, 64), make(32, 64, 2), make(32, 64, 2), make(64, 32, 2)
+    x, router = torch.randn(2, 64, device="cuda"), torch.randn(2, 64, device="cuda")
+    moe = lambda **kw: rb.w4_moe(router, gates, ups, downs, x, 1, **kw)
+    for shape, call in (((2, 64), lambda t: rb.w4_matvec(m, x, out=t)), ((2, 64), lambda t: rb.w4_glu(m, up, x, out=t)), ((2, 64), lambda t: moe(out=t)),
+                        ((2, 1), lambda t: moe(weights=t))):
+        saved, scale = torch.randn(shape, device="cuda"), torch.ones(shape, device="cuda", requires_grad=True)
+        loss = (saved * scale).sum()
+        call(saved)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            call(torch.randn(shape, device="cuda"))
