@@ -242,6 +242,8 @@ def w4_moe(router, gate: W4Matrix, up: W4Matrix, down: W4Matrix, x, n_used: int,
     for name, t, dtype in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
         if t is not None and (t.dtype != dtype or tuple(t.shape) != (tokens, n_used) or t.get_device() != device or not t.is_contiguous()):
             raise InvalidArgument(f"w4_moe: {name} must be contiguous {dtype} [{tokens}, {n_used}] on the weights' device")
+        if t is not None and t.requires_grad:
+            _no_backward("w4_moe", name)
     if not tokens:
         return y
     on, given = _stream(stream, device), workspace

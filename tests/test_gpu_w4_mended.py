@@ -84,11 +84,12 @@ def test_operands_that_require_a_gradient_are_refused_where_one_is_recorded(rb):
     make = lambda n_out, n_in, E=1: rb.W4Matrix(Q4_0, np.concatenate([stored_rows(rng, Q4_0, n_out, n_in) for _ in range(E)]), n_out, n_in, n_expert=E)
     m, up, gates, ups, downs = make(64, 64), make(64, 64), make(32, 64, 2), make(32, 64, 2), make(64, 32, 2)
     plain = {"x": torch.randn(2, 64, device="cuda"), "norm": torch.randn(64, device="cuda"), "bias": torch.randn(64, device="cuda"),
-             "residual": torch.randn(2, 64, device="cuda"), "router": torch.randn(2, 64, device="cuda"), "out": torch.empty(2, 64, device="cuda")}
+             "residual": torch.randn(2, 64, device="cuda"), "router": torch.randn(2, 64, device="cuda"), "out": torch.empty(2, 64, device="cuda"), "weights": torch.empty(2, 1, device="cuda")}
     calls = {
         ("x", "norm", "bias", "residual", "out"): lambda o: rb.w4_matvec(m, o["x"], norm=o["norm"], bias=o["bias"], residual=o["residual"], out=o["out"]),
         ("x", "norm", "out"): lambda o: rb.w4_glu(m, up, o["x"], norm=o["norm"], out=o["out"]),
-        ("router", "x", "norm", "residual", "out"): lambda o: rb.w4_moe(o["router"], gates, ups, downs, o["x"], 1, norm=o["norm"], residual=o["residual"], out=o["out"]),
+        ("router", "x", "norm", "residual", "out", "weights"): lambda o: rb.w4_moe(o["router"], gates, ups, downs, o["x"], 1, norm=o["norm"], residual=o["residual"], out=o["out"],
+                                                                                 weights=o["weights"]),
     }
     for names, call in calls.items():
         want = call(plain).clone()
@@ -184,3 +185,16 @@ def test_a_backward_pass_notices_that_a_call_wrote_what_it_saved(rb):
             loss.backward()
         with torch.inference_mode():
             call(torch.randn(shape, device="cuda"))
+
+
+def test_the_null_stream_by_its_handle_while_another_is_current(rb):
+    import torch
+
+    m = rb.W4Matrix(Q4_0, stored_rows(np.random.default_rng(1), Q4_0, 96, 128), 96, 128)
+    x = torch.randn(3, 128, device="cuda")
+    want = rb.w4_matvec(m, x)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        y = rb.w4_matvec(m, x, stream=0)
+        z = rb.w4_matvec(m, x, stream=torch.cuda.default_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and torch.equal(z, want)
