@@ -497,7 +497,8 @@ int retro_b200_gemm_q4k_noalloc(const uint8_t * d_w, uint32_t n_out, uint32_t n_
  * per 32 weights, 18 bytes) and MXFP4 (39: E8M0 scale per 32, 17 bytes).
  *
  * retro_b200_w4_new lays `rows` ([n_expert][n_out][n_in / 32 blocks], host or device memory, read before the call returns) out on
- * the current device, in about the same number of bytes; n_expert is 1 for a plain matrix. NULL and a message when the type is another one,
+ * the current device, in about the same number of bytes; n_expert is 1 for a plain matrix. It waits for all the device has pending, and reads rows that are in
+ * its memory where they are. NULL and a message when the type is another one,
  * n_in is no multiple of 32 or above 262144, n_expert is above 256, or an MXFP4 scale is above 2^80. The handle is immutable: calls
  * from several threads and streams may use it at once. Free it when no call that uses it is pending.
  *
